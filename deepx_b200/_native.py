@@ -25,12 +25,27 @@ SQRT, LOG, EXP, SIN, COS, TAN, INVERT = range(7)
 EQ, NE, LT, GT = range(4)
 SUM, PROD, RMAX, RMIN = range(4)
 
+CACHE_I8, CACHE_E4M3 = range(2)
+
 OK, E_DTYPE, E_SHAPE, E_ARG, E_CUDA, E_WORKSPACE, E_ALIAS, E_UNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7
 MAX_DIMS = 12
 SWITCH_MAX = 16
 
 _vp, _i, _i64, _d, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_double, C.c_float, C.c_size_t
 _pi64, _pi32, _pvp = C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_void_p)
+
+class KvCache(C.Structure):
+    """dx_kvcache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("kv_heads", _i64), ("page_tokens", _i64),
+                ("head_dim", _i64), ("format", _i)]
+
+
+class KvSeqs(C.Structure):
+    """dx_kvseqs"""
+    _fields_ = [("starts", _vp), ("lens", _vp), ("table", _vp), ("batch", _i64), ("table_cols", _i64), ("rows", _i64)]
+
+
+_pcache, _pseqs = C.POINTER(KvCache), C.POINTER(KvSeqs)
 
 # name → (restype, argtypes); every symbol include/dx_kernels.h declares
 SIGNATURES = {
@@ -78,6 +93,11 @@ SIGNATURES = {
     "dx_comm_emulated_allgather_rows": (_i, [_vp, _pvp, _i64, _i64, _vp]),
     "dx_rmsnorm": (_i, [_i, _vp, _vp, _vp, _i64, _i64, _d, _d, _vp]),
     "dx_softmax": (_i, [_i, _vp, _vp, _i64, _i64, _vp]),
+    "dx_qknorm_rope": (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp, _d, _vp, _i64, _i, _i, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "dx_kvcache_write": (_i, [_i, _vp, _i64, _vp, _i64, _pseqs, _pcache, _vp, _vp]),
+    "dx_kvcache_read": (_i, [_i, _pseqs, _pcache, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "dx_kvcache_attention_workspace_bytes": (_sz, [_i, _i64, _pseqs, _pcache, _i64]),
+    "dx_kvcache_attention": (_i, [_i, _vp, _i64, _i64, _pseqs, _pcache, _d, _i64, _i64, _vp, _i64, _vp, _sz, _vp, _vp]),
     "dx_transpose": (_i, [_i, _vp, _pi64, _i, _pi32, _vp, _vp]),
     "dx_concat": (_i, [_i, _pvp, _pi64, _i, _pi64, _i, _i, _vp, _vp]),
     "dx_broadcast_to": (_i, [_i, _vp, _pi64, _i, _pi64, _i, _vp, _vp]),

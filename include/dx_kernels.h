@@ -275,6 +275,69 @@ int dx_rmsnorm(int dtype, const void *x, const void *weight, void *out, int64_t 
                double eps, void *stream);
 int dx_softmax(int dtype, const void *x, void *out, int64_t rows, int64_t cols, void *stream);
 
+/* ---- queries and keys: norm of each head and position rotation ---------------
+ * No single function in the reference: its front end builds a norm out of single ops
+ * (front/py/deepx/nn/modules/norm/t5layernorm.py:19-23).  One pass: with `norm` each head's vector x of head_dim elements
+ * becomes weight * x / sqrt(mean(x^2) + eps) (weights of head_dim elements, NULL = left out), then its first
+ * `rotated` dimensions turn by the angles positions[t] * inv_freq[i], i < rotated/2, in the pairs (i, i + rotated/2), or
+ * (2i, 2i+1) when `interleaved`; the others pass.  float32 arithmetic, angles in float64, one rounding at the end.
+ * q is [tokens][q_heads][head_dim] with `q_stride` elements from token to token (k alike; k_heads = 0: no keys), the
+ * outputs likewise; an output may be its input (same pointer and stride).  head_dim <= DX_ROPE_MAX_DIM, `rotated` even,
+ * 0..head_dim.  positions: DX_I32 or DX_I64.  dtype: DX_F32, DX_F16, DX_BF16 (weights the same, inv_freq float32). */
+#define DX_ROPE_MAX_DIM 512
+int dx_qknorm_rope(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const void *k, int64_t k_stride, int64_t k_heads,
+                   int64_t tokens, int64_t head_dim, int norm, const void *q_weight, const void *k_weight, double eps, const float *inv_freq,
+                   int64_t rotated, int interleaved, int pos_dtype, const void *positions, void *q_out, int64_t q_out_stride, void *k_out,
+                   int64_t k_out_stride, void *stream);
+
+/* ---- key/value cache in 8 bits -------------------------------------------------
+ * No reference counterpart (its front end's attention has no cache).  The cache lies in pages of page_tokens tokens:
+ * k and v are [pages][kv_heads][page_tokens][head_dim] codes of one byte, k_scale and v_scale [pages][kv_heads] floats; a
+ * value is code * scale.  The scales dx_kvcache_write makes are powers of two.  page_tokens 16, 32, 64, 128 or 256;
+ * head_dim a multiple of 16 up to 256; k and v 16-byte aligned.
+ *
+ * A call's sequences: starts[batch+1] says where each one's new tokens are among the `rows` packed rows of the call's
+ * tensors, lens[batch] how many tokens it holds with them, table[batch][table_cols] which pages it is in.  New token i of n
+ * sits at position lens - n + i; with n > lens the ones in front of position 0 do not exist: they are not written, read as
+ * zeros, and their attention is zero.  Rows of no sequence are left as they were.  All three are int32 on the device, and
+ * can change between replays of a captured call.
+ *
+ * `flag` (device int32, may be NULL) collects: bit 0, a page number outside the cache (its tokens are not written, read as
+ * zeros and masked); bit 1, starts that do not ascend within the rows, or a length outside the table (what fits is worked
+ * on); bit 2, a value that is not a number (stored as 0).  No call touches memory out of range for any content of these. */
+typedef enum { DX_CACHE_I8 = 0, DX_CACHE_E4M3 = 1, DX_CACHE_FORMAT_COUNT = 2 } dx_cache_format;
+typedef struct dx_kvcache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t pages, kv_heads, page_tokens, head_dim;
+    int format;
+} dx_kvcache;
+typedef struct dx_kvseqs {
+    const int32_t *starts, *lens, *table;
+    int64_t batch, table_cols, rows;
+} dx_kvseqs;
+/* The new tokens' keys and values ([rows][kv_heads][head_dim], `stride` elements from row to row) into the cache.  A page's
+ * scale is the least power of two in whose units all of its tokens are within the codes' range; while earlier tokens
+ * stay in the page it never falls, and when it grows their codes are rounded again with it.  Codes are rounded to the
+ * nearest, ties to even; infinities take the largest code.  Slots behind a sequence's last token are left as they were.
+ * A page that a call writes belongs to one of its sequences (and once): what two sequences write into one page is undefined.
+ * dtype: DX_F32, DX_F16, DX_BF16. */
+int dx_kvcache_write(int dtype, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const dx_kvseqs *seqs,
+                     const dx_kvcache *cache, int32_t *flag, void *stream);
+/* The way back: the sequences' last tokens (all of them with n = lens) as values, rounded once to dtype. */
+int dx_kvcache_read(int dtype, const dx_kvseqs *seqs, const dx_kvcache *cache, void *k, int64_t k_stride, void *v, int64_t v_stride,
+                    int32_t *flag, void *stream);
+/* Attention of the new tokens over the cache: out[t,h] = sum_j p_j v_j with p = softmax_j(scale * q[t,h] . k_j) over the
+ * positions j <= the token's own, and j > own - window when window > 0; key head h / (q_heads / kv_heads).  The new tokens'
+ * keys are in the cache already (dx_kvcache_write).  A row that sees no key is zero.  q and out: [rows][q_heads][head_dim],
+ * DX_F16 or DX_BF16; scale > 0.  max_new: the most new tokens of a sequence, 0 if not known; it chooses the kernels
+ * and with them the speed, never what is computed.  The workspace serves one stream at a time; its size depends on
+ * the shapes alone. */
+size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache, int64_t max_new);
+int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
+                         double scale, int64_t max_new, int64_t window, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                         int32_t *flag, void *stream);
+
 /* ---- changeshape -----------------------------------------------------------
  * Replace launch_transpose/concat/broadcastTo/indexselect/repeat
  * (changeshape_miaobyte.cuh:16-88).  Pure data movement, bit-exact for every
