@@ -188,8 +188,8 @@ def run(s):
 def own_rope(s, case):
     from deepx_b200 import tensorfunc as TF
 
-    TF.qknorm_rope(s["q"], s["k"], s["q_weight"], s["k_weight"], s["inv_freq"], s["positions"], 1e-6 if case["norm"] else None,
-                   case["interleaved"], s["q_out"], s["k_out"])
+    norm = (s["q_weight"], s["k_weight"], 1e-6) if case["norm"] else (None, None, None)
+    TF.qknorm_rope(s["q"], s["k"], norm[0], norm[1], s["inv_freq"], s["positions"], norm[2], case["interleaved"], s["q_out"], s["k_out"])
     return s["q_out"], s["k_out"]
 
 
