@@ -135,6 +135,24 @@ template <int FMT> __device__ __forceinline__ __half2 decode2(uint32_t x) {
         return __hmin2(*reinterpret_cast<const __half2 *>(&r), __half2half2(__ushort_as_half(0x5F00)));  // 448
     }
 }
+// Four codes → four halfs, as two pairs: the pairs (0,1) and (2,3) of the word.
+template <int FMT> __device__ __forceinline__ void decode4(uint32_t x, uint32_t &lo, uint32_t &hi) {
+    if constexpr (FMT == DX_CACHE_I8) {
+        x ^= 0x80808080u;
+        const __half2 off = __half2half2(__ushort_as_half(0x6480));
+        lo = __byte_perm(x, 0x64646464u, 0x4140);
+        hi = __byte_perm(x, 0x64646464u, 0x4342);
+        __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&lo), off), b = __hsub2(*reinterpret_cast<const __half2 *>(&hi), off);
+        lo = *reinterpret_cast<uint32_t *>(&a);
+        hi = *reinterpret_cast<uint32_t *>(&b);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(x));
+        const __half2 top = __half2half2(__ushort_as_half(0x5F00));
+        __half2 a = __hmin2(*reinterpret_cast<const __half2 *>(&lo), top), b = __hmin2(*reinterpret_cast<const __half2 *>(&hi), top);
+        lo = *reinterpret_cast<uint32_t *>(&a);
+        hi = *reinterpret_cast<uint32_t *>(&b);
+    }
+}
 #endif
 
 }  // namespace kv

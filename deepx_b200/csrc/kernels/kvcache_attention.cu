@@ -1,84 +1,602 @@
 // dx_kvcache_attention: attention of packed new tokens over an 8-bit paged cache.
 //
-//   out[t,h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q[t,h].k_j - m),   m the running maximum,   j <= pos(t), j > pos(t) - window
+//   out[t,h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q[t,h].k_j - m),   c = scale log2(e),   j <= pos(t), j > pos(t) - window
+//
+// The rows of one sequence that share a key head (new token i, head i's group: n * group rows) are taken sixteen at a time: one
+// tensor-core tile of queries.  For one new token a sequence this is bound by memory: every code is read once and used for at
+// most sixteen rows.  One pass with the running maximum m and sum of the softmax; codes become halfs exactly, so the only
+// rounding to 16 bits is that of the weights (and each row of a bfloat16 query is brought to size 1 by a power of two first,
+// which keeps its 8 bits; elements 2^-17 below the row's largest begin to lose some).
+//
+// Work is split over the keys: the 64-token steps of all rows tiles and heads of all sequences stand in one line, and each
+// block takes an equal piece of it, whatever the lengths are (they are known on the device alone).  A piece may begin or end
+// inside an item (one tile of rows, one head); such items' parts meet in the workspace and a second kernel joins them, always
+// in the order of the keys: the same bits every time.
+#include <atomic>
+
 #include "kvcache.cuh"
 
 namespace dx {
 namespace kv {
 namespace {
 
-constexpr int CTA = 128;
+constexpr int WARPS = 4, CTA = WARPS * 32;
+constexpr int ROWS = 16;   // rows of an item
+constexpr int WT = 16;     // tokens a warp takes at a time: never more than one page
+constexpr int STEP = WARPS * WT;
+constexpr int JOIN_CTA = 512;
+// Weights are held as 2^(x - m + 7): m lags the true maximum by up to 2^8, so a weight is at most 2^15, and what is 2^-31 of the
+// largest is still a half.
+constexpr float LAG = 8.f, UP = 7.f;
+constexpr float NEG_INF = -__builtin_huge_valf();
 
 struct Attn {
     const void *q;
     void *out;
     int64_t q_stride, out_stride;
     int q_heads, group, window;
-    float scale;
+    float scale_log2;
+    int q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of out
+    int min_steps;
+    uint8_t *ws;
     int32_t *flag;
 };
 
-// A warp takes one head of one row and walks its keys.
-template <typename T, int FMT> __global__ void __launch_bounds__(CTA) attention_row_kernel(Attn a, Cache c, Seqs s) {
+// What the joining kernel needs to know of the item that ends inside block i's first piece: `parts` blocks from i - 1 on hold
+// parts of it (0: block i does not begin inside an item, or an earlier one joins it).
+struct alignas(32) Join {
+    int64_t row0;
+    int first_row, rows, head, parts;
+};
+
+template <int DP> struct Cfg {
+    static constexpr int STAGES = DP == 256 ? 3 : 4;
+    static constexpr int BLOCKS = DP == 256 ? 2 : DP == 128 ? 3 : 4;  // resident on an SM
+    static constexpr int TILE = WT * DP;                              // bytes of a warp's keys (or values) of a stage
+    static constexpr int RING = STAGES * 2 * TILE;                    // of a warp; holds its 16 x DP floats at the end
+    static constexpr int SMEM = WARPS * RING;
+    static constexpr int PART = ROWS * DP + 2 * ROWS;                 // floats of a part in the workspace: output, m, l
+    static_assert(RING >= ROWS * DP * 4, "the ring holds a warp's output");
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Where chunk `c` (16 bytes) of token `r` of a warp's tile lies: rows of DP bytes whose chunks are exchanged so that both ways the
+// tile is read (eight tokens, every other chunk; four tokens of one parity, two chunks) touch every bank once.
+template <int DP> __device__ __forceinline__ int place(int r, int c) {
+    if constexpr (DP == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ ((r >> 1) & 7)) << 4);
+    else return r * DP + ((c ^ (r & 7)) << 4);
+}
+// The chunk that lane t of a quad multiplies in its i-th turn.
+template <int DP> __device__ __forceinline__ int key_chunk(int t, int i) { return DP == 64 ? t : 2 * t + (i & 1) + 8 * (i >> 1); }
+
+// One sequence as the line of steps sees it.
+struct Line {
+    int lo, steps, tiles;  // first token of the range (a multiple of STEP), steps of a tile of rows, tiles of rows of a head
+};
+__device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
+    Line l;
+    const int64_t hi = min(int64_t(q.end), int64_t(q.first) + q.n);
+    const int64_t lo = a.window > 0 ? max(int64_t(0), int64_t(q.first) - a.window + 1) : 0;
+    l.lo = int(min(lo, max(hi, int64_t(0))) / STEP * STEP);
+    l.steps = hi > l.lo ? int((hi - l.lo + STEP - 1) / STEP) : 1;  // a row that sees nothing is written too
+    l.tiles = int((int64_t(q.n) * a.group + ROWS - 1) / ROWS);
+    return l;
+}
+__device__ __forceinline__ int64_t steps_of(const Seqs &s, const Cache &c, const Attn &a, int b) {
+    const Seq q = seq_at(s, c, b);
+    if (q.n == 0) return 0;
+    const Line l = line_of(q, a);
+    return int64_t(l.steps) * l.tiles * c.heads;
+}
+
+template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cfg<DP>::BLOCKS) attention_kernel(Attn a, Cache c, Seqs s) {
+    using K = Cfg<DP>;
+    constexpr int NT = DP / 8;             // column tiles of the output
+    constexpr int KC = DP / 64;            // chunks of a key that a lane multiplies
+    constexpr int VC = DP == 256 ? 2 : 1;  // chunks of a value that a lane multiplies (half of one at DP 64)
+    extern __shared__ __align__(1024) uint8_t ring[];
+    __shared__ float scales[WARPS][K::STAGES][2];
+    __shared__ int in_cache[WARPS][K::STAGES];
+    __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS];
+    __shared__ int64_t before[CTA], total_steps;
+    __shared__ int64_t found_at;
+    __shared__ int found_b;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    griddep_wait_cta();
     if (blockIdx.x == 0) check_seqs(s, c, a.flag);
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = int64_t(blockIdx.x) * (CTA / 32) + (threadIdx.x >> 5);
-    if (unit >= s.rows * a.q_heads) return;
-    const int64_t row = unit / a.q_heads;
-    const int h = int(unit - row * a.q_heads), kh = h / a.group;
-    const int b = seq_of_row(s.starts, s.batch, row);
-    if (b < 0) return;
-    const Seq sq = seq_at(s, c, b);
-    const int64_t i = row - sq.row0;
-    if (i < 0 || i >= sq.n) return;
-    const int64_t pos = sq.first + i;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + int64_t(h) * c.dim;
-    const int units = c.dim / 4;  // lane: four dimensions at 4 * lane, four at 128 + 4 * lane
-    float qv[8], o[8] = {};
+
+    // ---- this block's piece of the line ----
+    const int per = (s.batch + CTA - 1) / CTA;
+    {
+        int64_t mine = 0;
+        for (int b = threadIdx.x * per; b < min(s.batch, int(threadIdx.x + 1) * per); ++b) mine += steps_of(s, c, a, b);
+        int64_t sum = mine;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int d = (j / 4) * 128 + lane * 4 + j % 4;
-        qv[j] = d < c.dim ? to_compute(q[d]) : 0.f;
-    }
-    float m = -__int_as_float(0x7f800000), l = 0.f;
-    const int end = int(min(int64_t(sq.end), pos + 1));
-    const int begin = a.window > 0 ? int(max(int64_t(0), pos - a.window + 1)) : 0;
-    int64_t page = -1;
-    for (int j = begin; j < end; ++j) {
-        if (j == begin || (j & (c.page - 1)) == 0) page = page_at(s, c, b, j, a.flag);
-        if (page < 0) continue;
-        const int64_t at = ((page * c.heads + kh) * c.page + (j & (c.page - 1))) * c.dim;
-        float kf[8], vf[8];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const bool in = p * 32 + lane < units;
-            const uint32_t kw = in ? *reinterpret_cast<const uint32_t *>(c.k + at + p * 128 + lane * 4) : 0u;
-            const uint32_t vw = in ? *reinterpret_cast<const uint32_t *>(c.v + at + p * 128 + lane * 4) : 0u;
-            const float2 k0 = __half22float2(decode2<FMT>(kw & 0xFFFFu)), k1 = __half22float2(decode2<FMT>(kw >> 16));
-            const float2 v0 = __half22float2(decode2<FMT>(vw & 0xFFFFu)), v1 = __half22float2(decode2<FMT>(vw >> 16));
-            kf[4 * p] = k0.x, kf[4 * p + 1] = k0.y, kf[4 * p + 2] = k1.x, kf[4 * p + 3] = k1.y;
-            vf[4 * p] = v0.x, vf[4 * p + 1] = v0.y, vf[4 * p + 2] = v1.x, vf[4 * p + 3] = v1.y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
         }
-        float dot = 0.f;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) dot += qv[d] * kf[d];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        const float x = dot * c.k_scale[page * c.heads + kh] * a.scale;
-        const float top = fmaxf(m, x);
-        const float turn = m == top ? 1.f : __expf(m - top), p = __expf(x - top);
-        const float w = p * c.v_scale[page * c.heads + kh];
-        m = top;
-        l = l * turn + p;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) o[d] = o[d] * turn + w * vf[d];
+        if (lane == 31) before[warp] = sum;
+        __syncthreads();
+        int64_t base = 0;
+        for (int w = 0; w < warp; ++w) base += before[w];
+        __syncthreads();
+        before[threadIdx.x] = base + sum - mine;
+        if (threadIdx.x == CTA - 1) total_steps = base + sum;
+        __syncthreads();
     }
-    T *out = static_cast<T *>(a.out) + row * a.out_stride + int64_t(h) * c.dim;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int d = (j / 4) * 128 + lane * 4 + j % 4;
-        if (d < c.dim) out[d] = from_compute<T>(l == 0.f ? 0.f : o[j] / l);
+    const int64_t total = total_steps;
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / a.min_steps));
+    Join *join = reinterpret_cast<Join *>(a.ws) + blockIdx.x;
+    float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
+    if (total == 0 || int64_t(blockIdx.x) >= blocks) {
+        if (threadIdx.x == 0) join->parts = 0;
+        return;
     }
+    const int64_t begin = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
+    if (before[threadIdx.x] <= begin && (threadIdx.x == CTA - 1 || before[threadIdx.x + 1] > begin)) {
+        int64_t at = before[threadIdx.x];
+        int b = threadIdx.x * per;
+        for (; b < s.batch; ++b) {
+            const int64_t n = steps_of(s, c, a, b);
+            if (at + n > begin) break;
+            at += n;
+        }
+        found_b = b;
+        found_at = at;
+    }
+    __syncthreads();
+    int b = found_b;
+    int64_t seq_begin = found_at;
+    if (threadIdx.x == 0) join->parts = 0;
+
+    uint8_t *my_ring = ring + warp * K::RING;
+    const uint32_t ring_u = smem_u32(my_ring);
+    for (int64_t at = begin; at < end;) {
+        const Seq sq = seq_at(s, c, b);
+        const Line ln = line_of(sq, a);
+        const int64_t seq_steps = sq.n ? int64_t(ln.steps) * ln.tiles * c.heads : 0;
+        if (at >= seq_begin + seq_steps) {  // on to the next sequence
+            seq_begin += seq_steps;
+            ++b;
+            continue;
+        }
+        const int64_t item = (at - seq_begin) / ln.steps;
+        const int64_t item_begin = seq_begin + item * ln.steps, item_end = item_begin + ln.steps;
+        const int step0 = int(at - item_begin), step1 = int(min(end, item_end) - item_begin);
+        const int head = int(item / ln.tiles), first_row = int(item - int64_t(head) * ln.tiles) * ROWS;
+        const int rows = min(ROWS, int(min(int64_t(sq.n) * a.group - first_row, int64_t(ROWS))));
+        const int steps = step1 - step0;
+
+        // ---- the queries: row g and row g + 8 of the item, the chunks this lane multiplies ----
+        uint32_t qa[KC][4][4];
+        float c_row[2];
+        int pos[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int fr = first_row + g + 8 * r;
+            const bool live = g + 8 * r < rows;
+            const int i = live ? fr / a.group : 0;
+            pos[r] = live ? sq.first + i : INT32_MIN;
+            const T *q = static_cast<const T *>(a.q) + (sq.row0 + i) * a.q_stride + int64_t(head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+            Pack<T, 8> x[KC][2];
+            float amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const int d = key_chunk<DP>(t, k) * 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (live && d < c.dim && a.q_vec) x[k][h] = ld_cached<T, 8>(q + d + 8 * h);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[k][h].v[e] = live && d < c.dim ? q[d + 8 * h + e] : from_compute<T>(0.f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k][h].v[e])));
+                }
+            }
+            float down = 1.f;
+            c_row[r] = a.scale_log2;
+            if constexpr (std::is_same<T, bf16>::value) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
+                    down = __uint_as_float((254u - e) << 23);
+                    c_row[r] *= __uint_as_float(e << 23);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {  // word w of the chunk: dimensions 4w..4w+3
+                    const Pack<T, 8> &p = x[k][w >> 1];
+                    const int e = (w & 1) * 4;
+                    qa[k][w][r] = half2_bits(to_compute(p.v[e]) * down, to_compute(p.v[e + 1]) * down);
+                    qa[k][w][2 + r] = half2_bits(to_compute(p.v[e + 2]) * down, to_compute(p.v[e + 3]) * down);
+                }
+        }
+        const int pos_min = sq.first + first_row / a.group, pos_max = sq.first + (first_row + rows - 1) / a.group;
+        const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's
+
+        float o[NT][4], l[4] = {}, m[2] = {NEG_INF, NEG_INF}, v_ref = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+        // ---- keys and values in flight ----
+        const int32_t *table = s.table + int64_t(b) * s.cols;
+        auto token0 = [&](int step) { return ln.lo + (step0 + step) * STEP + warp * WT; };
+        auto page_number = [&](int step) {
+            const int j = token0(step);
+            return step < steps && j < seen_end ? table[j >> c.page_shift] : -1;
+        };
+        auto issue = [&](int step, int stage, int32_t number) {
+            if (step < steps) {
+                const int j = token0(step);
+                const bool some = j < seen_end;
+                const bool ok = some && number >= 0 && number < c.pages;
+                if (some && !ok && lane == 0) raise(a.flag, FLAG_PAGE);
+                const int64_t ph = ok ? int64_t(number) * c.heads + head : 0;
+                const int64_t base = (ph * c.page + (j & (c.page - 1))) * c.dim;
+                const uint32_t dst = ring_u + stage * 2 * K::TILE;
+#pragma unroll
+                for (int i = 0; i < K::TILE / 512; ++i) {
+                    const int idx = i * 32 + lane, r = idx / (DP / 16), ch = idx % (DP / 16);
+                    const bool in = ok && j + r < seen_end && ch * 16 < c.dim;
+                    const int64_t off = in ? base + r * c.dim + ch * 16 : 0;
+                    cp_async16(dst + place<DP>(r, ch), c.k + off, in);
+                    cp_async16(dst + K::TILE + place<DP>(r, ch), c.v + off, in);
+                }
+                if (lane < 2) cp_async4(smem_u32(&scales[warp][stage][lane]), (lane ? c.v_scale : c.k_scale) + ph, ok);
+                if (lane == 2) in_cache[warp][stage] = ok;
+            }
+            cp_commit();
+        };
+        int32_t next = page_number(0);
+#pragma unroll
+        for (int p = 0; p < K::STAGES - 1; ++p) {
+            const int32_t number = next;
+            next = page_number(p + 1);
+            issue(p, p, number);
+        }
+
+        int stage = 0;
+        for (int step = 0; step < steps; ++step) {
+            cp_wait<K::STAGES - 2>();
+            __syncwarp();
+            {
+                const int32_t number = next;
+                next = page_number(step + K::STAGES);
+                issue(step + K::STAGES - 1, stage == 0 ? K::STAGES - 1 : stage - 1, number);
+            }
+            const uint32_t ks = ring_u + stage * 2 * K::TILE, vs = ks + K::TILE;
+            const float k_scale = scales[warp][stage][0], v_scale = scales[warp][stage][1];
+            const bool ok = in_cache[warp][stage];
+            const int j0 = token0(step);
+            if (++stage == K::STAGES) stage = 0;
+            if (!ok) {
+                __syncwarp();
+                continue;  // no token of a page: nothing to see
+            }
+
+            // ---- scores of sixteen rows and sixteen tokens: lane (g, t) holds rows g, g+8 and tokens 2t, 2t+1, 2t+8, 2t+9 ----
+            float x[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint4 w = lds128(ks + place<DP>(g + 8 * n, key_chunk<DP>(t, k)));
+                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t b0, b1;
+                        decode4<FMT>(ww[i], b0, b1);
+                        mma(x[n], qa[k][i], b0, b1);
+                    }
+                }
+            const float c0 = c_row[0] * k_scale, c1 = c_row[1] * k_scale;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                x[n][0] *= c0;
+                x[n][1] *= c0;
+                x[n][2] *= c1;
+                x[n][3] *= c1;
+            }
+            if (j0 + WT - 1 > pos_min || j0 + WT > sq.end || (a.window > 0 && j0 <= int64_t(pos_max) - a.window)) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + 8 * n + 2 * t + (e & 1), p = pos[e >> 1];
+                        const bool seen = j <= p && j < sq.end && (a.window <= 0 || j > int64_t(p) - a.window);
+                        if (!seen) x[n][e] = NEG_INF;
+                    }
+            }
+            // ---- running maximum: a row's rises when a score is 2^8 above it ----
+            float top[2];
+            bool rise = false;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float v = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                top[r] = v > m[r] + LAG ? v : m[r];
+                rise |= top[r] != m[r];
+            }
+            const bool scale_up = v_scale > v_ref;
+            if (__any_sync(0xffffffffu, rise) || scale_up) {
+                const float turn = scale_up ? v_ref / v_scale : 1.f;  // values in units of the largest scale so far
+                if (scale_up) v_ref = v_scale;
+                float by[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    by[r] = top[r] == m[r] ? 1.f : exp2_approx(m[r] - top[r]);
+                    m[r] = top[r];
+                    l[2 * r] *= by[r];
+                    l[2 * r + 1] *= by[r];
+                    by[r] *= turn;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[n][0] *= by[0];
+                    o[n][1] *= by[0];
+                    o[n][2] *= by[1];
+                    o[n][3] *= by[1];
+                }
+            }
+            const float m0 = (m[0] == NEG_INF ? 0.f : m[0]) - UP, m1 = (m[1] == NEG_INF ? 0.f : m[1]) - UP;
+            uint32_t p[4];
+            p[0] = half2_bits(exp2_approx(x[0][0] - m0), exp2_approx(x[0][1] - m0));
+            p[1] = half2_bits(exp2_approx(x[0][2] - m1), exp2_approx(x[0][3] - m1));
+            p[2] = half2_bits(exp2_approx(x[1][0] - m0), exp2_approx(x[1][1] - m0));
+            p[3] = half2_bits(exp2_approx(x[1][2] - m1), exp2_approx(x[1][3] - m1));
+            mma(l, p, 0x3C003C00u, 0x3C003C00u);  // the sum of the very weights that multiply the values
+
+            // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
+            const bool same = v_scale == v_ref;
+            const __half2 unit = __float2half2_rn(v_scale / v_ref);
+            auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int n) {
+                uint32_t b0[4], b1[4];
+                decode4<FMT>(__byte_perm(wa, wb, 0x5140), b0[0], b0[1]);
+                decode4<FMT>(__byte_perm(wa, wb, 0x7362), b0[2], b0[3]);
+                decode4<FMT>(__byte_perm(wc, wd, 0x5140), b1[0], b1[1]);
+                decode4<FMT>(__byte_perm(wc, wd, 0x7362), b1[2], b1[3]);
+                if (!same) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const __half2 u = __hmul2(*reinterpret_cast<__half2 *>(&b0[i]), unit), w = __hmul2(*reinterpret_cast<__half2 *>(&b1[i]), unit);
+                        b0[i] = *reinterpret_cast<const uint32_t *>(&u);
+                        b1[i] = *reinterpret_cast<const uint32_t *>(&w);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma(o[n + i], p, b0[i], b1[i]);
+            };
+            if constexpr (DP == 64) {
+                const int half = (g & 1) * 8;
+                const uint2 wa = lds64(vs + place<DP>(2 * t, g >> 1) + half), wb = lds64(vs + place<DP>(2 * t + 1, g >> 1) + half);
+                const uint2 wc = lds64(vs + place<DP>(2 * t + 8, g >> 1) + half), wd = lds64(vs + place<DP>(2 * t + 9, g >> 1) + half);
+                four(wa.x, wb.x, wc.x, wd.x, 0);
+                four(wa.y, wb.y, wc.y, wd.y, 4);
+            } else {
+#pragma unroll
+                for (int h = 0; h < VC; ++h) {
+                    const int ch = g + 8 * h;
+                    const uint4 wa = lds128(vs + place<DP>(2 * t, ch)), wb = lds128(vs + place<DP>(2 * t + 1, ch));
+                    const uint4 wc = lds128(vs + place<DP>(2 * t + 8, ch)), wd = lds128(vs + place<DP>(2 * t + 9, ch));
+                    four(wa.x, wb.x, wc.x, wd.x, 16 * h);
+                    four(wa.y, wb.y, wc.y, wd.y, 16 * h + 4);
+                    four(wa.z, wb.z, wc.z, wd.z, 16 * h + 8);
+                    four(wa.w, wb.w, wc.w, wd.w, 16 * h + 12);
+                }
+            }
+            __syncwarp();  // the stage may be filled again
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp is done with its ring
+
+        // ---- the four warps' parts, each divided by its own sum, into the rings ----
+        constexpr int W = DP == 64 ? 8 : 16;  // dimensions of a lane's run
+        float *mine = reinterpret_cast<float *>(my_ring);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float sum = l[2 * r], by = sum == 0.f ? 0.f : v_ref / sum;
+            const int row = g + 8 * r;
+            if (t == 0) {
+                sm_m[warp][row] = m[r];
+                sm_l[warp][row] = sum;
+            }
+#pragma unroll
+            for (int h = 0; h < VC; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < W; i += 4) {
+                        const int d = h * 128 + (2 * t + e) * W + i;
+                        float4 v;
+                        v.x = o[h * 16 + i][2 * r + e] * by;
+                        v.y = o[h * 16 + i + 1][2 * r + e] * by;
+                        v.z = o[h * 16 + i + 2][2 * r + e] * by;
+                        v.w = o[h * 16 + i + 3][2 * r + e] * by;
+                        *reinterpret_cast<float4 *>(mine + row * DP + (((d >> 2) ^ ((((d >> 5) & 3) << 1) | (row & 1))) << 2)) = v;
+                    }
+        }
+        __syncthreads();
+        const bool whole = step0 == 0 && step1 == ln.steps;
+        float *part = parts + (int64_t(blockIdx.x) * 2 + (step0 == 0 ? 1 : 0)) * K::PART;
+        for (int u = threadIdx.x; u < ROWS * (DP / 4); u += CTA) {
+            const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
+            if (row >= rows || d >= c.dim) continue;
+            float top = NEG_INF, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w][row]);
+            const float base = top == NEG_INF ? 0.f : top;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float by = sm_l[w][row] * exp2_approx(sm_m[w][row] - base);
+                const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring + w * K::RING) + row * DP +
+                                                                  (((d >> 2) ^ ((((d >> 5) & 3) << 1) | (row & 1))) << 2));
+                sum += by;
+                v.x += by * x.x;
+                v.y += by * x.y;
+                v.z += by * x.z;
+                v.w += by * x.w;
+            }
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            v.x *= by;
+            v.y *= by;
+            v.z *= by;
+            v.w *= by;
+            if (whole) {
+                const int fr = first_row + row, i = fr / a.group;
+                T *out = static_cast<T *>(a.out) + (sq.row0 + i) * a.out_stride + int64_t(head * a.group + fr - i * a.group) * c.dim + d;
+                Pack<T, 4> y;
+                y.v[0] = from_compute<T>(v.x);
+                y.v[1] = from_compute<T>(v.y);
+                y.v[2] = from_compute<T>(v.z);
+                y.v[3] = from_compute<T>(v.w);
+                if (a.out_vec) st_stream<T, 4>(out, y);
+                else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[e] = y.v[e];
+                }
+            } else {
+                *reinterpret_cast<float4 *>(part + row * DP + d) = v;
+                if (d == 0) {
+                    part[ROWS * DP + row] = top;
+                    part[ROWS * DP + ROWS + row] = sum;
+                }
+            }
+        }
+        // the item begins in the block before and this block's begin lies inside it: here is where it is joined
+        if (threadIdx.x == 0 && at == begin && step0 > 0 && item_begin >= total * (int64_t(blockIdx.x) - 1) / blocks) {
+            join->row0 = sq.row0;
+            join->first_row = first_row;
+            join->rows = rows;
+            join->head = head;
+            join->parts = int((item_end * blocks - 1) / total) - int(blockIdx.x) + 2;  // the last block that has steps of it
+        }
+        __syncthreads();  // the rings are free again
+        at = item_begin + step1;
+    }
+}
+
+// Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
+// of the keys.  Sixteen warps share the item's rows; the warps of a row share its parts.
+template <typename T, int DP> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
+    constexpr int V = DP / 32;
+    __shared__ float sh[JOIN_CTA / 32][DP];
+    griddep_wait_cta();
+    const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
+    if (j.parts == 0) return;
+    const float *parts = reinterpret_cast<const float *>(a.ws + gridDim.x * sizeof(Join));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int each = j.rows > 8 ? 1 : j.rows > 4 ? 2 : j.rows > 2 ? 4 : j.rows > 1 ? 8 : 16;  // warps of a row
+    const int row = warp / each, sub = warp % each;
+    // part 0: the second part of block i - 1; part p > 0: the first of block i - 1 + p
+    auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * Cfg<DP>::PART; };
+    float acc[V] = {}, sum = 0.f;
+    if (row < j.rows) {
+        float top = NEG_INF;
+        for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, at(p)[ROWS * DP + row]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == NEG_INF ? 0.f : top;
+        for (int p0 = 0; p0 < j.parts; p0 += 32) {
+            float w = 0.f;
+            if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
+            float s = w;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            sum += s;
+            const int n = min(32, j.parts - p0);
+#pragma unroll 4
+            for (int p = sub; p < n; p += each) {
+                const float by = __shfl_sync(0xffffffffu, w, p);
+                const float *src = at(p0 + p) + row * DP + lane * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
+    __syncthreads();
+    if (row >= j.rows || sub) return;
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    const int fr = j.first_row + row, i = fr / a.group;
+    T *out = static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
+    for (int d = lane; d < c.dim; d += 32) {
+        float v = 0.f;
+        for (int w = 0; w < each; ++w) v += sh[warp + w][d];
+        out[d] = from_compute<T>(v * by);
+    }
+}
+
+// A kernel's shared memory above 48 KB has to be allowed once on each device.
+template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_t> *prepared) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (e == cudaSuccess && !(prepared->load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) prepared->fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e == cudaSuccess ? DX_OK : fail(DX_E_CUDA, "kvcache_attention: %s", cudaGetErrorString(e));
+}
+
+template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+    static std::atomic<uint64_t> prepared{0};  // one bit for each device
+    if (int e = allow_shared(attention_kernel<T, FMT, DP>, Cfg<DP>::SMEM, &prepared)) return e;
+    const unsigned grid = unsigned(sm_count() * Cfg<DP>::BLOCKS);
+    launch_pdl(attention_kernel<T, FMT, DP>, dim3(grid), dim3(CTA), Cfg<DP>::SMEM, st, a, c, s);
+    if (int e = check_launch("kvcache_attention")) return e;
+    launch_pdl(join_kernel<T, DP>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
+    return check_launch("kvcache_attention (join)");
+}
+
+int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+size_t workspace(int dim) {
+    const int dp = padded(dim);
+    const size_t blocks = size_t(sm_count()) * (dp == 64 ? Cfg<64>::BLOCKS : dp == 128 ? Cfg<128>::BLOCKS : Cfg<256>::BLOCKS);
+    const size_t part = dp == 64 ? Cfg<64>::PART : dp == 128 ? Cfg<128>::PART : Cfg<256>::PART;
+    return blocks * (sizeof(Join) + 2 * part * sizeof(float));
 }
 
 }  // namespace
@@ -86,7 +604,11 @@ template <typename T, int FMT> __global__ void __launch_bounds__(CTA) attention_
 }  // namespace dx
 
 extern "C" size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache, int64_t max_new) {
-    return 0;
+    using namespace dx;
+    kv::Cache c;
+    kv::Seqs s;
+    if (kv::check("kvcache_attention", cache, seqs, &c, &s) || s.rows == 0 || s.batch == 0) return 0;
+    return kv::workspace(c.dim);
 }
 
 extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
@@ -100,23 +622,32 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     if (q_heads < 1 || q_heads % c.heads || q_heads > 65535) return fail(DX_E_SHAPE, "kvcache_attention: %lld query heads over %d key heads", (long long)q_heads, c.heads);
     const int64_t width = q_heads * c.dim;
     if (q_stride < width || out_stride < width) return fail(DX_E_SHAPE, "kvcache_attention: rows of %lld elements overlap at strides %lld and %lld", (long long)width, (long long)q_stride, (long long)out_stride);
-    if (!(scale > 0) || !(float(scale) > 0) || scale > 3e38) return fail(DX_E_ARG, "kvcache_attention: scale %g", scale);
+    if (!(scale > 0) || !(float(scale * 1.4426950408889634) > 0) || scale > 1e38) return fail(DX_E_ARG, "kvcache_attention: scale %g", scale);
     if (max_new < 0 || window < 0) return fail(DX_E_ARG, "kvcache_attention: max_new %lld, window %lld", (long long)max_new, (long long)window);
+    if (s.rows * (q_heads / c.heads) > INT32_MAX) return fail(DX_E_SHAPE, "kvcache_attention: %lld rows of %lld heads each over a key head", (long long)s.rows, (long long)(q_heads / c.heads));
     if (s.rows == 0 || s.batch == 0) return DX_OK;
     if (!q || !out) return fail(DX_E_ARG, "kvcache_attention: null tensor pointer");
     const int64_t qb = ((s.rows - 1) * q_stride + width) * 2, ob = ((s.rows - 1) * out_stride + width) * 2;
     const int64_t codes = c.pages * c.heads * int64_t(c.page) * c.dim;
     if (kv::overlap(q, qb, out, ob) || kv::overlap(out, ob, c.k, codes) || kv::overlap(out, ob, c.v, codes))
         return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
-    kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale), flag};
+    const size_t need = kv::workspace(c.dim);
+    if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
+    kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),
+               q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 4 == 0 && aligned_to(out, 8), 2, static_cast<uint8_t *>(workspace), flag};
     cudaStream_t st = as_stream(stream);
-    const unsigned grid = unsigned((s.rows * q_heads + 3) / 4);
-    if (dtype == DX_F16) {
-        if (cache->format == DX_CACHE_I8) kv::attention_row_kernel<f16, DX_CACHE_I8><<<grid, kv::CTA, 0, st>>>(a, c, s);
-        else kv::attention_row_kernel<f16, DX_CACHE_E4M3><<<grid, kv::CTA, 0, st>>>(a, c, s);
-    } else {
-        if (cache->format == DX_CACHE_I8) kv::attention_row_kernel<bf16, DX_CACHE_I8><<<grid, kv::CTA, 0, st>>>(a, c, s);
-        else kv::attention_row_kernel<bf16, DX_CACHE_E4M3><<<grid, kv::CTA, 0, st>>>(a, c, s);
+#define DX_CALL(T, FMT)                                                             \
+    switch (kv::padded(c.dim)) {                                                    \
+        case 64: return kv::launch<T, FMT, 64>(a, c, s, st);                        \
+        case 128: return kv::launch<T, FMT, 128>(a, c, s, st);                      \
+        default: return kv::launch<T, FMT, 256>(a, c, s, st);                       \
     }
-    return check_launch("kvcache_attention");
+    if (dtype == DX_F16) {
+        if (cache->format == DX_CACHE_I8) { DX_CALL(f16, DX_CACHE_I8) }
+        DX_CALL(f16, DX_CACHE_E4M3)
+    }
+    if (cache->format == DX_CACHE_I8) { DX_CALL(bf16, DX_CACHE_I8) }
+    DX_CALL(bf16, DX_CACHE_E4M3)
+#undef DX_CALL
 }

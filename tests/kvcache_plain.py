@@ -124,7 +124,9 @@ def attention(batch, Q, scale, window=0):
     may cut where others round): an error of dim * 2^-23 * scale * sum |q||k| in the exponent, twice since the maximum has it
     too, and the weights and their sum have it both: four times.  The output is a float32 sum over the keys: keys * 2^-23 of A.
     A q of bfloat16 keeps its 8 bits; 2^-24 of the row's largest for elements far below it is inside the dim term.  The exponential
-    itself and its argument's rounding: 2^-21 + 2^-23 * |argument|, the argument below 200 where a weight counts: 2^-15 of A."""
+    itself and its argument's rounding: 2^-21 + 2^-23 * |argument|, the argument below 200 where a weight counts: 2^-15 of A.
+    16-bit floats below 2^-14 have the fixed step 2^-24: with weights held so that the largest is 2^7 or more, each is off by
+    2^-25 / 2^7 of the sum at most on top (sum |v| over the keys seen), and values held in units of the largest scale by 2^-25 of it."""
     heads = Q.shape[1]
     group = heads // batch.heads
     out = torch.zeros(Q.shape, dtype=torch.float64, device=Q.device)
@@ -133,6 +135,7 @@ def attention(batch, Q, scale, window=0):
         if m == 0 or n == 0:
             continue
         k, v = batch.history(batch.k, batch.ks, b), batch.history(batch.v, batch.vs, b)
+        largest = batch.vs[batch.host_table[b, : -(-n // batch.page)].to(Q.device)].max()
         key = torch.arange(n, device=Q.device)[None, :]
         pos = torch.arange(n - m, n, device=Q.device)[:, None]
         seen = key <= pos
@@ -148,7 +151,8 @@ def attention(batch, Q, scale, window=0):
             out[row: row + m, h] = p @ vh
             size = p @ vh.abs()
             score = ((q.abs() @ kh.abs().T) * scale * seen).amax(-1, keepdim=True)
-            bound[row: row + m, h] = size * (2.0**-10 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
+            fixed = 2.0**-32 * (seen.double() @ vh.abs()) + 2.0**-25 * float(largest)
+            bound[row: row + m, h] = fixed + size * (2.0**-10 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
     return out, bound
 
 

@@ -71,6 +71,16 @@ def test_attention_arguments_are_checked():
     assert attend(max_new=-1) == N.E_ARG and attend(window=-1) == N.E_ARG
     assert attend(q=None) == N.E_ARG and attend(out=None) == N.E_ARG
     assert attend(out=FAR + 64) == N.E_ALIAS and attend(out=4096) == N.E_ALIAS
+    assert attend(s=seqs(rows=(1 << 31) - 1)) == N.E_SHAPE  # rows of a key head's group beyond 32 bits
+
+
+def test_attention_workspace_is_checked():
+    need = N.lib.dx_kvcache_attention_workspace_bytes(N.BF16, 4, seqs(), cache(), 0)
+    assert need > 0
+    assert N.lib.dx_kvcache_attention_workspace_bytes(N.BF16, 4, seqs(rows=0), cache(), 0) == 0
+    assert N.lib.dx_kvcache_attention_workspace_bytes(N.BF16, 4, seqs(), cache(format=7), 0) == 0
+    assert attend() == N.E_WORKSPACE and attend(ws=FAR * 4, ws_bytes=need - 1) == N.E_WORKSPACE
+    assert attend(ws=FAR * 4 + 64, ws_bytes=need) == N.E_ARG
 
 
 def rope(dtype=N.F32, q=FAR, qs=256, qh=4, k=FAR * 2, ks=128, kh=2, tokens=3, dim=64, norm=1, eps=1e-6, inv=64, rotated=64, pos_dtype=N.I32, pos=64, qo=FAR * 3,
