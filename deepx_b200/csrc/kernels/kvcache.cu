@@ -30,135 +30,244 @@ int check(const char *what, const dx_kvcache *c, const dx_kvseqs *s, Cache *cach
 
 namespace {
 
-constexpr int W_CTA = 128;
+constexpr int CTA = 256;
 constexpr int MAX_CHUNK = 128;
+constexpr int STARTS = 512;  // sequences whose starts a block copies into shared memory before it searches them
 
-template <typename T> __device__ __forceinline__ float4 load4(const T *p, bool vec) {
-    if (vec) {
-        const Pack<T, 4> v = ld_cached<T, 4>(p);
-        return make_float4(to_compute(v.v[0]), to_compute(v.v[1]), to_compute(v.v[2]), to_compute(v.v[3]));
+// Eight values of a row as they lie in memory.
+template <typename T> struct Eight {
+    static constexpr int N = 16 / sizeof(T), P = 8 / N;
+    Pack<T, N> p[P];
+    __device__ __forceinline__ void load(const T *x, bool vec) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (vec) p[i] = ld_cached<T, N>(x + i * N);
+            else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) p[i].v[e] = x[i * N + e];
+            }
+        }
     }
-    return make_float4(to_compute(p[0]), to_compute(p[1]), to_compute(p[2]), to_compute(p[3]));
+    __device__ __forceinline__ float get(int e) const { return to_compute(p[e / N].v[e % N]); }
+};
+// The larger of the sizes of eight values and `top`: not a number or infinite if one of them is.
+template <typename T> __device__ __forceinline__ float size_of(const Eight<T> &x, float top) {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x.get(e))));
+        return top;
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, f16>::value, __half2, __nv_bfloat162>::type;
+        const T2 *v = reinterpret_cast<const T2 *>(x.p[0].v);
+        const T2 m = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(to_compute(m.x)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(to_compute(m.y)));
+        return top;
+    }
+}
+// The same of the finite ones among them.
+template <typename T> __device__ __forceinline__ float finite_size_of(const Eight<T> &x, float top, bool &nan) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float f = fabsf(x.get(e));
+        nan |= f != f;
+        top = fmaxf(top, f < __int_as_float(0x7f800000) ? f : 0.f);
+    }
+    return top;
+}
+template <typename T, int FMT> __device__ __forceinline__ uint2 codes_of(const Eight<T> &x, float inv, bool finite) {
+    if (finite) return make_uint2(encode4_finite<FMT>(x.get(0), x.get(1), x.get(2), x.get(3), inv), encode4_finite<FMT>(x.get(4), x.get(5), x.get(6), x.get(7), inv));
+    return make_uint2(encode4<FMT>(x.get(0) * inv, x.get(1) * inv, x.get(2) * inv, x.get(3) * inv),
+                      encode4<FMT>(x.get(4) * inv, x.get(5) * inv, x.get(6) * inv, x.get(7) * inv));
+}
+// The starts, copied into shared memory where they fit: a search is then one trip to memory instead of one for each halving.
+__device__ __forceinline__ const int32_t *starts_near(const Seqs &s, int32_t *copy) {
+    if (s.batch > STARTS) return s.starts;
+    for (int i = threadIdx.x; i <= s.batch; i += CTA) copy[i] = s.starts[i];
+    __syncthreads();
+    return copy;
 }
 
-// A block takes the pages whose first new token is one of `chunk` packed rows, for one head, of the keys (blockIdx.z = 0) or
-// the values: the largest size of the page's new values, the page's scale from it, the codes in a second pass over the
-// same rows (which the first has left in L1 / L2).
-template <typename T, int FMT>
-__global__ void __launch_bounds__(W_CTA) write_kernel(const T *k, int64_t k_stride, const T *v, int64_t v_stride, Cache c, Seqs s, int chunk,
-                                                      bool vec, int32_t *flag) {
-    __shared__ int list[MAX_CHUNK], count;
-    __shared__ float part[W_CTA / 32];
-    const int head = blockIdx.y;
-    const T *x = blockIdx.z ? v : k;
-    const int64_t stride = blockIdx.z ? v_stride : k_stride;
-    uint8_t *codes = blockIdx.z ? c.v : c.k;
-    float *scales = blockIdx.z ? c.v_scale : c.k_scale;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_seqs(s, c, flag);
+// A block takes the pages whose first new token is one of `chunk` packed rows, for one head: half of its threads the keys, half the
+// values.  The page's values are loaded once: up to KEEP vectors of eight stay in a thread's registers between the search for
+// their largest size and the rounding (a page of 64 tokens of 128 dimensions whole); the rest of larger pages is read again,
+// out of the cache the first time has left it in.
+template <typename T, int FMT, int KEEP>
+__global__ void __launch_bounds__(CTA, 4) write_kernel(const T *k, int64_t k_stride, const T *v, int64_t v_stride, Cache c, Seqs s, int chunk,
+                                                       FastDiv by_units, bool vec, int32_t *flag) {
+    constexpr int SIDE = CTA / 2;
+    struct Found {
+        int64_t row;
+        int b, pos, tokens;
+    };
+    __shared__ Found list[MAX_CHUNK];
+    __shared__ int32_t copy[STARTS + 1];
+    __shared__ int count;
+    __shared__ float part[2][CTA / 32];
+    griddep_wait_cta();
+    const int side = threadIdx.x / SIDE, tid = threadIdx.x % SIDE, head = blockIdx.y;
+    const T *x = side ? v : k;
+    const int64_t stride = side ? v_stride : k_stride;
+    uint8_t *codes = side ? c.v : c.k;
+    float *scales = side ? c.v_scale : c.k_scale;
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_seqs(s, c, flag);
     if (threadIdx.x == 0) count = 0;
+    const int32_t *starts = starts_near(s, copy);
     __syncthreads();
     const int64_t row0 = int64_t(blockIdx.x) * chunk;
     if (int(threadIdx.x) < chunk && row0 + threadIdx.x < s.rows) {
         const int64_t row = row0 + threadIdx.x;
-        const int b = seq_of_row(s.starts, s.batch, row);
+        const int b = seq_of_row(starts, s.batch, row);
         if (b >= 0) {
             const Seq q = seq_at(s, c, b);
             const int64_t i = row - q.row0;
             const int64_t pos = q.first + i;
-            if (i >= 0 && i < q.n && pos >= 0 && pos < q.end && (i == 0 || pos == 0 || (pos & (c.page - 1)) == 0)) list[atomicAdd(&count, 1)] = int(row);
+            if (i >= 0 && i < q.n && pos >= 0 && pos < q.end && (i == 0 || pos == 0 || (pos & (c.page - 1)) == 0)) {
+                const int room = min(c.page - int(pos & (c.page - 1)), q.end - int(pos));
+                list[atomicAdd(&count, 1)] = Found{row, b, int(pos), int(min(int64_t(room), q.n - i))};
+            }
         }
     }
     __syncthreads();
-    const int units = c.dim / 4;
-    const int found = count;
+    const int units = c.dim / 8, found = count;
     for (int n = 0; n < found; ++n) {
-        const int64_t row = list[n];
-        const int b = seq_of_row(s.starts, s.batch, row);
-        const Seq q = seq_at(s, c, b);
-        const int pos = int(q.first + (row - q.row0));
-        const int slot = pos & (c.page - 1);
-        const int tokens = int(min(int64_t(min(c.page - slot, q.end - pos)), q.n - (row - q.row0)));
-        const int64_t page = page_at(s, c, b, pos, flag);
+        const Found f = list[n];
+        const int slot = f.pos & (c.page - 1), total = f.tokens * units;
+        const int64_t page = page_at(s, c, f.b, f.pos, threadIdx.x == 0 ? flag : nullptr);
         if (page < 0) continue;  // the same answer in every thread
-        const T *src = x + row * stride + int64_t(head) * c.dim;
+        const T *src = x + f.row * stride + int64_t(head) * c.dim;
         uint8_t *dst = codes + ((page * c.heads + head) * c.page) * int64_t(c.dim);
+        float *scale_at = scales + page * c.heads + head;
+        const float had = slot ? *scale_at : 0.f;
+        auto at = [&](int u) {
+            const int t = int(fd_div(uint32_t(u), by_units));
+            return src + t * stride + (u - t * units) * 8;
+        };
+        Eight<T> kept[KEEP];
         float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (tid + i * SIDE < total) kept[i].load(at(tid + i * SIDE), vec);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (tid + i * SIDE < total) amax = size_of(kept[i], amax);
+        for (int u = tid + KEEP * SIDE; u < total; u += SIDE) {
+            Eight<T> more;
+            more.load(at(u), vec);
+            amax = size_of(more, amax);
+        }
+        const bool finite = amax < __int_as_float(0x7f800000);  // of this thread's values
         bool nan = false;
-        for (int u = threadIdx.x; u < tokens * units; u += W_CTA) {
-            const int t = u / units;
-            const float4 a = load4(src + t * stride + (u - t * units) * 4, vec);
-            auto size = [&](float f) {
-                nan |= f != f;
-                f = fabsf(f);
-                return f < __int_as_float(0x7f800000) ? f : 0.f;
-            };
-            amax = fmaxf(amax, fmaxf(fmaxf(size(a.x), size(a.y)), fmaxf(size(a.z), size(a.w))));
+        if (!finite) {
+            amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i)
+                if (tid + i * SIDE < total) amax = finite_size_of(kept[i], amax, nan);
+            for (int u = tid + KEEP * SIDE; u < total; u += SIDE) {
+                Eight<T> more;
+                more.load(at(u), vec);
+                amax = finite_size_of(more, amax, nan);
+            }
         }
         if (nan) raise(flag, FLAG_NAN);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-        const float had = slot ? scales[page * c.heads + head] : 0.f;
-        __syncthreads();  // every thread has read the old scale
+        if ((threadIdx.x & 31) == 0) part[n & 1][threadIdx.x >> 5] = amax;
+        __syncthreads();  // and every thread has read the old scale
 #pragma unroll
-        for (int w = 0; w < W_CTA / 32; ++w) amax = fmaxf(amax, part[w]);
+        for (int w = 0; w < SIDE / 32; ++w) amax = fmaxf(amax, part[n & 1][side * (SIDE / 32) + w]);
         float scale = scale_for<FMT>(amax);
         if (slot) scale = fmaxf(scale, scale_kept(had));
         const float inv = inverse_of(scale);
         if (slot && scale != had) {  // the earlier tokens' codes in units of the grown scale
             const float by = had * inv;
-            for (int u = threadIdx.x; u < slot * units; u += W_CTA) {
-                uint32_t w = *reinterpret_cast<const uint32_t *>(dst + int64_t(u) * 4);
-                const float2 lo = __half22float2(decode2<FMT>(w & 0xFFFFu)), hi = __half22float2(decode2<FMT>(w >> 16));
-                w = encode4<FMT>(lo.x * by, lo.y * by, hi.x * by, hi.y * by);
-                *reinterpret_cast<uint32_t *>(dst + int64_t(u) * 4) = w;
+            for (int u = tid; u < slot * units; u += SIDE) {
+                uint2 w = *reinterpret_cast<const uint2 *>(dst + int64_t(u) * 8);
+                for (uint32_t *e : {&w.x, &w.y}) {
+                    const float2 lo = __half22float2(decode2<FMT>(*e & 0xFFFFu)), hi = __half22float2(decode2<FMT>(*e >> 16));
+                    *e = encode4<FMT>(lo.x * by, lo.y * by, hi.x * by, hi.y * by);
+                }
+                *reinterpret_cast<uint2 *>(dst + int64_t(u) * 8) = w;
             }
         }
-        for (int u = threadIdx.x; u < tokens * units; u += W_CTA) {
-            const int t = u / units;
-            const float4 a = load4(src + t * stride + (u - t * units) * 4, vec);
-            *reinterpret_cast<uint32_t *>(dst + (int64_t(slot) * units + u) * 4) = encode4<FMT>(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        uint2 *out = reinterpret_cast<uint2 *>(dst) + int64_t(slot) * units;
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (tid + i * SIDE < total) out[tid + i * SIDE] = codes_of<T, FMT>(kept[i], inv, finite);
+        for (int u = tid + KEEP * SIDE; u < total; u += SIDE) {
+            Eight<T> more;
+            more.load(at(u), vec);
+            out[u] = codes_of<T, FMT>(more, inv, finite);
         }
-        if (threadIdx.x == 0) scales[page * c.heads + head] = scale;
-        __syncthreads();  // `part` is free again
+        if (tid == 0) *scale_at = scale;
     }
 }
 
+// A block takes `chunk` packed rows: where each one's codes are is worked out once, then sixteen codes (one 16-byte load) a thread and
+// turn, keys and values in one go.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(W_CTA) read_kernel(Cache c, Seqs s, T *k, int64_t k_stride, T *v, int64_t v_stride, bool vec, int32_t *flag) {
-    if (blockIdx.x == 0 && blockIdx.y == 0) check_seqs(s, c, flag);
-    const int64_t row = blockIdx.x;
-    const int b = seq_of_row(s.starts, s.batch, row);
-    if (b < 0) return;
-    const Seq q = seq_at(s, c, b);
-    const int64_t i = row - q.row0;
-    if (i < 0 || i >= q.n) return;
-    const int64_t pos = q.first + i;
-    const int64_t page = pos >= 0 && pos < q.end ? page_at(s, c, b, int(pos), flag) : -1;
-    const uint8_t *codes = blockIdx.y ? c.v : c.k;
-    const float *scales = blockIdx.y ? c.v_scale : c.k_scale;
-    T *out = blockIdx.y ? v + row * v_stride : k + row * k_stride;
-    const int units = c.dim / 4;
-    for (int u = threadIdx.x; u < c.heads * units; u += W_CTA) {
-        const int h = u / units;
-        Pack<T, 4> o;
-        if (page < 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o.v[j] = from_compute<T>(0.f);
-        } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + ((page * c.heads + h) * c.page + (pos & (c.page - 1))) * c.dim + (u - h * units) * 4);
-            const float f = scales[page * c.heads + h];
-            const float2 lo = __half22float2(decode2<FMT>(w & 0xFFFFu)), hi = __half22float2(decode2<FMT>(w >> 16));
-            o.v[0] = from_compute<T>(lo.x * f);
-            o.v[1] = from_compute<T>(lo.y * f);
-            o.v[2] = from_compute<T>(hi.x * f);
-            o.v[3] = from_compute<T>(hi.y * f);
+__global__ void __launch_bounds__(CTA) read_kernel(Cache c, Seqs s, T *k, int64_t k_stride, T *v, int64_t v_stride, int chunk, FastDiv by_row,
+                                                   FastDiv by_units, bool vec, int32_t *flag) {
+    constexpr int N = 16 / sizeof(T);
+    constexpr int64_t NONE = -1, ZERO = -2;
+    __shared__ int64_t page_of[MAX_CHUNK];  // page number, or NONE: no sequence's row, ZERO: no token's
+    __shared__ int slot_of[MAX_CHUNK];
+    __shared__ int32_t copy[STARTS + 1];
+    griddep_wait_cta();
+    if (blockIdx.x == 0) check_seqs(s, c, flag);
+    const int32_t *starts = starts_near(s, copy);
+    const int64_t row0 = int64_t(blockIdx.x) * chunk;
+    const int rows = int(min(int64_t(chunk), s.rows - row0));
+    if (int(threadIdx.x) < rows) {
+        const int64_t row = row0 + threadIdx.x;
+        const int b = seq_of_row(starts, s.batch, row);
+        int64_t page = NONE;
+        if (b >= 0) {
+            const Seq q = seq_at(s, c, b);
+            const int64_t i = row - q.row0, pos = q.first + i;
+            if (i >= 0 && i < q.n) {
+                page = ZERO;
+                if (pos >= 0 && pos < q.end) {
+                    page = page_at(s, c, b, int(pos), flag);
+                    if (page < 0) page = ZERO;
+                    slot_of[threadIdx.x] = int(pos & (c.page - 1));
+                }
+            }
         }
-        T *dst = out + int64_t(u) * 4;
-        if (vec) st_stream<T, 4>(dst, o);
-        else {
+        page_of[threadIdx.x] = page;
+    }
+    __syncthreads();
+    const int units = c.dim / 16, per_row = c.heads * units;
+    for (int i = threadIdx.x; i < 2 * rows * per_row; i += CTA) {
+        const int line = int(fd_div(uint32_t(i), by_row)), u = i - line * per_row, r = line >> 1;  // a row's keys, then its values
+        const bool is_v = line & 1;
+        const int64_t page = page_of[r];
+        if (page == NONE) continue;
+        T *out = (is_v ? v + (row0 + r) * v_stride : k + (row0 + r) * k_stride) + int64_t(u) * 16;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        float f = 0.f;
+        if (page >= 0) {
+            const int h = int(fd_div(uint32_t(u), by_units));
+            const int64_t ph = page * c.heads + h;
+            w = __ldcs(reinterpret_cast<const uint4 *>((is_v ? c.v : c.k) + (ph * c.page + slot_of[r]) * c.dim + (u - h * units) * 16));
+            f = (is_v ? c.v_scale : c.k_scale)[ph];
+        }
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        Pack<T, N> o[16 / N];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[j] = o.v[j];
+        for (int e = 0; e < 4; ++e) {
+            const float2 lo = __half22float2(decode2<FMT>(words[e] & 0xFFFFu)), hi = __half22float2(decode2<FMT>(words[e] >> 16));
+            const float x[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[(4 * e + d) / N].v[(4 * e + d) % N] = from_compute<T>(x[d] * f);
+        }
+#pragma unroll
+        for (int p = 0; p < 16 / N; ++p) {
+            if (vec) st_stream<T, N>(out + p * N, o[p]);
+            else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) out[p * N + e] = o[p].v[e];
+            }
         }
     }
 }
@@ -177,20 +286,27 @@ int check_rows(const char *what, int dtype, const Seqs &s, const Cache &c, const
     return DX_OK;
 }
 
-template <typename T> bool packs_of_4(const void *k, int64_t k_stride, const void *v, int64_t v_stride) {
-    return k_stride % 4 == 0 && v_stride % 4 == 0 && aligned_to(k, 4 * sizeof(T)) && aligned_to(v, 4 * sizeof(T));
+template <typename T> bool vectors(const void *k, int64_t k_stride, const void *v, int64_t v_stride) {
+    constexpr int N = 16 / sizeof(T);
+    return k_stride % N == 0 && v_stride % N == 0 && aligned_to(k, 16) && aligned_to(v, 16);
 }
 
 template <typename T, int FMT>
 void launch_write(const void *k, int64_t ks, const void *v, int64_t vs, const Cache &c, const Seqs &s, int32_t *flag, cudaStream_t st) {
+    // rows a block searches for first tokens of pages: one for single tokens, a page's worth for prompts
     int chunk = 1;
     while (chunk < MAX_CHUNK && chunk < c.page && int64_t(chunk) * s.batch < s.rows) chunk *= 2;
-    const dim3 grid(unsigned((s.rows + chunk - 1) / chunk), unsigned(c.heads), 2);
-    write_kernel<T, FMT><<<grid, W_CTA, 0, st>>>(static_cast<const T *>(k), ks, static_cast<const T *>(v), vs, c, s, chunk, packs_of_4<T>(k, ks, v, vs), flag);
+    const dim3 grid(unsigned((s.rows + chunk - 1) / chunk), unsigned(c.heads));
+    const bool vec = vectors<T>(k, ks, v, vs);
+    if (chunk == 1) launch_pdl(write_kernel<T, FMT, 1>, grid, dim3(CTA), 0, st, static_cast<const T *>(k), ks, static_cast<const T *>(v), vs, c, s, chunk, make_fastdiv(c.dim / 8), vec, flag);
+    else launch_pdl(write_kernel<T, FMT, 8>, grid, dim3(CTA), 0, st, static_cast<const T *>(k), ks, static_cast<const T *>(v), vs, c, s, chunk, make_fastdiv(c.dim / 8), vec, flag);
 }
 template <typename T, int FMT>
 void launch_read(const Cache &c, const Seqs &s, void *k, int64_t ks, void *v, int64_t vs, int32_t *flag, cudaStream_t st) {
-    read_kernel<T, FMT><<<dim3(unsigned(s.rows), 2), W_CTA, 0, st>>>(c, s, static_cast<T *>(k), ks, static_cast<T *>(v), vs, packs_of_4<T>(k, ks, v, vs), flag);
+    int chunk = 1;
+    while (chunk < 16 && s.rows > int64_t(sm_count()) * 8 * chunk) chunk *= 2;
+    launch_pdl(read_kernel<T, FMT>, dim3(unsigned((s.rows + chunk - 1) / chunk)), dim3(CTA), 0, st, c, s, static_cast<T *>(k), ks, static_cast<T *>(v), vs, chunk,
+               make_fastdiv(unsigned(c.heads * (c.dim / 16))), make_fastdiv(c.dim / 16), vectors<T>(k, ks, v, vs), flag);
 }
 
 }  // namespace

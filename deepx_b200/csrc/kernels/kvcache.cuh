@@ -123,8 +123,21 @@ template <int FMT> __device__ __forceinline__ uint32_t encode4(float a, float b,
         return lo | hi << 16;
     }
 }
-// Two codes in the low half of `x` → two halfs (exact).  The codes 0x7F and 0xFF of e4m3, which no cache written here holds,
-// read as 448, so that nothing that lies in a page's unused slots or behind a mask can reach a result as a NaN.
+// The same of finite values within the codes' range, times `inv`, a power of two: for int8 one fused multiply-add rounds a value to a
+// whole number in the low bits of a float (ties to even, as the unit of 1.5 * 2^23 is 1).
+template <int FMT> __device__ __forceinline__ uint32_t encode4_finite(float a, float b, float c, float d, float inv) {
+    if constexpr (FMT == DX_CACHE_I8) {
+        constexpr float magic = 12582912.f;
+        const uint32_t u = __float_as_uint(__fmaf_rn(a, inv, magic)), v = __float_as_uint(__fmaf_rn(b, inv, magic));
+        const uint32_t w = __float_as_uint(__fmaf_rn(c, inv, magic)), x = __float_as_uint(__fmaf_rn(d, inv, magic));
+        return __byte_perm(__byte_perm(u, v, 0x0040), __byte_perm(w, x, 0x0040), 0x5410);
+    } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
+    }
+}
+// Two codes in the low half of `x` → two halfs (exact).
 template <int FMT> __device__ __forceinline__ __half2 decode2(uint32_t x) {
     if constexpr (FMT == DX_CACHE_I8) {
         const uint32_t u = __byte_perm((x ^ 0x8080u), 0x64646464u, 0x4140);  // 1024 + (code + 128), twice
@@ -132,25 +145,28 @@ template <int FMT> __device__ __forceinline__ __half2 decode2(uint32_t x) {
     } else {
         uint32_t r;
         asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(x));
-        return __hmin2(*reinterpret_cast<const __half2 *>(&r), __half2half2(__ushort_as_half(0x5F00)));  // 448
+        return *reinterpret_cast<const __half2 *>(&r);
     }
 }
-// Four codes → four halfs, as two pairs: the pairs (0,1) and (2,3) of the word.
-template <int FMT> __device__ __forceinline__ void decode4(uint32_t x, uint32_t &lo, uint32_t &hi) {
+// Four codes → four halfs, as the pairs (0,1) and (2,3) of the word.  FINITE: the codes 0x7F and 0xFF of e4m3, which no cache written
+// here holds, come out as 448, so that what lies behind a mask (a weight of zero) cannot reach a result as a NaN.
+template <int FMT, bool FINITE> __device__ __forceinline__ void decode4(uint32_t x, uint32_t &lo, uint32_t &hi) {
     if constexpr (FMT == DX_CACHE_I8) {
         x ^= 0x80808080u;
         const __half2 off = __half2half2(__ushort_as_half(0x6480));
         lo = __byte_perm(x, 0x64646464u, 0x4140);
         hi = __byte_perm(x, 0x64646464u, 0x4342);
-        __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&lo), off), b = __hsub2(*reinterpret_cast<const __half2 *>(&hi), off);
-        lo = *reinterpret_cast<uint32_t *>(&a);
-        hi = *reinterpret_cast<uint32_t *>(&b);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&lo), off), b = __hsub2(*reinterpret_cast<const __half2 *>(&hi), off);
+        lo = *reinterpret_cast<const uint32_t *>(&a);
+        hi = *reinterpret_cast<const uint32_t *>(&b);
     } else {
         asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(x));
-        const __half2 top = __half2half2(__ushort_as_half(0x5F00));
-        __half2 a = __hmin2(*reinterpret_cast<const __half2 *>(&lo), top), b = __hmin2(*reinterpret_cast<const __half2 *>(&hi), top);
-        lo = *reinterpret_cast<uint32_t *>(&a);
-        hi = *reinterpret_cast<uint32_t *>(&b);
+        if constexpr (FINITE) {
+            const __half2 top = __half2half2(__ushort_as_half(0x5F00));
+            const __half2 a = __hmin2(*reinterpret_cast<const __half2 *>(&lo), top), b = __hmin2(*reinterpret_cast<const __half2 *>(&hi), top);
+            lo = *reinterpret_cast<const uint32_t *>(&a);
+            hi = *reinterpret_cast<const uint32_t *>(&b);
+        }
     }
 }
 #endif

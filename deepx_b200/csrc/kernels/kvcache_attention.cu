@@ -2,13 +2,14 @@
 //
 //   out[t,h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q[t,h].k_j - m),   c = scale log2(e),   j <= pos(t), j > pos(t) - window
 //
-// The rows of one sequence that share a key head (new token i, head i's group: n * group rows) are taken sixteen at a time: one
-// tensor-core tile of queries.  For one new token a sequence this is bound by memory: every code is read once and used for at
-// most sixteen rows.  One pass with the running maximum m and sum of the softmax; codes become halfs exactly, so the only
-// rounding to 16 bits is that of the weights (and each row of a bfloat16 query is brought to size 1 by a power of two first,
-// which keeps its 8 bits; elements 2^-17 below the row's largest begin to lose some).
+// The rows of one sequence that share a key head (new token i, head i's group: n * group rows) are taken eight or sixteen at a time.
+// For one new token a sequence this is bound by memory: every code is read once and used for a few rows.  Keys and values are the
+// tensor cores' 16-row operand (sixteen tokens times a few rows; sixteen dimensions times a few rows), so that a group of up to eight
+// rows wastes nothing and the halfs made of a code serve all rows at once.  One pass with the running maximum m and sum of the
+// softmax; codes become halfs exactly, so the only rounding to 16 bits is that of the weights (and each row of a bfloat16 query is
+// brought to size 1 by a power of two first, which keeps its 8 bits; elements 2^-17 below the row's largest begin to lose some).
 //
-// Work is split over the keys: the 64-token steps of all rows tiles and heads of all sequences stand in one line, and each
+// Work is split over the keys: the 64-token steps of all tiles of rows and heads of all sequences stand in one line, and each
 // block takes an equal piece of it, whatever the lengths are (they are known on the device alone).  A piece may begin or end
 // inside an item (one tile of rows, one head); such items' parts meet in the workspace and a second kernel joins them, always
 // in the order of the keys: the same bits every time.
@@ -21,7 +22,6 @@ namespace kv {
 namespace {
 
 constexpr int WARPS = 4, CTA = WARPS * 32;
-constexpr int ROWS = 16;   // rows of an item
 constexpr int WT = 16;     // tokens a warp takes at a time: never more than one page
 constexpr int STEP = WARPS * WT;
 constexpr int JOIN_CTA = 512;
@@ -49,13 +49,15 @@ struct alignas(32) Join {
     int first_row, rows, head, parts;
 };
 
-template <int DP> struct Cfg {
-    static constexpr int STAGES = DP == 256 ? 3 : 4;
-    static constexpr int BLOCKS = DP == 256 ? 2 : DP == 128 ? 3 : 4;  // resident on an SM
-    static constexpr int TILE = WT * DP;                              // bytes of a warp's keys (or values) of a stage
-    static constexpr int RING = STAGES * 2 * TILE;                    // of a warp; holds its 16 x DP floats at the end
+// DP: the head's dimensions, padded; NB: blocks of eight rows of an item.
+template <int DP, int NB> struct Cfg {
+    static constexpr int ROWS = 8 * NB;
+    static constexpr int STAGES = DP == 64 ? 4 : 3;
+    static constexpr int BLOCKS = DP == 256 ? 2 : NB == 1 ? 4 : 3;  // resident on an SM
+    static constexpr int TILE = WT * DP;                                            // bytes of a warp's keys (or values) of a stage
+    static constexpr int RING = STAGES * 2 * TILE;                                  // of a warp; holds its ROWS x DP floats at the end
     static constexpr int SMEM = WARPS * RING;
-    static constexpr int PART = ROWS * DP + 2 * ROWS;                 // floats of a part in the workspace: output, m, l
+    static constexpr int PART = ROWS * DP + 2 * ROWS;  // floats of a part in the workspace: output, m, l
     static_assert(RING >= ROWS * DP * 4, "the ring holds a warp's output");
 };
 
@@ -83,6 +85,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The transpose of an 8 x 8 matrix of halfs: lane (g, t) gives row g, columns 2t and 2t+1 and takes column g, rows 2t and 2t+1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -106,7 +114,7 @@ template <int DP> __device__ __forceinline__ int key_chunk(int t, int i) { retur
 struct Line {
     int lo, steps, tiles;  // first token of the range (a multiple of STEP), steps of a tile of rows, tiles of rows of a head
 };
-__device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
+template <int ROWS> __device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
     Line l;
     const int64_t hi = min(int64_t(q.end), int64_t(q.first) + q.n);
     const int64_t lo = a.window > 0 ? max(int64_t(0), int64_t(q.first) - a.window + 1) : 0;
@@ -115,16 +123,17 @@ __device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
     l.tiles = int((int64_t(q.n) * a.group + ROWS - 1) / ROWS);
     return l;
 }
-__device__ __forceinline__ int64_t steps_of(const Seqs &s, const Cache &c, const Attn &a, int b) {
+template <int ROWS> __device__ __forceinline__ int64_t steps_of(const Seqs &s, const Cache &c, const Attn &a, int b) {
     const Seq q = seq_at(s, c, b);
     if (q.n == 0) return 0;
-    const Line l = line_of(q, a);
+    const Line l = line_of<ROWS>(q, a);
     return int64_t(l.steps) * l.tiles * c.heads;
 }
 
-template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cfg<DP>::BLOCKS) attention_kernel(Attn a, Cache c, Seqs s) {
-    using K = Cfg<DP>;
-    constexpr int NT = DP / 8;             // column tiles of the output
+template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__(CTA, Cfg<DP, NB>::BLOCKS) attention_kernel(Attn a, Cache c, Seqs s) {
+    using K = Cfg<DP, NB>;
+    constexpr int ROWS = K::ROWS;
+    constexpr int MT = DP / 16;            // tiles of sixteen dimensions of the output
     constexpr int KC = DP / 64;            // chunks of a key that a lane multiplies
     constexpr int VC = DP == 256 ? 2 : 1;  // chunks of a value that a lane multiplies (half of one at DP 64)
     extern __shared__ __align__(1024) uint8_t ring[];
@@ -142,7 +151,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
     const int per = (s.batch + CTA - 1) / CTA;
     {
         int64_t mine = 0;
-        for (int b = threadIdx.x * per; b < min(s.batch, int(threadIdx.x + 1) * per); ++b) mine += steps_of(s, c, a, b);
+        for (int b = threadIdx.x * per; b < min(s.batch, int(threadIdx.x + 1) * per); ++b) mine += steps_of<ROWS>(s, c, a, b);
         int64_t sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -171,7 +180,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
         int64_t at = before[threadIdx.x];
         int b = threadIdx.x * per;
         for (; b < s.batch; ++b) {
-            const int64_t n = steps_of(s, c, a, b);
+            const int64_t n = steps_of<ROWS>(s, c, a, b);
             if (at + n > begin) break;
             at += n;
         }
@@ -185,9 +194,12 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
 
     uint8_t *my_ring = ring + warp * K::RING;
     const uint32_t ring_u = smem_u32(my_ring);
+    // the sixteen bytes of a tile that this lane loads first; the others lie whole rows further
+    const int lane_row = lane / (DP / 16), lane_chunk = lane % (DP / 16), lane_src = lane_row * c.dim + lane_chunk * 16, row_step = (512 / DP) * c.dim;
+    const bool lane_in = lane_chunk * 16 < c.dim;
     for (int64_t at = begin; at < end;) {
         const Seq sq = seq_at(s, c, b);
-        const Line ln = line_of(sq, a);
+        const Line ln = line_of<ROWS>(sq, a);
         const int64_t seq_steps = sq.n ? int64_t(ln.steps) * ln.tiles * c.heads : 0;
         if (at >= seq_begin + seq_steps) {  // on to the next sequence
             seq_begin += seq_steps;
@@ -201,16 +213,15 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
         const int rows = min(ROWS, int(min(int64_t(sq.n) * a.group - first_row, int64_t(ROWS))));
         const int steps = step1 - step0;
 
-        // ---- the queries: row g and row g + 8 of the item, the chunks this lane multiplies ----
-        uint32_t qa[KC][4][4];
-        float c_row[2];
-        int pos[2];
+        // ---- the queries: row g of each block of eight, the chunks this lane multiplies ----
+        uint32_t qb[NB][KC][4][2];
+        float c_row[NB][2];  // of the rows 2t and 2t + 1, whose scores this lane has
+        int pos[NB][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int fr = first_row + g + 8 * r;
-            const bool live = g + 8 * r < rows;
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g, fr = first_row + r;
+            const bool live = r < rows;
             const int i = live ? fr / a.group : 0;
-            pos[r] = live ? sq.first + i : INT32_MIN;
             const T *q = static_cast<const T *>(a.q) + (sq.row0 + i) * a.q_stride + int64_t(head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
             Pack<T, 8> x[KC][2];
             float amax = 0.f;
@@ -228,15 +239,14 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
                     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k][h].v[e])));
                 }
             }
-            float down = 1.f;
-            c_row[r] = a.scale_log2;
+            float down = 1.f, c_mine = a.scale_log2;
             if constexpr (std::is_same<T, bf16>::value) {
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
                 if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
                     down = __uint_as_float((254u - e) << 23);
-                    c_row[r] *= __uint_as_float(e << 23);
+                    c_mine *= __uint_as_float(e << 23);
                 }
             }
 #pragma unroll
@@ -245,18 +255,30 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
                 for (int w = 0; w < 4; ++w) {  // word w of the chunk: dimensions 4w..4w+3
                     const Pack<T, 8> &p = x[k][w >> 1];
                     const int e = (w & 1) * 4;
-                    qa[k][w][r] = half2_bits(to_compute(p.v[e]) * down, to_compute(p.v[e + 1]) * down);
-                    qa[k][w][2 + r] = half2_bits(to_compute(p.v[e + 2]) * down, to_compute(p.v[e + 3]) * down);
+                    qb[nb][k][w][0] = half2_bits(to_compute(p.v[e]) * down, to_compute(p.v[e + 1]) * down);
+                    qb[nb][k][w][1] = half2_bits(to_compute(p.v[e + 2]) * down, to_compute(p.v[e + 3]) * down);
                 }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = 8 * nb + 2 * t + e;
+                c_row[nb][e] = __shfl_sync(0xffffffffu, c_mine, (2 * t + e) * 4);
+                pos[nb][e] = col < rows ? sq.first + (first_row + col) / a.group : INT32_MIN;
+            }
         }
         const int pos_min = sq.first + first_row / a.group, pos_max = sq.first + (first_row + rows - 1) / a.group;
         const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's
 
-        float o[NT][4], l[4] = {}, m[2] = {NEG_INF, NEG_INF}, v_ref = 0.f;
+        float o[NB][MT][4], l[NB][4], m[NB][2], v_ref = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb][0] = m[nb][1] = NEG_INF;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) {
+                l[nb][e] = 0.f;
+#pragma unroll
+                for (int d = 0; d < MT; ++d) o[nb][d][e] = 0.f;
+            }
+        }
 
         // ---- keys and values in flight ----
         const int32_t *table = s.table + int64_t(b) * s.cols;
@@ -268,19 +290,23 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
         auto issue = [&](int step, int stage, int32_t number) {
             if (step < steps) {
                 const int j = token0(step);
-                const bool some = j < seen_end;
-                const bool ok = some && number >= 0 && number < c.pages;
-                if (some && !ok && lane == 0) raise(a.flag, FLAG_PAGE);
+                const int left = seen_end - j;  // tokens to load
+                const bool ok = left > 0 && number >= 0 && number < c.pages;
+                if (left > 0 && !ok && lane == 0) raise(a.flag, FLAG_PAGE);
                 const int64_t ph = ok ? int64_t(number) * c.heads + head : 0;
-                const int64_t base = (ph * c.page + (j & (c.page - 1))) * c.dim;
+                const int64_t base = ok ? (ph * c.page + (j & (c.page - 1))) * c.dim + lane_src : 0;
                 const uint32_t dst = ring_u + stage * 2 * K::TILE;
+                const uint8_t *ksrc = c.k + base, *vsrc = c.v + base;
 #pragma unroll
                 for (int i = 0; i < K::TILE / 512; ++i) {
-                    const int idx = i * 32 + lane, r = idx / (DP / 16), ch = idx % (DP / 16);
-                    const bool in = ok && j + r < seen_end && ch * 16 < c.dim;
-                    const int64_t off = in ? base + r * c.dim + ch * 16 : 0;
-                    cp_async16(dst + place<DP>(r, ch), c.k + off, in);
-                    cp_async16(dst + K::TILE + place<DP>(r, ch), c.v + off, in);
+                    const bool in = ok && lane_in && i * (512 / DP) + lane_row < left;
+                    const uint32_t at = dst + place<DP>(i * (512 / DP) + lane_row, lane_chunk);
+                    cp_async16(at, ksrc, in);
+                    cp_async16(at + K::TILE, vsrc, in);
+                    if (in) {
+                        ksrc += row_step;
+                        vsrc += row_step;
+                    }
                 }
                 if (lane < 2) cp_async4(smem_u32(&scales[warp][stage][lane]), (lane ? c.v_scale : c.k_scale) + ph, ok);
                 if (lane == 2) in_cache[warp][stage] = ok;
@@ -298,7 +324,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
         int stage = 0;
         for (int step = 0; step < steps; ++step) {
             cp_wait<K::STAGES - 2>();
-            __syncwarp();
+            __syncwarp();  // the stage has arrived, and every lane is done with the one before it
             {
                 const int32_t number = next;
                 next = page_number(step + K::STAGES);
@@ -309,153 +335,157 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
             const bool ok = in_cache[warp][stage];
             const int j0 = token0(step);
             if (++stage == K::STAGES) stage = 0;
-            if (!ok) {
-                __syncwarp();
-                continue;  // no token of a page: nothing to see
-            }
+            if (!ok) continue;  // no token of a page: nothing to see
 
-            // ---- scores of sixteen rows and sixteen tokens: lane (g, t) holds rows g, g+8 and tokens 2t, 2t+1, 2t+8, 2t+9 ----
-            float x[2][4] = {};
+            // ---- scores: lane (g, t) holds tokens g, g+8 of rows 2t, 2t+1 ----
+            float x[NB][4];
 #pragma unroll
-            for (int k = 0; k < KC; ++k)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint4 w = lds128(ks + place<DP>(g + 8 * n, key_chunk<DP>(t, k)));
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                for (int e = 0; e < 4; ++e) x[nb][e] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t b0, b1;
-                        decode4<FMT>(ww[i], b0, b1);
-                        mma(x[n], qa[k][i], b0, b1);
-                    }
+            for (int k = 0; k < KC; ++k) {
+                const uint4 w0 = lds128(ks + place<DP>(g, key_chunk<DP>(t, k))), w1 = lds128(ks + place<DP>(g + 8, key_chunk<DP>(t, k)));
+                const uint32_t lo[4] = {w0.x, w0.y, w0.z, w0.w}, hi[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t ka[4];
+                    decode4<FMT, false>(lo[i], ka[0], ka[2]);
+                    decode4<FMT, false>(hi[i], ka[1], ka[3]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) mma(x[nb], ka, qb[nb][k][i][0], qb[nb][k][i][1]);
                 }
-            const float c0 = c_row[0] * k_scale, c1 = c_row[1] * k_scale;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                x[n][0] *= c0;
-                x[n][1] *= c0;
-                x[n][2] *= c1;
-                x[n][3] *= c1;
             }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[nb][e] *= c_row[nb][e & 1] * k_scale;
             if (j0 + WT - 1 > pos_min || j0 + WT > sq.end || (a.window > 0 && j0 <= int64_t(pos_max) - a.window)) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int j = j0 + 8 * n + 2 * t + (e & 1), p = pos[e >> 1];
+                        const int j = j0 + g + 8 * (e >> 1), p = pos[nb][e & 1];
                         const bool seen = j <= p && j < sq.end && (a.window <= 0 || j > int64_t(p) - a.window);
-                        if (!seen) x[n][e] = NEG_INF;
+                        if (!seen) x[nb][e] = NEG_INF;
                     }
             }
             // ---- running maximum: a row's rises when a score is 2^8 above it ----
-            float top[2];
+            float top[NB][2];
             bool rise = false;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float v = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                top[r] = v > m[r] + LAG ? v : m[r];
-                rise |= top[r] != m[r];
-            }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v = fmaxf(x[nb][e], x[nb][e + 2]);
+                    rise |= v > m[nb][e] + LAG;
+                    top[nb][e] = v;
+                }
             const bool scale_up = v_scale > v_ref;
             if (__any_sync(0xffffffffu, rise) || scale_up) {
                 const float turn = scale_up ? v_ref / v_scale : 1.f;  // values in units of the largest scale so far
                 if (scale_up) v_ref = v_scale;
-                float by[2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    by[r] = top[r] == m[r] ? 1.f : exp2_approx(m[r] - top[r]);
-                    m[r] = top[r];
-                    l[2 * r] *= by[r];
-                    l[2 * r + 1] *= by[r];
-                    by[r] *= turn;
-                }
+                for (int nb = 0; nb < NB; ++nb) {
+                    float by[2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    o[n][0] *= by[0];
-                    o[n][1] *= by[0];
-                    o[n][2] *= by[1];
-                    o[n][3] *= by[1];
+                    for (int e = 0; e < 2; ++e) {
+                        float v = top[nb][e];
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                        v = v > m[nb][e] + LAG ? v : m[nb][e];
+                        by[e] = v == m[nb][e] ? 1.f : exp2_approx(m[nb][e] - v);
+                        m[nb][e] = v;
+                        l[nb][e] *= by[e];
+                        by[e] *= turn;
+                    }
+#pragma unroll
+                    for (int d = 0; d < MT; ++d) {
+                        o[nb][d][0] *= by[0];
+                        o[nb][d][1] *= by[1];
+                        o[nb][d][2] *= by[0];
+                        o[nb][d][3] *= by[1];
+                    }
                 }
             }
-            const float m0 = (m[0] == NEG_INF ? 0.f : m[0]) - UP, m1 = (m[1] == NEG_INF ? 0.f : m[1]) - UP;
-            uint32_t p[4];
-            p[0] = half2_bits(exp2_approx(x[0][0] - m0), exp2_approx(x[0][1] - m0));
-            p[1] = half2_bits(exp2_approx(x[0][2] - m1), exp2_approx(x[0][3] - m1));
-            p[2] = half2_bits(exp2_approx(x[1][0] - m0), exp2_approx(x[1][1] - m0));
-            p[3] = half2_bits(exp2_approx(x[1][2] - m1), exp2_approx(x[1][3] - m1));
-            mma(l, p, 0x3C003C00u, 0x3C003C00u);  // the sum of the very weights that multiply the values
+            uint32_t p[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float m0 = (m[nb][0] == NEG_INF ? 0.f : m[nb][0]) - UP, m1 = (m[nb][1] == NEG_INF ? 0.f : m[nb][1]) - UP;
+                p[nb][0] = transpose8(half2_bits(exp2_approx(x[nb][0] - m0), exp2_approx(x[nb][1] - m1)));
+                p[nb][1] = transpose8(half2_bits(exp2_approx(x[nb][2] - m0), exp2_approx(x[nb][3] - m1)));
+                const uint32_t one[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+                mma(l[nb], one, p[nb][0], p[nb][1]);  // the sum of the very weights that multiply the values
+            }
 
             // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
             const bool same = v_scale == v_ref;
             const __half2 unit = __float2half2_rn(v_scale / v_ref);
-            auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int n) {
-                uint32_t b0[4], b1[4];
-                decode4<FMT>(__byte_perm(wa, wb, 0x5140), b0[0], b0[1]);
-                decode4<FMT>(__byte_perm(wa, wb, 0x7362), b0[2], b0[3]);
-                decode4<FMT>(__byte_perm(wc, wd, 0x5140), b1[0], b1[1]);
-                decode4<FMT>(__byte_perm(wc, wd, 0x7362), b1[2], b1[3]);
+            auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
+                uint32_t v0[4], v1[4];  // of dimensions 2 tile, 2 tile + 1 and the two after: tokens 2t.., tokens 2t + 8..
+                decode4<FMT, true>(__byte_perm(wa, wb, 0x5140), v0[0], v0[1]);
+                decode4<FMT, true>(__byte_perm(wc, wd, 0x5140), v0[2], v0[3]);
+                decode4<FMT, true>(__byte_perm(wa, wb, 0x7362), v1[0], v1[1]);
+                decode4<FMT, true>(__byte_perm(wc, wd, 0x7362), v1[2], v1[3]);
                 if (!same) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const __half2 u = __hmul2(*reinterpret_cast<__half2 *>(&b0[i]), unit), w = __hmul2(*reinterpret_cast<__half2 *>(&b1[i]), unit);
-                        b0[i] = *reinterpret_cast<const uint32_t *>(&u);
-                        b1[i] = *reinterpret_cast<const uint32_t *>(&w);
+                        const __half2 u = __hmul2(*reinterpret_cast<__half2 *>(&v0[i]), unit), w = __hmul2(*reinterpret_cast<__half2 *>(&v1[i]), unit);
+                        v0[i] = *reinterpret_cast<const uint32_t *>(&u);
+                        v1[i] = *reinterpret_cast<const uint32_t *>(&w);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma(o[n + i], p, b0[i], b1[i]);
+                for (int nb = 0; nb < NB; ++nb) {
+                    mma(o[nb][tile], v0, p[nb][0], p[nb][1]);
+                    mma(o[nb][tile + 1], v1, p[nb][0], p[nb][1]);
+                }
             };
             if constexpr (DP == 64) {
                 const int half = (g & 1) * 8;
                 const uint2 wa = lds64(vs + place<DP>(2 * t, g >> 1) + half), wb = lds64(vs + place<DP>(2 * t + 1, g >> 1) + half);
                 const uint2 wc = lds64(vs + place<DP>(2 * t + 8, g >> 1) + half), wd = lds64(vs + place<DP>(2 * t + 9, g >> 1) + half);
                 four(wa.x, wb.x, wc.x, wd.x, 0);
-                four(wa.y, wb.y, wc.y, wd.y, 4);
+                four(wa.y, wb.y, wc.y, wd.y, 2);
             } else {
 #pragma unroll
                 for (int h = 0; h < VC; ++h) {
                     const int ch = g + 8 * h;
                     const uint4 wa = lds128(vs + place<DP>(2 * t, ch)), wb = lds128(vs + place<DP>(2 * t + 1, ch));
                     const uint4 wc = lds128(vs + place<DP>(2 * t + 8, ch)), wd = lds128(vs + place<DP>(2 * t + 9, ch));
-                    four(wa.x, wb.x, wc.x, wd.x, 16 * h);
-                    four(wa.y, wb.y, wc.y, wd.y, 16 * h + 4);
-                    four(wa.z, wb.z, wc.z, wd.z, 16 * h + 8);
-                    four(wa.w, wb.w, wc.w, wd.w, 16 * h + 12);
+                    four(wa.x, wb.x, wc.x, wd.x, 8 * h);
+                    four(wa.y, wb.y, wc.y, wd.y, 8 * h + 2);
+                    four(wa.z, wb.z, wc.z, wd.z, 8 * h + 4);
+                    four(wa.w, wb.w, wc.w, wd.w, 8 * h + 6);
                 }
             }
-            __syncwarp();  // the stage may be filled again
         }
         cp_wait<0>();
         __syncthreads();  // every warp is done with its ring
 
         // ---- the four warps' parts, each divided by its own sum, into the rings ----
         constexpr int W = DP == 64 ? 8 : 16;  // dimensions of a lane's run
+        auto in_part = [&](int row, int d) { return row * DP + (((d >> 2) ^ ((row >> 1) & 3)) << 2); };
         float *mine = reinterpret_cast<float *>(my_ring);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float sum = l[2 * r], by = sum == 0.f ? 0.f : v_ref / sum;
-            const int row = g + 8 * r;
-            if (t == 0) {
-                sm_m[warp][row] = m[r];
-                sm_l[warp][row] = sum;
-            }
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int h = 0; h < VC; ++h)
+            for (int e = 0; e < 2; ++e) {
+                const float sum = l[nb][e], by = sum == 0.f ? 0.f : v_ref / sum;
+                const int row = 8 * nb + 2 * t + e;
+                if (g == 0) {
+                    sm_m[warp][row] = m[nb][e];
+                    sm_l[warp][row] = sum;
+                }
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int h = 0; h < VC; ++h)
 #pragma unroll
                     for (int i = 0; i < W; i += 4) {
-                        const int d = h * 128 + (2 * t + e) * W + i;
-                        float4 v;
-                        v.x = o[h * 16 + i][2 * r + e] * by;
-                        v.y = o[h * 16 + i + 1][2 * r + e] * by;
-                        v.z = o[h * 16 + i + 2][2 * r + e] * by;
-                        v.w = o[h * 16 + i + 3][2 * r + e] * by;
-                        *reinterpret_cast<float4 *>(mine + row * DP + (((d >> 2) ^ ((((d >> 5) & 3) << 1) | (row & 1))) << 2)) = v;
+                        const int d = h * 128 + g * W + i, tile = h * 8 + i / 2;
+                        *reinterpret_cast<float4 *>(mine + in_part(row, d)) =
+                            make_float4(o[nb][tile][e] * by, o[nb][tile][2 + e] * by, o[nb][tile + 1][e] * by, o[nb][tile + 1][2 + e] * by);
                     }
-        }
+            }
         __syncthreads();
         const bool whole = step0 == 0 && step1 == ln.steps;
         float *part = parts + (int64_t(blockIdx.x) * 2 + (step0 == 0 ? 1 : 0)) * K::PART;
@@ -470,8 +500,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float by = sm_l[w][row] * exp2_approx(sm_m[w][row] - base);
-                const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring + w * K::RING) + row * DP +
-                                                                  (((d >> 2) ^ ((((d >> 5) & 3) << 1) | (row & 1))) << 2));
+                const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring + w * K::RING) + in_part(row, d));
                 sum += by;
                 v.x += by * x.x;
                 v.y += by * x.y;
@@ -519,8 +548,8 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(CTA, Cf
 
 // Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
 // of the keys.  Sixteen warps share the item's rows; the warps of a row share its parts.
-template <typename T, int DP> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
-    constexpr int V = DP / 32;
+template <typename T, int DP, int NB> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
+    constexpr int V = DP / 32, ROWS = Cfg<DP, NB>::ROWS;
     __shared__ float sh[JOIN_CTA / 32][DP];
     griddep_wait_cta();
     const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
@@ -530,7 +559,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(JOIN_CTA) join_k
     const int each = j.rows > 8 ? 1 : j.rows > 4 ? 2 : j.rows > 2 ? 4 : j.rows > 1 ? 8 : 16;  // warps of a row
     const int row = warp / each, sub = warp % each;
     // part 0: the second part of block i - 1; part p > 0: the first of block i - 1 + p
-    auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * Cfg<DP>::PART; };
+    auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * Cfg<DP, NB>::PART; };
     float acc[V] = {}, sum = 0.f;
     if (row < j.rows) {
         float top = NEG_INF;
@@ -581,22 +610,37 @@ template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_
     return e == cudaSuccess ? DX_OK : fail(DX_E_CUDA, "kvcache_attention: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+template <typename T, int FMT, int DP, int NB> int launch_rows(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+    using K = Cfg<DP, NB>;
     static std::atomic<uint64_t> prepared{0};  // one bit for each device
-    if (int e = allow_shared(attention_kernel<T, FMT, DP>, Cfg<DP>::SMEM, &prepared)) return e;
-    const unsigned grid = unsigned(sm_count() * Cfg<DP>::BLOCKS);
-    launch_pdl(attention_kernel<T, FMT, DP>, dim3(grid), dim3(CTA), Cfg<DP>::SMEM, st, a, c, s);
+    if (int e = allow_shared(attention_kernel<T, FMT, DP, NB>, K::SMEM, &prepared)) return e;
+    const unsigned grid = unsigned(sm_count() * K::BLOCKS);
+    launch_pdl(attention_kernel<T, FMT, DP, NB>, dim3(grid), dim3(CTA), K::SMEM, st, a, c, s);
     if (int e = check_launch("kvcache_attention")) return e;
-    launch_pdl(join_kernel<T, DP>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
+    launch_pdl(join_kernel<T, DP, NB>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
     return check_launch("kvcache_attention (join)");
 }
+template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, int64_t rows, cudaStream_t st) {
+    if (rows <= 8) return launch_rows<T, FMT, DP, 1>(a, c, s, st);
+    return launch_rows<T, FMT, DP, 2>(a, c, s, st);
+}
 
+template <int DP, int NB> size_t workspace_of() {
+    using K = Cfg<DP, NB>;
+    return size_t(sm_count()) * K::BLOCKS * (sizeof(Join) + 2 * K::PART * sizeof(float));
+}
+template <int DP> size_t workspace_rows(int64_t rows) { return rows <= 8 ? workspace_of<DP, 1>() : workspace_of<DP, 2>(); }
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-size_t workspace(int dim) {
-    const int dp = padded(dim);
-    const size_t blocks = size_t(sm_count()) * (dp == 64 ? Cfg<64>::BLOCKS : dp == 128 ? Cfg<128>::BLOCKS : Cfg<256>::BLOCKS);
-    const size_t part = dp == 64 ? Cfg<64>::PART : dp == 128 ? Cfg<128>::PART : Cfg<256>::PART;
-    return blocks * (sizeof(Join) + 2 * part * sizeof(float));
+size_t workspace(int dim, int64_t rows) {
+    switch (padded(dim)) {
+        case 64: return workspace_rows<64>(rows);
+        case 128: return workspace_rows<128>(rows);
+        default: return workspace_rows<256>(rows);
+    }
+}
+// The most rows of a sequence that share a key head, as far as the caller says.
+int64_t rows_of(int64_t q_heads, const Cache &c, const Seqs &s, int64_t max_new) {
+    return (max_new > 0 && max_new < s.rows ? max_new : s.rows) * (q_heads / c.heads);
 }
 
 }  // namespace
@@ -608,7 +652,7 @@ extern "C" size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_head
     kv::Cache c;
     kv::Seqs s;
     if (kv::check("kvcache_attention", cache, seqs, &c, &s) || s.rows == 0 || s.batch == 0) return 0;
-    return kv::workspace(c.dim);
+    return kv::workspace(c.dim, kv::rows_of(q_heads, c, s, max_new));
 }
 
 extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
@@ -631,7 +675,8 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     const int64_t codes = c.pages * c.heads * int64_t(c.page) * c.dim;
     if (kv::overlap(q, qb, out, ob) || kv::overlap(out, ob, c.k, codes) || kv::overlap(out, ob, c.v, codes))
         return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
-    const size_t need = kv::workspace(c.dim);
+    const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
+    const size_t need = kv::workspace(c.dim, rows);
     if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
     kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),
@@ -639,9 +684,9 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     cudaStream_t st = as_stream(stream);
 #define DX_CALL(T, FMT)                                                             \
     switch (kv::padded(c.dim)) {                                                    \
-        case 64: return kv::launch<T, FMT, 64>(a, c, s, st);                        \
-        case 128: return kv::launch<T, FMT, 128>(a, c, s, st);                      \
-        default: return kv::launch<T, FMT, 256>(a, c, s, st);                       \
+        case 64: return kv::launch<T, FMT, 64>(a, c, s, rows, st);                        \
+        case 128: return kv::launch<T, FMT, 128>(a, c, s, rows, st);                      \
+        default: return kv::launch<T, FMT, 256>(a, c, s, rows, st);                       \
     }
     if (dtype == DX_F16) {
         if (cache->format == DX_CACHE_I8) { DX_CALL(f16, DX_CACHE_I8) }

@@ -23,14 +23,15 @@ struct RopeArgs {
     int pos64;
 };
 
-__device__ __forceinline__ void angles(const RopeArgs &a, int64_t token, float2 *cs) {
-    const double pos = a.pos64 ? double(static_cast<const int64_t *>(a.positions)[token]) : double(static_cast<const int32_t *>(a.positions)[token]);
-    for (int i = threadIdx.x; i < a.rotated / 2; i += blockDim.x) {
-        const double turns = pos * double(a.inv_freq[i]) * 0.15915494309189533577;  // 1 / (2 pi)
-        float s, c;
-        sincospif(2.f * float(turns - rint(turns)), &s, &c);
-        cs[i] = make_float2(c, s);
-    }
+__device__ __forceinline__ double position(const RopeArgs &a, int64_t token) {
+    return a.pos64 ? double(static_cast<const int64_t *>(a.positions)[token]) : double(static_cast<const int32_t *>(a.positions)[token]);
+}
+// (cosine, sine) of the angle pos * inv_freq
+__device__ __forceinline__ float2 turn_of(double pos, float inv_freq) {
+    const double turns = pos * double(inv_freq) * 0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif(2.f * float(turns - rint(turns)), &s, &c);
+    return make_float2(c, s);
 }
 
 // Any head size, stride and alignment: a warp takes a head, its elements in shared memory.
@@ -38,7 +39,8 @@ template <typename T> __global__ void __launch_bounds__(CTA) qknorm_rope_any_ker
     __shared__ float2 cs[DX_ROPE_MAX_DIM / 2];
     __shared__ float row[CTA / 32][DX_ROPE_MAX_DIM];
     const int64_t token = blockIdx.x;
-    angles(a, token, cs);
+    griddep_wait_cta();
+    for (int i = threadIdx.x; i < a.rotated / 2; i += CTA) cs[i] = turn_of(position(a, token), a.inv_freq[i]);
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float *y = row[warp];
@@ -74,6 +76,170 @@ template <typename T> __global__ void __launch_bounds__(CTA) qknorm_rope_any_ker
         for (int i = a.rotated + lane; i < a.dim; i += 32) o[i] = from_compute<T>(y[i]);
         __syncwarp();
     }
+}
+
+// Whole 16-byte vectors: LANES threads share a head, each with one UNIT of sixteen elements, two chunks of eight.  In the rotated
+// part a unit is a chunk and its partner half the rotated part further (or, interleaved, two chunks side by side): both elements of
+// every pair are in one thread, so the rotation needs no exchange.  A block takes `per_block` tokens, whose angles are in shared
+// memory; the first head's elements are loaded before the angles are worked out.
+template <typename T> struct Eight {
+    static constexpr int N = 16 / sizeof(T), P = 8 / N;
+    Pack<T, N> p[P];
+    __device__ __forceinline__ void load(const T *x) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) p[i] = ld_stream<T, N>(x + i * N);
+    }
+    __device__ __forceinline__ void load_weight(const T *x) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) p[i] = ld_cached<T, N>(x + i * N);
+    }
+    __device__ __forceinline__ void store(T *x) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) st_stream<T, N>(x + i * N, p[i]);
+    }
+    __device__ __forceinline__ float get(int e) const { return to_compute(p[e / N].v[e % N]); }
+    __device__ __forceinline__ void set(int e, float f) { p[e / N].v[e % N] = from_compute<T>(f); }
+};
+
+template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_bounds__(CTA) qknorm_rope_kernel(RopeArgs a, int per_block, FastDiv by_heads) {
+    extern __shared__ __align__(16) float shared[];
+    // two weights of 16 * LANES, then [per_block][rotated / 2] pairs of cosine and sine
+    float *weights = shared;
+    float2 *cs = reinterpret_cast<float2 *>(shared + 2 * 16 * LANES);
+    griddep_wait_cta();
+    const int heads = a.q_heads + a.k_heads, half = a.rotated / 2;
+    const int64_t token0 = int64_t(blockIdx.x) * per_block;
+    const int tokens = int(min(int64_t(per_block), a.tokens - token0));
+    const int team = threadIdx.x / LANES, u = threadIdx.x % LANES;
+    const int chunks = a.dim / 8, rotated_units = INTERLEAVED ? 0 : half / 8;
+    const bool apart = u < rotated_units;  // the rest: two chunks side by side
+    const int first = apart ? u : 2 * u, second = apart ? u + rotated_units : 2 * u + 1;
+    const bool has0 = first < chunks, has1 = second < chunks;
+    const int rows = tokens * heads;
+    const T *const q = static_cast<const T *>(a.q) + token0 * a.q_stride, *const k = static_cast<const T *>(a.k) + token0 * a.k_stride;
+    T *const qo = static_cast<T *>(a.qo) + token0 * a.qo_stride, *const ko = static_cast<T *>(a.ko) + token0 * a.ko_stride;
+    Eight<T> x0, x1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // what a short last unit does not have stays zero
+        x0.set(e, 0.f);
+        x1.set(e, 0.f);
+    }
+    auto load = [&](int row) {
+        const int t = int(fd_div(uint32_t(row), by_heads)), h = row - t * heads;
+        const T *x = h < a.q_heads ? q + t * a.q_stride + h * a.dim : k + t * a.k_stride + (h - a.q_heads) * a.dim;
+        if (has0) x0.load(x + first * 8);
+        if (has1) x1.load(x + second * 8);
+    };
+    if (team < rows) load(team);
+    if (a.norm) {
+        for (int i = threadIdx.x; i < 2 * a.dim; i += CTA) {
+            const bool is_k = i >= a.dim;
+            const int d = i - (is_k ? a.dim : 0);
+            const T *w = static_cast<const T *>(is_k ? a.kw : a.qw);
+            weights[(is_k ? 16 * LANES : 0) + d] = w ? to_compute(w[d]) : 1.f;
+        }
+    }
+    for (int i = threadIdx.x; i < tokens * half; i += CTA) {
+        const int t = i / half, f = i - t * half;
+        cs[i] = turn_of(position(a, token0 + t), a.inv_freq[f]);
+    }
+    __syncthreads();
+    // every thread of a warp takes the same number of turns: the sums are warp shuffles
+    for (int row0 = 0; row0 < rows; row0 += CTA / LANES) {
+        const int row = row0 + team;
+        const bool live = row < rows;
+        if (row0 > 0 && live) load(row);
+        float y0[8], y1[8], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            y0[e] = x0.get(e);
+            y1[e] = x1.get(e);
+            sum += y0[e] * y0[e];
+            sum += y1[e] * y1[e];
+        }
+        const int t = int(fd_div(uint32_t(row), by_heads)), h = row - t * heads;
+        const bool is_q = h < a.q_heads;
+        if (a.norm) {
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float r = 1.f / sqrtf(sum / float(a.dim) + a.eps);
+            const float *w = weights + (is_q ? 0 : 16 * LANES);
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 w0 = *reinterpret_cast<const float4 *>(w + (has0 ? first : 0) * 8 + e), w1 = *reinterpret_cast<const float4 *>(w + (has1 ? second : 0) * 8 + e);
+                const float m0[4] = {w0.x, w0.y, w0.z, w0.w}, m1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    y0[e + d] *= r * m0[d];
+                    y1[e + d] *= r * m1[d];
+                }
+            }
+        }
+        if (!live) continue;
+        const float2 *turn = cs + t * half;
+        if constexpr (INTERLEAVED) {
+            auto rotate = [&](float (&y)[8], int chunk) {
+                if (chunk * 8 >= a.rotated) return;
+#pragma unroll
+                for (int p = 0; p < 4; p += 2) {
+                    const float4 c = *reinterpret_cast<const float4 *>(turn + chunk * 4 + p);
+                    const float s = y[2 * p], v = y[2 * p + 1], z = y[2 * p + 2], w = y[2 * p + 3];
+                    y[2 * p] = s * c.x - v * c.y;
+                    y[2 * p + 1] = v * c.x + s * c.y;
+                    y[2 * p + 2] = z * c.z - w * c.w;
+                    y[2 * p + 3] = w * c.z + z * c.w;
+                }
+            };
+            rotate(y0, first);
+            rotate(y1, second);
+        } else if (apart) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float4 c = *reinterpret_cast<const float4 *>(turn + u * 8 + e);
+                const float s = y0[e], v = y1[e], z = y0[e + 1], w = y1[e + 1];
+                y0[e] = s * c.x - v * c.y;
+                y1[e] = v * c.x + s * c.y;
+                y0[e + 1] = z * c.z - w * c.w;
+                y1[e + 1] = w * c.z + z * c.w;
+            }
+        }
+        T *o = is_q ? qo + t * a.qo_stride + h * a.dim : ko + t * a.ko_stride + (h - a.q_heads) * a.dim;
+        Eight<T> z0, z1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            z0.set(e, y0[e]);
+            z1.set(e, y1[e]);
+        }
+        if (has0) z0.store(o + first * 8);
+        if (has1) z1.store(o + second * 8);
+    }
+}
+
+template <typename T, int LANES> void launch_lanes(const RopeArgs &a, cudaStream_t st) {
+    // enough blocks for every SM's eight, then up to sixteen tokens each
+    int per_block = 1;
+    while (per_block < 16 && a.tokens > int64_t(sm_count()) * 8 * per_block) per_block *= 2;
+    const unsigned grid = unsigned((a.tokens + per_block - 1) / per_block);
+    const size_t smem = 2 * 16 * LANES * sizeof(float) + size_t(per_block) * (a.rotated / 2) * sizeof(float2);
+    const FastDiv by_heads = make_fastdiv(unsigned(a.q_heads + a.k_heads));
+    if (a.interleaved) launch_pdl(qknorm_rope_kernel<T, LANES, true>, dim3(grid), dim3(CTA), smem, st, a, per_block, by_heads);
+    else launch_pdl(qknorm_rope_kernel<T, LANES, false>, dim3(grid), dim3(CTA), smem, st, a, per_block, by_heads);
+}
+
+template <typename T> void launch_rope(const RopeArgs &a, cudaStream_t st) {
+    constexpr int N = 16 / sizeof(T);
+    bool vec = a.dim % 8 == 0 && a.rotated % (a.interleaved ? 8 : 16) == 0;
+    for (const void *p : {a.q, a.k, a.qw, a.kw, static_cast<const void *>(a.qo), static_cast<const void *>(a.ko)}) vec = vec && aligned_to(p, 16);
+    for (int64_t stride : {a.q_heads ? a.q_stride : 0, a.k_heads ? a.k_stride : 0, a.q_heads ? a.qo_stride : 0, a.k_heads ? a.ko_stride : 0}) vec = vec && stride % N == 0;
+    if (!vec) {
+        launch_pdl(qknorm_rope_any_kernel<T>, dim3(unsigned(a.tokens)), dim3(CTA), 0, st, a);
+        return;
+    }
+    const int units = (a.dim + 15) / 16;
+    if (units <= 4) launch_lanes<T, 4>(a, st);
+    else if (units <= 8) launch_lanes<T, 8>(a, st);
+    else if (units <= 16) launch_lanes<T, 16>(a, st);
+    else launch_lanes<T, 32>(a, st);
 }
 
 }  // namespace
@@ -120,9 +286,9 @@ extern "C" int dx_qknorm_rope(int dtype, const void *q, int64_t q_stride, int64_
                int(head_dim), int(rotated), interleaved, norm, float(eps), inv_freq, positions, pos_dtype == DX_I64};
     cudaStream_t st = as_stream(stream);
     switch (dtype) {
-        case DX_F32: qknorm_rope_any_kernel<float><<<unsigned(tokens), CTA, 0, st>>>(a); break;
-        case DX_F16: qknorm_rope_any_kernel<f16><<<unsigned(tokens), CTA, 0, st>>>(a); break;
-        default: qknorm_rope_any_kernel<bf16><<<unsigned(tokens), CTA, 0, st>>>(a); break;
+        case DX_F32: launch_rope<float>(a, st); break;
+        case DX_F16: launch_rope<f16>(a, st); break;
+        default: launch_rope<bf16>(a, st); break;
     }
     return check_launch("qknorm_rope");
 }
