@@ -297,15 +297,21 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                 const int64_t base = ok ? (ph * c.page + (j & (c.page - 1))) * c.dim + lane_src : 0;
                 const uint32_t dst = ring_u + stage * 2 * K::TILE;
                 const uint8_t *ksrc = c.k + base, *vsrc = c.v + base;
+                if (ok && left >= WT && c.dim == DP) {
 #pragma unroll
-                for (int i = 0; i < K::TILE / 512; ++i) {
-                    const bool in = ok && lane_in && i * (512 / DP) + lane_row < left;
-                    const uint32_t at = dst + place<DP>(i * (512 / DP) + lane_row, lane_chunk);
-                    cp_async16(at, ksrc, in);
-                    cp_async16(at + K::TILE, vsrc, in);
-                    if (in) {
-                        ksrc += row_step;
-                        vsrc += row_step;
+                    for (int i = 0; i < K::TILE / 512; ++i) {
+                        const uint32_t at = dst + place<DP>(i * (512 / DP) + lane_row, lane_chunk);
+                        cp_async16(at, ksrc + i * 512, true);
+                        cp_async16(at + K::TILE, vsrc + i * 512, true);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < K::TILE / 512; ++i) {
+                        const bool in = ok && lane_in && i * (512 / DP) + lane_row < left;
+                        const uint32_t at = dst + place<DP>(i * (512 / DP) + lane_row, lane_chunk);
+                        const int64_t off = in ? int64_t(i) * row_step : 0;
+                        cp_async16(at, in ? ksrc + off : c.k, in);
+                        cp_async16(at + K::TILE, in ? vsrc + off : c.v, in);
                     }
                 }
                 if (lane < 2) cp_async4(smem_u32(&scales[warp][stage][lane]), (lane ? c.v_scale : c.k_scale) + ph, ok);
@@ -419,22 +425,23 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
             }
 
             // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
-            const bool same = v_scale == v_ref;
-            const __half2 unit = __float2half2_rn(v_scale / v_ref);
+            // Values are in units of the largest scale so far; a page of a smaller one has the difference in its weights, a power of two.
+            if (v_scale != v_ref) {
+                const __half2 unit = __float2half2_rn(v_scale / v_ref);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const __half2 w = __hmul2(*reinterpret_cast<const __half2 *>(&p[nb][i]), unit);
+                        p[nb][i] = *reinterpret_cast<const uint32_t *>(&w);
+                    }
+            }
             auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
                 uint32_t v0[4], v1[4];  // of dimensions 2 tile, 2 tile + 1 and the two after: tokens 2t.., tokens 2t + 8..
                 decode4<FMT, true>(__byte_perm(wa, wb, 0x5140), v0[0], v0[1]);
                 decode4<FMT, true>(__byte_perm(wc, wd, 0x5140), v0[2], v0[3]);
                 decode4<FMT, true>(__byte_perm(wa, wb, 0x7362), v1[0], v1[1]);
                 decode4<FMT, true>(__byte_perm(wc, wd, 0x7362), v1[2], v1[3]);
-                if (!same) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const __half2 u = __hmul2(*reinterpret_cast<__half2 *>(&v0[i]), unit), w = __hmul2(*reinterpret_cast<__half2 *>(&v1[i]), unit);
-                        v0[i] = *reinterpret_cast<const uint32_t *>(&u);
-                        v1[i] = *reinterpret_cast<const uint32_t *>(&w);
-                    }
-                }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     mma(o[nb][tile], v0, p[nb][0], p[nb][1]);

@@ -126,7 +126,8 @@ def attention(batch, Q, scale, window=0):
     A q of bfloat16 keeps its 8 bits; 2^-24 of the row's largest for elements far below it is inside the dim term.  The exponential
     itself and its argument's rounding: 2^-21 + 2^-23 * |argument|, the argument below 200 where a weight counts: 2^-15 of A.
     16-bit floats below 2^-14 have the fixed step 2^-24: with weights held so that the largest is 2^7 or more, each is off by
-    2^-25 / 2^7 of the sum at most on top (sum |v| over the keys seen), and values held in units of the largest scale by 2^-25 of it."""
+    2^-25 / 2^7 of the sum at most on top, where the largest value is that of the largest code and scale (codes may be in units of the
+    largest scale, the weights taking the difference, in which a scale that is no power of two rounds once more: 2^-11 of A)."""
     heads = Q.shape[1]
     group = heads // batch.heads
     out = torch.zeros(Q.shape, dtype=torch.float64, device=Q.device)
@@ -151,8 +152,8 @@ def attention(batch, Q, scale, window=0):
             out[row: row + m, h] = p @ vh
             size = p @ vh.abs()
             score = ((q.abs() @ kh.abs().T) * scale * seen).amax(-1, keepdim=True)
-            fixed = 2.0**-32 * (seen.double() @ vh.abs()) + 2.0**-25 * float(largest)
-            bound[row: row + m, h] = fixed + size * (2.0**-10 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
+            fixed = 2.0**-32 * seen.double().sum(-1, keepdim=True) * (LARGEST[batch.fmt] * float(largest))
+            bound[row: row + m, h] = fixed + size * (2.0**-10 + 2.0**-11 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
     return out, bound
 
 
