@@ -98,6 +98,7 @@ SIGNATURES = {
     "dx_kvcache_read": (_i, [_i, _pseqs, _pcache, _vp, _i64, _vp, _i64, _vp, _vp]),
     "dx_kvcache_attention_workspace_bytes": (_sz, [_i, _i64, _pseqs, _pcache, _i64]),
     "dx_kvcache_attention": (_i, [_i, _vp, _i64, _i64, _pseqs, _pcache, _d, _i64, _i64, _vp, _i64, _vp, _sz, _vp, _vp]),
+    "dx_kvcache_status": (_i, [_vp]),
     "dx_transpose": (_i, [_i, _vp, _pi64, _i, _pi32, _vp, _vp]),
     "dx_concat": (_i, [_i, _pvp, _pi64, _i, _pi64, _i, _i, _vp, _vp]),
     "dx_broadcast_to": (_i, [_i, _vp, _pi64, _i, _pi64, _i, _vp, _vp]),

@@ -13,9 +13,7 @@
 // block takes an equal piece of it, whatever the lengths are (they are known on the device alone).  A piece may begin or end
 // inside an item (one tile of rows, one head); such items' parts meet in the workspace and a second kernel joins them, always
 // in the order of the keys: the same bits every time.
-#include <atomic>
-
-#include "kvcache.cuh"
+#include "kvcache_attention.cuh"
 
 namespace dx {
 namespace kv {
@@ -24,30 +22,7 @@ namespace {
 constexpr int WARPS = 4, CTA = WARPS * 32;
 constexpr int WT = 16;     // tokens a warp takes at a time: never more than one page
 constexpr int STEP = WARPS * WT;
-constexpr int JOIN_CTA = 512;
-// Weights are held as 2^(x - m + 7): m lags the true maximum by up to 2^8, so a weight is at most 2^15, and what is 2^-31 of the
-// largest is still a half.
-constexpr float LAG = 8.f, UP = 7.f;
-constexpr float NEG_INF = -__builtin_huge_valf();
-
-struct Attn {
-    const void *q;
-    void *out;
-    int64_t q_stride, out_stride;
-    int q_heads, group, window;
-    float scale_log2;
-    int q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of out
-    int min_steps;
-    uint8_t *ws;
-    int32_t *flag;
-};
-
-// What the joining kernel needs to know of the item that ends inside block i's first piece: `parts` blocks from i - 1 on hold
-// parts of it (0: block i does not begin inside an item, or an earlier one joins it).
-struct alignas(32) Join {
-    int64_t row0;
-    int first_row, rows, head, parts;
-};
+constexpr int MIN_STEPS = 2;  // of a block: fewer would cost more in joining than they save
 
 // DP: the head's dimensions, padded; NB: blocks of eight rows of an item.
 template <int DP, int NB> struct Cfg {
@@ -61,7 +36,6 @@ template <int DP, int NB> struct Cfg {
     static_assert(RING >= ROWS * DP * 4, "the ring holds a warp's output");
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -91,16 +65,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Where chunk `c` (16 bytes) of token `r` of a warp's tile lies: rows of DP bytes whose chunks are exchanged so that both ways the
 // tile is read (eight tokens, every other chunk; four tokens of one parity, two chunks) touch every bank once.
 template <int DP> __device__ __forceinline__ int place(int r, int c) {
@@ -168,7 +132,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
         __syncthreads();
     }
     const int64_t total = total_steps;
-    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / a.min_steps));
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / MIN_STEPS));
     Join *join = reinterpret_cast<Join *>(a.ws) + blockIdx.x;
     float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
     if (total == 0 || int64_t(blockIdx.x) >= blocks) {
@@ -553,70 +517,6 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     }
 }
 
-// Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
-// of the keys.  Sixteen warps share the item's rows; the warps of a row share its parts.
-template <typename T, int DP, int NB> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
-    constexpr int V = DP / 32, ROWS = Cfg<DP, NB>::ROWS;
-    __shared__ float sh[JOIN_CTA / 32][DP];
-    griddep_wait_cta();
-    const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
-    if (j.parts == 0) return;
-    const float *parts = reinterpret_cast<const float *>(a.ws + gridDim.x * sizeof(Join));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int each = j.rows > 8 ? 1 : j.rows > 4 ? 2 : j.rows > 2 ? 4 : j.rows > 1 ? 8 : 16;  // warps of a row
-    const int row = warp / each, sub = warp % each;
-    // part 0: the second part of block i - 1; part p > 0: the first of block i - 1 + p
-    auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * Cfg<DP, NB>::PART; };
-    float acc[V] = {}, sum = 0.f;
-    if (row < j.rows) {
-        float top = NEG_INF;
-        for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, at(p)[ROWS * DP + row]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float base = top == NEG_INF ? 0.f : top;
-        for (int p0 = 0; p0 < j.parts; p0 += 32) {
-            float w = 0.f;
-            if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
-            float s = w;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            sum += s;
-            const int n = min(32, j.parts - p0);
-#pragma unroll 4
-            for (int p = sub; p < n; p += each) {
-                const float by = __shfl_sync(0xffffffffu, w, p);
-                const float *src = at(p0 + p) + row * DP + lane * V;
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e];
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
-    __syncthreads();
-    if (row >= j.rows || sub) return;
-    const float by = sum == 0.f ? 0.f : 1.f / sum;
-    const int fr = j.first_row + row, i = fr / a.group;
-    T *out = static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
-    for (int d = lane; d < c.dim; d += 32) {
-        float v = 0.f;
-        for (int w = 0; w < each; ++w) v += sh[warp + w][d];
-        out[d] = from_compute<T>(v * by);
-    }
-}
-
-// A kernel's shared memory above 48 KB has to be allowed once on each device.
-template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_t> *prepared) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (e == cudaSuccess && !(prepared->load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) prepared->fetch_or(bit, std::memory_order_relaxed);
-    }
-    return e == cudaSuccess ? DX_OK : fail(DX_E_CUDA, "kvcache_attention: %s", cudaGetErrorString(e));
-}
-
 template <typename T, int FMT, int DP, int NB> int launch_rows(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
     using K = Cfg<DP, NB>;
     static std::atomic<uint64_t> prepared{0};  // one bit for each device
@@ -624,7 +524,7 @@ template <typename T, int FMT, int DP, int NB> int launch_rows(const Attn &a, co
     const unsigned grid = unsigned(sm_count() * K::BLOCKS);
     launch_pdl(attention_kernel<T, FMT, DP, NB>, dim3(grid), dim3(CTA), K::SMEM, st, a, c, s);
     if (int e = check_launch("kvcache_attention")) return e;
-    launch_pdl(join_kernel<T, DP, NB>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
+    launch_pdl(join_kernel<T, DP, K::ROWS>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
     return check_launch("kvcache_attention (join)");
 }
 template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, int64_t rows, cudaStream_t st) {
@@ -645,6 +545,8 @@ size_t workspace(int dim, int64_t rows) {
         default: return workspace_rows<256>(rows);
     }
 }
+// Whether a call goes to the tiles of 128 rows: as soon as a sequence may have more rows than one item here.
+bool by_tiles(const Cache &c, int64_t rows) { return c.dim <= 128 && rows > 16; }
 // The most rows of a sequence that share a key head, as far as the caller says.
 int64_t rows_of(int64_t q_heads, const Cache &c, const Seqs &s, int64_t max_new) {
     return (max_new > 0 && max_new < s.rows ? max_new : s.rows) * (q_heads / c.heads);
@@ -659,7 +561,9 @@ extern "C" size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_head
     kv::Cache c;
     kv::Seqs s;
     if (kv::check("kvcache_attention", cache, seqs, &c, &s) || s.rows == 0 || s.batch == 0) return 0;
-    return kv::workspace(c.dim, kv::rows_of(q_heads, c, s, max_new));
+    if (q_heads < 1 || q_heads % c.heads) return 0;
+    const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
+    return kv::by_tiles(c, rows) ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim, rows);
 }
 
 extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
@@ -683,12 +587,14 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     if (kv::overlap(q, qb, out, ob) || kv::overlap(out, ob, c.k, codes) || kv::overlap(out, ob, c.v, codes))
         return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
     const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
-    const size_t need = kv::workspace(c.dim, rows);
+    const bool tiles = kv::by_tiles(c, rows);
+    const size_t need = tiles ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim, rows);
     if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
     kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),
-               q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 4 == 0 && aligned_to(out, 8), 2, static_cast<uint8_t *>(workspace), flag};
+               q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 4 == 0 && aligned_to(out, 8), static_cast<uint8_t *>(workspace), flag};
     cudaStream_t st = as_stream(stream);
+    if (tiles) return kv::launch_tiles(dtype, cache->format, a, c, s, st);
 #define DX_CALL(T, FMT)                                                             \
     switch (kv::padded(c.dim)) {                                                    \
         case 64: return kv::launch<T, FMT, 64>(a, c, s, rows, st);                        \

@@ -1,0 +1,118 @@
+// What the kernels of dx_kvcache_attention share: the call's arguments, the parts of items that several blocks work on, and the
+// kernel that joins them.
+#pragma once
+#include <atomic>
+
+#include "kvcache.cuh"
+
+namespace dx {
+namespace kv {
+
+struct Attn {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int q_heads, group, window;
+    float scale_log2;
+    int q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of out
+    uint8_t *ws;
+    int32_t *flag;
+};
+
+// What the joining kernel needs to know of the item that ends inside block i's first piece: `parts` blocks from i - 1 on hold
+// parts of it (0: block i does not begin inside an item, or an earlier one joins it).
+struct alignas(32) Join {
+    int64_t row0;
+    int first_row, rows, head, parts;
+};
+
+// Attention by tiles of 128 rows on the fifth-generation tensor cores (kvcache_tiles.cu), for head_dim up to 128.
+size_t tiles_workspace(const Cache &c, const Seqs &s, int group);
+int launch_tiles(int dtype, int format, const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st);
+
+// A kernel's shared memory above 48 KB has to be allowed once on each device.
+template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_t> *prepared) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (e == cudaSuccess && !(prepared->load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) prepared->fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e == cudaSuccess ? DX_OK : fail(DX_E_CUDA, "kvcache_attention: %s", cudaGetErrorString(e));
+}
+
+#ifdef __CUDACC__
+// Weights are held as 2^(x - m + 7): m lags the true maximum by up to 2^8, so a weight is at most 2^15, and what is 2^-31 of the
+// largest is still a half.
+constexpr float LAG = 8.f, UP = 7.f;
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr int JOIN_CTA = 512, JOIN_ROWS = 16;
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
+// of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
+// with its item and does not end it part 2i + 1.  Sixteen warps share sixteen of the item's rows; the warps of a row share its parts.
+template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
+    constexpr int V = DP / 32, PART = ROWS * DP + 2 * ROWS;
+    __shared__ float sh[JOIN_CTA / 32][DP];
+    griddep_wait_cta();
+    const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
+    const int row0 = blockIdx.y * JOIN_ROWS, rows = min(j.rows - row0, JOIN_ROWS);
+    if (j.parts == 0 || rows <= 0) return;
+    const float *parts = reinterpret_cast<const float *>(a.ws + gridDim.x * sizeof(Join));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int each = rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;  // warps of a row
+    const int r = warp / each, row = row0 + r, sub = warp % each;
+    auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * PART; };
+    float acc[V] = {}, sum = 0.f;
+    if (r < rows) {
+        float top = NEG_INF;
+        for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, at(p)[ROWS * DP + row]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == NEG_INF ? 0.f : top;
+        for (int p0 = 0; p0 < j.parts; p0 += 32) {
+            float w = 0.f;
+            if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
+            float s = w;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            sum += s;
+            const int n = min(32, j.parts - p0);
+#pragma unroll 4
+            for (int p = sub; p < n; p += each) {
+                const float by = __shfl_sync(0xffffffffu, w, p);
+                const float *src = at(p0 + p) + row * DP + lane * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
+    __syncthreads();
+    if (r >= rows || sub) return;
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    const int fr = j.first_row + row, i = fr / a.group;
+    T *out = static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
+    for (int d = lane; d < c.dim; d += 32) {
+        float v = 0.f;
+        for (int w = 0; w < each; ++w) v += sh[warp + w][d];
+        out[d] = from_compute<T>(v * by);
+    }
+}
+#endif
+
+}  // namespace kv
+}  // namespace dx

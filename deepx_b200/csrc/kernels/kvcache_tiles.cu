@@ -1,0 +1,743 @@
+// dx_kvcache_attention for prompts: tiles of 128 rows on tcgen05 tensor cores.
+//
+// An item is up to 256 rows (new token i, head of the key head's group: i * group + g, flattened) of one sequence and key head: two
+// tiles of 128 rows that take turns, so that the tensor cores work on one while the other's exponentials are computed.  For each step
+// of 128 keys:
+//     S = Q K^T          128 x 128, into TMEM;                                Q, K halfs in shared memory
+//     P = 2^(c S - m)    a thread has a row; halfs, over S's place in TMEM
+//     O = O + P V        128 x dim, in TMEM, P from TMEM;                     V halfs in shared memory
+// Four exponentials' worth of tensor work (512 multiply-adds) goes with each exponential at 128 dimensions: a step of both tiles costs
+// 2048 cycles of the tensor cores and 2048 of the exponential unit, so both bound this kernel; what is neither stays off their threads.
+//
+// Roles (13 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each; 8-11 turn codes into halfs (sixteen a thread and turn,
+// loaded a step ahead); one thread of warp 12 issues the products.  Codes become halfs unscaled and
+// exact; the scales of a step's eight groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of
+// the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
+// scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
+//
+// The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it; items
+// that more than one block works on are joined as in kvcache_attention.cu.
+//
+// Every wait is bounded by a clock; when one runs out a status word is set (dx_kvcache_status), all roles leave, TMEM is freed.
+#include <mutex>
+
+#include "kvcache_attention.cuh"
+
+namespace dx {
+namespace kv {
+namespace {
+
+constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 128, GROUPS = KEYS / 16;
+constexpr int THREADS = 13 * 32;
+constexpr int STAGES = 2, INFO = 4;
+constexpr int PLAN_CTA = 1024;
+constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
+enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
+
+__device__ int g_status = 0;
+
+// The plan: for each group (256 rows of a sequence, all heads) its sequence, which 256 rows, and the steps in front of it.
+struct Plan {
+    int64_t *before;  // [groups + 1]
+    int2 *group;      // {sequence, tile of 256 rows}
+    int *first;       // [batch + 1] groups in front of a sequence
+    int *count;       // groups
+};
+__host__ __device__ inline int64_t most_groups(const Seqs &s, int group) { return s.rows * group / ITEM_ROWS + s.batch; }
+__host__ __device__ inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+__host__ __device__ inline Plan plan_at(uint8_t *base, const Seqs &s, int group) {
+    const int64_t n = most_groups(s, group);
+    Plan p;
+    p.before = reinterpret_cast<int64_t *>(base);
+    base += align256(size_t(n + 1) * 8);
+    p.group = reinterpret_cast<int2 *>(base);
+    base += align256(size_t(n) * 8);
+    p.first = reinterpret_cast<int *>(base);
+    base += align256(size_t(s.batch + 1) * 4);
+    p.count = reinterpret_cast<int *>(base);
+    return p;
+}
+inline size_t plan_bytes(const Seqs &s, int group) {
+    const int64_t n = most_groups(s, group);
+    return align256(size_t(n + 1) * 8) + align256(size_t(n) * 8) + align256(size_t(s.batch + 1) * 4) + 256;
+}
+
+// The keys of one item: rows first_row..first_row + rows of the sequence.
+struct Item {
+    int first_row, rows, lo, hi, steps;  // tokens lo..hi, in steps of KEYS from lo (a multiple of KEYS)
+};
+__device__ __forceinline__ Item item_of(const Seq &q, const Attn &a, int tile) {
+    Item x;
+    x.first_row = tile * ITEM_ROWS;
+    x.rows = int(min(int64_t(q.n) * a.group - x.first_row, int64_t(ITEM_ROWS)));
+    const int64_t p0 = int64_t(q.first) + x.first_row / a.group, p1 = int64_t(q.first) + (x.first_row + x.rows - 1) / a.group;
+    const int64_t hi = max(min(int64_t(q.end), p1 + 1), int64_t(0));
+    const int64_t lo = a.window > 0 ? max(int64_t(0), p0 - a.window + 1) : 0;
+    x.hi = int(hi);
+    x.lo = int(min(lo, hi) / KEYS * KEYS);
+    x.steps = hi > x.lo ? int((hi - x.lo + KEYS - 1) / KEYS) : 1;  // rows that see nothing are written too
+    return x;
+}
+
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sum, int64_t &total) {  // exclusive, PLAN_CTA threads
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += up;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int64_t base = 0, all = 0;
+    for (int w = 0; w < PLAN_CTA / 32; ++w) {
+        if (w < warp) base += warp_sum[w];
+        all += warp_sum[w];
+    }
+    total = all;
+    return base + s - v;
+}
+
+__global__ void __launch_bounds__(PLAN_CTA) plan_kernel(Attn a, Cache c, Seqs s, Plan p) {
+    __shared__ int64_t warp_sum[PLAN_CTA / 32];
+    griddep_wait_cta();
+    check_seqs(s, c, a.flag);
+    const int64_t room = most_groups(s, a.group);
+    int64_t groups = 0;
+    for (int b0 = 0; b0 < s.batch; b0 += PLAN_CTA) {
+        const int b = b0 + threadIdx.x;
+        int64_t n = 0, total;
+        if (b < s.batch) n = (int64_t(seq_at(s, c, b).n) * a.group + ITEM_ROWS - 1) / ITEM_ROWS;
+        const int64_t at = groups + block_scan(n, warp_sum, total);
+        if (b < s.batch) p.first[b] = int(min(at, room));
+        groups += total;
+    }
+    groups = min(groups, room);  // starts that overlap could ask for more than the rows allow; check_seqs has flagged them
+    if (threadIdx.x == 0) {
+        p.first[s.batch] = int(groups);
+        *p.count = int(groups);
+    }
+    __syncthreads();
+    int64_t steps = 0;
+    for (int64_t g0 = 0; g0 < groups; g0 += PLAN_CTA) {
+        const int64_t g = g0 + threadIdx.x;
+        int64_t n = 0, total;
+        if (g < groups) {
+            int lo = 0, hi = s.batch;  // the last b with first[b] <= g
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.first[mid] <= g) lo = mid;
+                else hi = mid;
+            }
+            const int tile = int(g - p.first[lo]);
+            p.group[g] = make_int2(lo, tile);
+            n = int64_t(item_of(seq_at(s, c, lo), a, tile).steps) * c.heads;
+        }
+        const int64_t at = steps + block_scan(n, warp_sum, total);
+        if (g < groups) p.before[g] = at;
+        steps += total;
+    }
+    if (threadIdx.x == 0) p.before[groups] = steps;
+}
+
+// ---- PTX ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded: false when the clock limit has passed or another role has given up; the first to give up says where.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int where) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+            *abort_flag = 1;
+            atomicCAS(&g_status, 0, where);
+            return false;
+        }
+    }
+}
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int where) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+          "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Shared-memory matrix descriptor: 128-byte swizzle, 8-row groups of 1024 bytes (stride), panels of 64 elements `leading` bytes apart.
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, uint32_t leading) {
+    return uint64_t((at >> 4) & 0x3FFF) | uint64_t((leading >> 4) & 0x3FFF) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// Instruction descriptor, halfs with float32 accumulators, M 128: N, and whether the second operand's rows are its K index.
+__host__ __device__ constexpr uint32_t instruction(int n, bool b_by_k) {
+    return (1u << 4) | (b_by_k ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(TILE_ROWS >> 4) << 24);
+}
+
+template <int DP> struct Cfg {
+    static constexpr int PANELS = DP / 64, PANEL = 128 * 128;  // 128 rows of 64 halfs
+    static constexpr int OPERAND = PANELS * PANEL;             // Q of a tile, K or V of a step
+    static constexpr int SMEM = (2 + 2 * STAGES) * OPERAND + 1024;
+    static constexpr int PART = ITEM_ROWS * DP + 2 * ITEM_ROWS;
+    static constexpr int S_COL = 0, O_COL = 256;  // TMEM columns of tile t: S_COL + 128 t, O_COL + DP t
+};
+
+// What the softmax needs of a step: for each group of sixteen tokens K's scale, log2 of V's in units of the largest so far and its
+// inverse; by how much O in units of the largest before shrinks, the largest; which groups are there.
+struct Info {
+    float k[GROUPS], v_log[GROUPS], v_inv[GROUPS];
+    float turn, v_ref;
+    int there;
+};
+
+template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(Attn a, Cache c, Seqs s, Plan plan) {
+    using C = Cfg<DP>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t bars[2 * STAGES * 2 + 4 * 2];
+    __shared__ Info info[INFO];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_shared;
+    __shared__ int found_group;
+    volatile int *abort_flag = &abort_shared;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t q_smem = base, k_smem = base + 2 * C::OPERAND, v_smem = k_smem + STAGES * C::OPERAND;
+    const uint32_t bar0 = smem_u32(bars);
+    auto k_full = [&](int i) { return bar0 + 8u * i; };
+    auto k_empty = [&](int i) { return bar0 + 8u * (STAGES + i); };
+    auto v_full = [&](int i) { return bar0 + 8u * (2 * STAGES + i); };
+    auto v_empty = [&](int i) { return bar0 + 8u * (3 * STAGES + i); };
+    auto s_full = [&](int t) { return bar0 + 8u * (4 * STAGES + t); };
+    auto p_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 2 + t); };
+    auto q_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 4 + t); };
+    auto o_full = [&](int t) { return bar0 + 8u * (4 * STAGES + 6 + t); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(k_full(i), 128);
+            mbar_init(k_empty(i), 1);
+            mbar_init(v_full(i), 128);
+            mbar_init(v_empty(i), 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(s_full(t), 2);  // the products' completion, and the issuing thread's own arrival, behind which info is visible
+            mbar_init(p_ready(t), 128);
+            mbar_init(q_ready(t), 128);
+            mbar_init(o_full(t), 1);
+        }
+        abort_shared = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    griddep_wait_cta();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // ---- this block's piece of the line ----
+    Join *join = reinterpret_cast<Join *>(a.ws) + blockIdx.x;
+    float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
+    const int groups = *plan.count;
+    const int64_t total = plan.before[groups];
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / 2));
+    const bool work = total > 0 && int64_t(blockIdx.x) < blocks;
+    const int64_t begin = work ? total * blockIdx.x / blocks : 0, end = work ? total * (blockIdx.x + 1) / blocks : 0;
+    if (threadIdx.x == 0) join->parts = 0;
+    for (int g = threadIdx.x; g < groups; g += THREADS)
+        if (plan.before[g] <= begin && plan.before[g + 1] > begin) found_group = g;
+    __syncthreads();
+
+    // Every role walks the same pieces: for each, its sequence, head, rows and steps.
+    struct Piece {
+        Seq sq;
+        Item it;
+        int b, head, step0, steps, tiles;
+        int64_t item_begin, item_end;
+    };
+    int group = found_group;
+    auto piece_at = [&](int64_t at) {
+        Piece p;
+        while (at >= plan.before[group + 1]) ++group;
+        const int2 gt = plan.group[group];
+        p.b = gt.x;
+        p.sq = seq_at(s, c, p.b);
+        p.it = item_of(p.sq, a, gt.y);
+        const int64_t g0 = plan.before[group];
+        p.head = int((at - g0) / p.it.steps);
+        p.item_begin = g0 + int64_t(p.head) * p.it.steps;
+        p.item_end = p.item_begin + p.it.steps;
+        p.step0 = int(at - p.item_begin);
+        p.steps = int(min(end, p.item_end) - at);
+        p.tiles = p.it.rows > TILE_ROWS ? 2 : 1;
+        return p;
+    };
+
+    if (warp < 8) {
+        // ===== softmax of tile t: this thread has one row =====
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t(warp & 3) * 32u << 16;
+        const uint32_t s_tmem = tmem + lanes + C::S_COL + 128 * t, o_tmem = tmem + lanes + C::O_COL + DP * t;
+        uint32_t n_s = 0, n_o = 0;
+        int n_info = 0;
+        bool ok = true;
+        for (int64_t at = begin; at < end && ok;) {
+            const Piece p = piece_at(at);
+            at += p.steps;
+            if (t >= p.tiles) {
+                n_info += p.steps;
+                continue;
+            }
+            const int row = t * TILE_ROWS + r;
+            const bool live = row < p.it.rows;
+            const int fr = p.it.first_row + row, i = live ? fr / a.group : 0;
+            const int last = live ? int(max(min(int64_t(p.sq.first) + i, int64_t(p.sq.end) - 1), int64_t(-1))) : -1;         // sees keys up to here
+            const int64_t after = live && a.window > 0 ? int64_t(p.sq.first) + i - a.window : -(int64_t(1) << 40);  // and behind this one
+            // ---- the row of Q as halfs into shared memory, a bfloat16 row divided by a power of two first ----
+            float c_row = a.scale_log2;
+            {
+                const T *q = static_cast<const T *>(a.q) + (p.sq.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+                Pack<T, 8> x[DP / 8];
+                float amax = 0.f;
+#pragma unroll
+                for (int k = 0; k < DP / 8; ++k) {
+                    if (live && k * 8 < c.dim && a.q_vec) x[k] = ld_cached<T, 8>(q + k * 8);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[k].v[e] = live && k * 8 < c.dim ? q[k * 8 + e] : from_compute<T>(0.f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k].v[e])));
+                }
+                float down = 1.f;
+                if constexpr (std::is_same<T, bf16>::value) {
+                    const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                    if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
+                        down = __uint_as_float((254u - e) << 23);
+                        c_row *= __uint_as_float(e << 23);
+                    }
+                }
+                const uint32_t dst = q_smem + t * C::OPERAND + r * 128;
+#pragma unroll
+                for (int k = 0; k < DP / 8; ++k) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = half2_bits(to_compute(x[k].v[2 * e]) * down, to_compute(x[k].v[2 * e + 1]) * down);
+                    sts128(dst + (k >> 3) * C::PANEL + (((k & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+                }
+            }
+            fence_async_smem();
+            fence_before();  // the reads of O of the item before
+            mbar_arrive(q_ready(t));
+            const int tile_first = int(min(int64_t(p.sq.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.sq.end) - 1));  // least `last` of the tile
+            const int64_t tile_after = a.window > 0 ? int64_t(p.sq.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
+
+            float m = NEG_INF, v_ref = 1.f;
+            uint64_t l2 = pair(0.f, 0.f);
+            for (int step = 0; step < p.steps; ++step, ++n_info) {
+                const int j0 = p.it.lo + (p.step0 + step) * KEYS;
+                if (!warp_wait(s_full(t), n_s & 1, abort_flag, S_SCORES)) { ok = false; break; }
+                ++n_s;
+                fence_after();
+                const Info &f = info[n_info % INFO];
+                const int there = f.there;
+                v_ref = f.v_ref;
+                const bool masked = j0 + KEYS - 1 > tile_first || j0 <= tile_after || there != (1 << GROUPS) - 1;  // the same in all threads
+                const int hi = last - j0;                                                       // columns up to here are seen
+                const int lo = int(max(after - j0, int64_t(-1)));                               // from behind here
+                auto seen = [&](int col) { return col <= hi && col > lo && (there >> (col >> 4) & 1); };
+                // ---- the row's largest score ----
+                float top = NEG_INF;
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t x[32];
+                    tmem_ld32(s_tmem + 32 * ch, x);
+                    wait_ld();
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!seen(32 * ch + e)) x[e] = __float_as_uint(NEG_INF);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        float v = __uint_as_float(x[16 * g]);
+#pragma unroll
+                        for (int e = 1; e < 16; ++e) v = fmaxf(v, __uint_as_float(x[16 * g + e]));
+                        top = fmaxf(top, v * (c_row * f.k[2 * ch + g]));
+                    }
+                }
+                const float turn = f.turn;
+                const bool rise = top > m + LAG;
+                if (__any_sync(0xffffffffu, rise) || turn != 1.f) {
+                    const float to = rise ? top : m;
+                    float by = to == m ? 1.f : exp2_approx(m - to);
+                    m = to;
+                    float l0, l1;
+                    unpair(l2, l0, l1);
+                    l2 = pair(l0 * by, l1 * by);
+                    by *= turn;
+                    if (step > 0) {  // the products of the step before are complete: these scores were issued behind them
+#pragma unroll 1
+                        for (int d = 0; d < DP; d += 32) {
+                            uint32_t x[32];
+                            tmem_ld32(o_tmem + d, x);
+                            wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * by);
+                            tmem_st32(o_tmem + d, x);
+                        }
+                    }
+                }
+                const float base_m = UP - (m == NEG_INF ? 0.f : m);
+                // ---- weights, over the scores that have been read ----
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t x[32], w[16];
+                    tmem_ld32(s_tmem + 32 * ch, x);
+                    wait_ld();
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float cg = c_row * f.k[2 * ch + g], mg = base_m + f.v_log[2 * ch + g], ig = f.v_inv[2 * ch + g];
+                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float y0, y1;
+                            unpair(fma2(pair(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1])), c2, m2), y0, y1);
+                            if (masked) {
+                                y0 = seen(32 * ch + 16 * g + e) ? y0 : NEG_INF;
+                                y1 = seen(32 * ch + 16 * g + e + 1) ? y1 : NEG_INF;
+                            }
+                            y0 = exp2_approx(y0);
+                            y1 = exp2_approx(y1);
+                            l2 = fma2(pair(y0, y1), i2, l2);
+                            w[8 * g + e / 2] = half2_bits(y0, y1);
+                        }
+                    }
+                    tmem_st16(s_tmem + 16 * ch, w);
+                }
+                wait_st();
+                fence_before();
+                mbar_arrive(p_ready(t));
+            }
+            if (!ok) break;
+            // ---- the way out ----
+            if (!warp_wait(o_full(t), n_o & 1, abort_flag, S_OUTPUT)) { ok = false; break; }
+            ++n_o;
+            fence_after();
+            float l0, l1;
+            unpair(l2, l0, l1);
+            const float sum = l0 + l1, by = sum == 0.f ? 0.f : v_ref / sum;
+            const bool whole = p.step0 == 0 && p.steps == p.it.steps;
+            float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
+            T *out = static_cast<T *>(a.out) + (p.sq.row0 + i) * a.out_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+            if (!whole && live) {
+                part[ITEM_ROWS * DP + row] = m;
+                part[ITEM_ROWS * DP + ITEM_ROWS + row] = sum;
+            }
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 32) {
+                uint32_t x[32];
+                tmem_ld32(o_tmem + d, x);
+                wait_ld();
+                if (!live) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    if (d + e >= c.dim) break;
+                    float4 v;
+                    // a row that has seen nothing has multiplied nothing but zeros
+                    v.x = __uint_as_float(x[e]) * by;
+                    v.y = __uint_as_float(x[e + 1]) * by;
+                    v.z = __uint_as_float(x[e + 2]) * by;
+                    v.w = __uint_as_float(x[e + 3]) * by;
+                    if (!whole) *reinterpret_cast<float4 *>(part + row * DP + d + e) = v;
+                    else {
+                        Pack<T, 4> y;
+                        y.v[0] = from_compute<T>(v.x);
+                        y.v[1] = from_compute<T>(v.y);
+                        y.v[2] = from_compute<T>(v.z);
+                        y.v[3] = from_compute<T>(v.w);
+                        if (a.out_vec) st_stream<T, 4>(out + d + e, y);
+                        else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) out[d + e + k] = y.v[k];
+                        }
+                    }
+                }
+            }
+            if (threadIdx.x == 0 && p.step0 > 0 && at - p.steps == begin && p.item_begin >= total * (int64_t(blockIdx.x) - 1) / blocks) {
+                join->row0 = p.sq.row0;
+                join->first_row = p.it.first_row;
+                join->rows = p.it.rows;
+                join->head = p.head;
+                join->parts = int((p.item_end * blocks - 1) / total) - int(blockIdx.x) + 2;
+            }
+        }
+    } else if (warp < 12) {
+        // ===== codes into halfs =====
+        const int tid = threadIdx.x & 127;
+        constexpr int PER_ROW = DP / 16, TURNS = KEYS * PER_ROW / 128, TURN_ROWS = 128 / PER_ROW;
+        const int ch = tid % PER_ROW, r0 = tid / PER_ROW;  // sixteen codes of row r0 + TURN_ROWS * turn
+        const bool in_dim = ch * 16 < c.dim;
+        // the two chunks of a thread, the second first in the second panel: eight lanes then touch every bank once
+        const int swap = (ch >> 2) & 1, c0 = (ch & 3) * 2 + swap, c1 = c0 ^ 1;
+        // lane g of a warp knows the page of group g of a step
+        auto page_of = [&](const Piece &p, int step) {
+            const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
+            int32_t number = -1;
+            if (step < p.steps && j < p.it.hi) {
+                number = s.table[int64_t(p.b) * s.cols + (j >> c.page_shift)];
+                if (number < 0 || number >= c.pages) {
+                    if (warp == 8 && lane < 8) raise(a.flag, FLAG_PAGE);
+                    number = -1;
+                }
+            }
+            return number;
+        };
+        uint32_t n = 0;
+        bool ok = true;
+        for (int64_t at = begin; at < end && ok;) {
+            const Piece p = piece_at(at);
+            at += p.steps;
+            uint4 xk[TURNS], xv[TURNS];
+            int32_t number = page_of(p, 0), next = page_of(p, 1);
+            auto load = [&](const uint8_t *codes, int step, int32_t numbers, int turn) {
+                const int row = r0 + TURN_ROWS * turn, j = p.it.lo + (p.step0 + step) * KEYS + row;
+                const int32_t page = __shfl_sync(0xffffffffu, numbers, row >> 4);  // a warp's rows of a turn are of one group
+                if (page < 0 || j >= p.it.hi || !in_dim) return make_uint4(0, 0, 0, 0);
+                return *reinterpret_cast<const uint4 *>(codes + ((int64_t(page) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim + ch * 16);
+            };
+            auto store = [&](uint32_t dst, int turn, uint4 x, auto finite) {
+                const int row = r0 + TURN_ROWS * turn;
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                uint32_t h[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) decode4<FMT, decltype(finite)::value>(w[e], h[2 * e], h[2 * e + 1]);
+                const uint32_t line = dst + (ch >> 2) * C::PANEL + row * 128;
+                sts128(line + ((c0 ^ (row & 7)) << 4), swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
+                sts128(line + ((c1 ^ (row & 7)) << 4), swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
+            };
+#pragma unroll
+            for (int turn = 0; turn < TURNS; ++turn) xk[turn] = load(c.k, 0, number, turn);
+#pragma unroll
+            for (int turn = 0; turn < TURNS; ++turn) xv[turn] = load(c.v, 0, number, turn);
+            float v_ref = 0.f;
+            for (int step = 0; step < p.steps; ++step, ++n) {
+                const int stage = n % STAGES;
+                const uint32_t empty = ((n / STAGES) & 1) ^ 1;
+                float ks = 1.f, vs = 0.f;
+                const bool there = number >= 0;
+                if (warp == 8 && there) {
+                    ks = c.k_scale[int64_t(number) * c.heads + p.head];
+                    vs = c.v_scale[int64_t(number) * c.heads + p.head];
+                }
+                if (!warp_wait(k_empty(stage), empty, abort_flag, S_ROOM)) { ok = false; break; }
+#pragma unroll
+                for (int turn = 0; turn < TURNS; ++turn) {
+                    store(k_smem + stage * C::OPERAND, turn, xk[turn], std::false_type());
+                    xk[turn] = load(c.k, step + 1, next, turn);
+                }
+                if (warp == 8) {
+                    float top = lane < 8 ? vs : 0.f;
+#pragma unroll
+                    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = fmaxf(__shfl_sync(0xffffffffu, top, 0), 1.17549435e-38f);
+                    const float ref = fmaxf(v_ref, top), unit = fmaxf(vs / ref, 8.6736174e-19f);  // 2^-60: below, values count for nothing
+                    const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xFFu;
+                    Info &f = info[n % INFO];
+                    if (lane < 8) {
+                        f.k[lane] = ks;
+                        f.v_log[lane] = log2f(unit);
+                        f.v_inv[lane] = 1.f / unit;
+                    }
+                    if (lane == 0) {
+                        f.turn = v_ref == 0.f ? 1.f : v_ref / ref;
+                        f.v_ref = ref;
+                        f.there = int(mask);
+                    }
+                    v_ref = ref;
+                }
+                fence_async_smem();
+                mbar_arrive(k_full(stage));
+                if (!warp_wait(v_empty(stage), empty, abort_flag, S_ROOM)) { ok = false; break; }
+#pragma unroll
+                for (int turn = 0; turn < TURNS; ++turn) {
+                    store(v_smem + stage * C::OPERAND, turn, xv[turn], std::true_type());
+                    xv[turn] = load(c.v, step + 1, next, turn);
+                }
+                fence_async_smem();
+                mbar_arrive(v_full(stage));
+                number = next;
+                next = page_of(p, step + 2);
+            }
+        }
+    } else if (lane == 0) {
+        // ===== the products =====
+        constexpr uint32_t qk = instruction(KEYS, false), pv = instruction(DP, true);
+        uint32_t n = 0, n_p[2] = {0, 0}, n_q[2] = {0, 0};
+        bool ok = true;
+        auto scores = [&](int t, uint32_t step) {
+            const uint32_t qs = q_smem + t * C::OPERAND, ks = k_smem + (step % STAGES) * C::OPERAND;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
+                mma_ss(tmem + C::S_COL + 128 * t, descriptor(qs + off, 16), descriptor(ks + off, 16), qk, k != 0);
+            }
+            commit(s_full(t));
+            mbar_arrive(s_full(t));
+        };
+        for (int64_t at = begin; at < end && ok;) {
+            const Piece p = piece_at(at);
+            at += p.steps;
+            for (int t = 0; t < p.tiles && ok; ++t) ok = mbar_wait(q_ready(t), n_q[t]++ & 1, abort_flag, S_QUERIES);
+            if (ok) ok = mbar_wait(k_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_KEYS);
+            if (!ok) break;
+            fence_after();
+            for (int t = 0; t < p.tiles; ++t) scores(t, n);
+            commit(k_empty(n % STAGES));
+            for (int step = 0; step < p.steps && ok; ++step, ++n) {
+                if (!(ok = mbar_wait(v_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_VALUES))) break;
+                const bool more = step + 1 < p.steps;
+                for (int t = 0; t < p.tiles; ++t) {
+                    if (!(ok = mbar_wait(p_ready(t), n_p[t]++ & 1, abort_flag, S_WEIGHTS))) break;
+                    fence_after();
+                    const uint32_t vs = v_smem + (n % STAGES) * C::OPERAND;
+#pragma unroll
+                    for (int k = 0; k < KEYS / 16; ++k)
+                        mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, descriptor(vs + k * 2048, C::PANEL), pv, step != 0 || k != 0);
+                    if (more) {
+                        if (t == 0 && !(ok = mbar_wait(k_full((n + 1) % STAGES), ((n + 1) / STAGES) & 1, abort_flag, S_KEYS))) break;
+                        fence_after();
+                        scores(t, n + 1);
+                    } else commit(o_full(t));
+                }
+                if (!ok) break;
+                commit(v_empty(n % STAGES));
+                if (more) commit(k_empty((n + 1) % STAGES));
+            }
+        }
+        if (*abort_flag) {  // products in flight: time to end before their memory is given back
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000ll) {}
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+    using C = Cfg<DP>;
+    static std::atomic<uint64_t> prepared{0};
+    if (int e = allow_shared(tiles_kernel<T, FMT, DP>, C::SMEM, &prepared)) return e;
+    const unsigned grid = unsigned(sm_count());
+    const Plan plan = plan_at(a.ws + align256(grid * (sizeof(Join) + 2 * C::PART * sizeof(float))), s, a.group);
+    launch_pdl(plan_kernel, dim3(1), dim3(PLAN_CTA), 0, st, a, c, s, plan);
+    if (int e = check_launch("kvcache_attention (plan)")) return e;
+    launch_pdl(tiles_kernel<T, FMT, DP>, dim3(grid), dim3(THREADS), C::SMEM, st, a, c, s, plan);
+    if (int e = check_launch("kvcache_attention (tiles)")) return e;
+    launch_pdl(join_kernel<T, DP, ITEM_ROWS>, dim3(grid, ITEM_ROWS / JOIN_ROWS), dim3(JOIN_CTA), 0, st, a, c);
+    return check_launch("kvcache_attention (join)");
+}
+
+}  // namespace
+
+size_t tiles_workspace(const Cache &c, const Seqs &s, int group) {
+    const size_t part = c.dim <= 64 ? Cfg<64>::PART : Cfg<128>::PART;
+    return align256(size_t(sm_count()) * (sizeof(Join) + 2 * part * sizeof(float))) + plan_bytes(s, group);
+}
+
+int launch_tiles(int dtype, int format, const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+#define DX_CALL(T, FMT) return c.dim <= 64 ? launch<T, FMT, 64>(a, c, s, st) : launch<T, FMT, 128>(a, c, s, st)
+    if (dtype == DX_F16) {
+        if (format == DX_CACHE_I8) DX_CALL(f16, DX_CACHE_I8);
+        DX_CALL(f16, DX_CACHE_E4M3);
+    }
+    if (format == DX_CACHE_I8) DX_CALL(bf16, DX_CACHE_I8);
+    DX_CALL(bf16, DX_CACHE_E4M3);
+#undef DX_CALL
+}
+
+}  // namespace kv
+}  // namespace dx
+
+extern "C" int dx_kvcache_status(void *stream) {
+    using namespace dx;
+    cudaStream_t st = as_stream(stream);
+    cudaError_t e = cudaStreamSynchronize(st);
+    int status = 0;
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&status, kv::g_status, sizeof(int));
+    if (e != cudaSuccess) return fail(DX_E_CUDA, "kvcache_status: %s", cudaGetErrorString(e));
+    if (status == 0) return DX_OK;
+    const int zero = 0;
+    cudaMemcpyToSymbol(kv::g_status, &zero, sizeof(int));
+    static const char *const where[] = {"", "keys", "values", "scores", "weights", "queries", "the output", "room for a step"};
+    return fail(DX_E_CUDA, "kvcache_attention: a bounded wait for %s ran out", status < 8 ? where[status] : "?");
+}

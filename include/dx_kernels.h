@@ -337,6 +337,8 @@ size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_heads, const dx
 int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
                          double scale, int64_t max_new, int64_t window, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes,
                          int32_t *flag, void *stream);
+/* As dx_matmul_status, for the tensor-core kernel of dx_kvcache_attention on the current device. */
+int dx_kvcache_status(void *stream);
 
 /* ---- changeshape -----------------------------------------------------------
  * Replace launch_transpose/concat/broadcastTo/indexselect/repeat

@@ -157,6 +157,8 @@ def check_attention(TF, b, Q, scale, window=0, max_new=0, Out=None):
     else:
         Out.copy_(filler)
     TF.kvcache_attention(Q, *b.cache(), *b.seqs(), scale, max_new, window, Out, b.flag)
+    from deepx_b200 import _native as N
+    N.check(N.lib.dx_kvcache_status(None))
     assert int(b.flag) == 0
     last = b.host_starts[-1]
     assert torch.equal(Out[last:], filler[last:]), "rows behind the last sequence changed"
