@@ -9,14 +9,16 @@
 // Four exponentials' worth of tensor work (512 multiply-adds) goes with each exponential at 128 dimensions: a step of both tiles costs
 // 2048 cycles of the tensor cores and 2048 of the exponential unit, so both bound this kernel; what is neither stays off their threads.
 //
-// Roles (13 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each; 8-11 turn codes into halfs (sixteen a thread and turn,
-// loaded a step ahead); one thread of warp 12 issues the products.  Codes become halfs unscaled and
-// exact; the scales of a step's eight groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of
-// the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
-// scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
+// Roles (16 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each, and the first thread of each issues its tile's
+// products (its P V, and behind it the scores of the next step, the moment its weights are there); 8-11 turn the codes of K into halfs,
+// 12-15 those of V (sixteen a thread and turn, loaded a step ahead).  Codes become halfs unscaled and exact; the scales of a step's
+// eight groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of the largest so far) into the
+// exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is scaled again (in TMEM, by the
+// row's thread), which after the first steps hardly happens.
 //
-// The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it; items
-// that more than one block works on are joined as in kvcache_attention.cu.
+// The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it, where an
+// item counts OVERHEAD steps more than it has (its queries, its way out; without that the blocks of a prompt's first rows, whose items
+// have few steps, took twice the others' time); items that more than one block works on are joined as in kvcache_attention.cu.
 //
 // Every wait is bounded by a clock; when one runs out a status word is set (dx_kvcache_status), all roles leave, TMEM is freed.
 #include <mutex>
@@ -28,20 +30,28 @@ namespace kv {
 namespace {
 
 constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 128, GROUPS = KEYS / 16;
-constexpr int THREADS = 13 * 32;
+constexpr int THREADS = 16 * 32;
 constexpr int STAGES = 2, INFO = 4;
+constexpr int OVERHEAD = 2;
 constexpr int PLAN_CTA = 1024;
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
 enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
 
 __device__ int g_status = 0;
 
-// The plan: for each group (256 rows of a sequence, all heads) its sequence, which 256 rows, and the steps in front of it.
+// 256 rows of a sequence, the same for all heads: rows first_row.. of the flattened (new token, head of the group), tokens lo..hi
+// in steps of KEYS from lo (a multiple of KEYS).
+struct alignas(16) Group {
+    int64_t row0;
+    int b, first, end;  // sequence, position of its first new token, tokens its pages can be read for
+    int first_row, rows, lo, hi, steps;
+};
+// The plan: the groups, the units of the line in front of each, the groups in front of a sequence.
 struct Plan {
     int64_t *before;  // [groups + 1]
-    int2 *group;      // {sequence, tile of 256 rows}
-    int *first;       // [batch + 1] groups in front of a sequence
-    int *count;       // groups
+    Group *group;
+    int *first;  // [batch + 1]
+    int *count;  // groups
 };
 __host__ __device__ inline int64_t most_groups(const Seqs &s, int group) { return s.rows * group / ITEM_ROWS + s.batch; }
 __host__ __device__ inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -50,8 +60,8 @@ __host__ __device__ inline Plan plan_at(uint8_t *base, const Seqs &s, int group)
     Plan p;
     p.before = reinterpret_cast<int64_t *>(base);
     base += align256(size_t(n + 1) * 8);
-    p.group = reinterpret_cast<int2 *>(base);
-    base += align256(size_t(n) * 8);
+    p.group = reinterpret_cast<Group *>(base);
+    base += align256(size_t(n) * sizeof(Group));
     p.first = reinterpret_cast<int *>(base);
     base += align256(size_t(s.batch + 1) * 4);
     p.count = reinterpret_cast<int *>(base);
@@ -59,15 +69,15 @@ __host__ __device__ inline Plan plan_at(uint8_t *base, const Seqs &s, int group)
 }
 inline size_t plan_bytes(const Seqs &s, int group) {
     const int64_t n = most_groups(s, group);
-    return align256(size_t(n + 1) * 8) + align256(size_t(n) * 8) + align256(size_t(s.batch + 1) * 4) + 256;
+    return align256(size_t(n + 1) * 8) + align256(size_t(n) * sizeof(Group)) + align256(size_t(s.batch + 1) * 4) + 256;
 }
 
-// The keys of one item: rows first_row..first_row + rows of the sequence.
-struct Item {
-    int first_row, rows, lo, hi, steps;  // tokens lo..hi, in steps of KEYS from lo (a multiple of KEYS)
-};
-__device__ __forceinline__ Item item_of(const Seq &q, const Attn &a, int tile) {
-    Item x;
+__device__ __forceinline__ Group group_of(const Seq &q, const Attn &a, int b, int tile) {
+    Group x;
+    x.row0 = q.row0;
+    x.b = b;
+    x.first = q.first;
+    x.end = q.end;
     x.first_row = tile * ITEM_ROWS;
     x.rows = int(min(int64_t(q.n) * a.group - x.first_row, int64_t(ITEM_ROWS)));
     const int64_t p0 = int64_t(q.first) + x.first_row / a.group, p1 = int64_t(q.first) + (x.first_row + x.rows - 1) / a.group;
@@ -130,9 +140,9 @@ __global__ void __launch_bounds__(PLAN_CTA) plan_kernel(Attn a, Cache c, Seqs s,
                 if (p.first[mid] <= g) lo = mid;
                 else hi = mid;
             }
-            const int tile = int(g - p.first[lo]);
-            p.group[g] = make_int2(lo, tile);
-            n = int64_t(item_of(seq_at(s, c, lo), a, tile).steps) * c.heads;
+            const Group x = group_of(seq_at(s, c, lo), a, lo, int(g - p.first[lo]));
+            p.group[g] = x;
+            n = (int64_t(x.steps) + OVERHEAD) * c.heads;
         }
         const int64_t at = steps + block_scan(n, warp_sum, total);
         if (g < groups) p.before[g] = at;
@@ -193,15 +203,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-          "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile(
@@ -278,9 +285,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(k_full(i), 128);
-            mbar_init(k_empty(i), 1);
+            mbar_init(k_empty(i), 2);  // one arrival for each tile
             mbar_init(v_full(i), 128);
-            mbar_init(v_empty(i), 1);
+            mbar_init(v_empty(i), 2);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(s_full(t), 2);  // the products' completion, and the issuing thread's own arrival, behind which info is visible
@@ -291,7 +298,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         abort_shared = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -306,7 +313,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
     const int groups = *plan.count;
     const int64_t total = plan.before[groups];
-    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / 2));
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / (OVERHEAD + 2)));
     const bool work = total > 0 && int64_t(blockIdx.x) < blocks;
     const int64_t begin = work ? total * blockIdx.x / blocks : 0, end = work ? total * (blockIdx.x + 1) / blocks : 0;
     if (threadIdx.x == 0) join->parts = 0;
@@ -314,27 +321,24 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         if (plan.before[g] <= begin && plan.before[g + 1] > begin) found_group = g;
     __syncthreads();
 
-    // Every role walks the same pieces: for each, its sequence, head, rows and steps.
+    // Every role walks the same pieces: for each, its group, head and steps (none where the piece holds only units of OVERHEAD).
     struct Piece {
-        Seq sq;
-        Item it;
-        int b, head, step0, steps, tiles;
-        int64_t item_begin, item_end;
+        Group it;
+        int head, step0, steps, tiles;
+        int64_t item_begin, next;  // units of the line: where the item begins, where the next piece does
     };
     int group = found_group;
     auto piece_at = [&](int64_t at) {
         Piece p;
         while (at >= plan.before[group + 1]) ++group;
-        const int2 gt = plan.group[group];
-        p.b = gt.x;
-        p.sq = seq_at(s, c, p.b);
-        p.it = item_of(p.sq, a, gt.y);
         const int64_t g0 = plan.before[group];
-        p.head = int((at - g0) / p.it.steps);
-        p.item_begin = g0 + int64_t(p.head) * p.it.steps;
-        p.item_end = p.item_begin + p.it.steps;
-        p.step0 = int(at - p.item_begin);
-        p.steps = int(min(end, p.item_end) - at);
+        p.it = plan.group[group];
+        const int units = p.it.steps + OVERHEAD;
+        p.head = int((at - g0) / units);
+        p.item_begin = g0 + int64_t(p.head) * units;
+        p.next = min(end, p.item_begin + units);
+        p.step0 = max(int(at - p.item_begin) - OVERHEAD, 0);
+        p.steps = max(int(p.next - p.item_begin) - OVERHEAD, 0) - p.step0;
         p.tiles = p.it.rows > TILE_ROWS ? 2 : 1;
         return p;
     };
@@ -344,39 +348,75 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = uint32_t(warp & 3) * 32u << 16;
         const uint32_t s_tmem = tmem + lanes + C::S_COL + 128 * t, o_tmem = tmem + lanes + C::O_COL + DP * t;
-        uint32_t n_s = 0, n_o = 0;
-        int n_info = 0;
+        uint32_t n = 0, n_s = 0, n_p = 0, n_q = 0, n_o = 0;  // steps of the block; phases of this tile's barriers
         bool ok = true;
+        constexpr uint32_t qk = instruction(KEYS, false), pv = instruction(DP, true);
+        // By the tile's first thread: the scores of step `n`, whose keys are awaited.  What info holds of the step is visible behind its arrival.
+        auto issue_scores = [&](uint32_t n) {
+            const int stage = n % STAGES;
+            if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
+            fence_after();
+            const uint32_t qs = q_smem + t * C::OPERAND, ks = k_smem + stage * C::OPERAND;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
+                mma_ss(tmem + C::S_COL + 128 * t, descriptor(qs + off, 16), descriptor(ks + off, 16), qk, k != 0);
+            }
+            commit(s_full(t));
+            mbar_arrive(s_full(t));
+            commit(k_empty(stage));
+            return true;
+        };
         for (int64_t at = begin; at < end && ok;) {
             const Piece p = piece_at(at);
-            at += p.steps;
+            const bool starts_here = at == begin;
+            at = p.next;
+            if (p.steps == 0) continue;
             if (t >= p.tiles) {
-                n_info += p.steps;
+                // No rows: the tile's arrivals all the same, step by step, so that its waits never fall behind or run ahead by a phase.
+                if (r == 0) {
+                    for (int step = 0; step < p.steps && ok; ++step) {
+                        const int stage = (n + step) % STAGES;
+                        const uint32_t full = ((n + step) / STAGES) & 1;
+                        ok = mbar_wait(k_full(stage), full, abort_flag, S_KEYS);
+                        mbar_arrive(k_empty(stage));
+                        ok = ok && mbar_wait(v_full(stage), full, abort_flag, S_VALUES);
+                        mbar_arrive(v_empty(stage));
+                    }
+                }
+                n += p.steps;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
                 continue;
             }
             const int row = t * TILE_ROWS + r;
             const bool live = row < p.it.rows;
             const int fr = p.it.first_row + row, i = live ? fr / a.group : 0;
-            const int last = live ? int(max(min(int64_t(p.sq.first) + i, int64_t(p.sq.end) - 1), int64_t(-1))) : -1;         // sees keys up to here
-            const int64_t after = live && a.window > 0 ? int64_t(p.sq.first) + i - a.window : -(int64_t(1) << 40);  // and behind this one
+            const int last = live ? int(max(min(int64_t(p.it.first) + i, int64_t(p.it.end) - 1), int64_t(-1))) : -1;  // sees keys up to here
+            const int64_t after = live && a.window > 0 ? int64_t(p.it.first) + i - a.window : -(int64_t(1) << 40);   // and behind this one
             // ---- the row of Q as halfs into shared memory, a bfloat16 row divided by a power of two first ----
             float c_row = a.scale_log2;
             {
-                const T *q = static_cast<const T *>(a.q) + (p.sq.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
-                Pack<T, 8> x[DP / 8];
-                float amax = 0.f;
+                const T *q = static_cast<const T *>(a.q) + (p.it.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+                uint4 x[DP / 8];
+                if (a.q_vec) {
 #pragma unroll
-                for (int k = 0; k < DP / 8; ++k) {
-                    if (live && k * 8 < c.dim && a.q_vec) x[k] = ld_cached<T, 8>(q + k * 8);
-                    else {
+                    for (int k = 0; k < DP / 8; ++k) x[k] = live && k * 8 < c.dim ? *reinterpret_cast<const uint4 *>(q + k * 8) : make_uint4(0, 0, 0, 0);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[k].v[e] = live && k * 8 < c.dim ? q[k * 8 + e] : from_compute<T>(0.f);
+                    for (int k = 0; k < DP / 8; ++k) {
+                        uint16_t h[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = live && k * 8 < c.dim ? reinterpret_cast<const uint16_t *>(q)[k * 8 + e] : uint16_t(0);
+                        x[k] = make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16, h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k].v[e])));
                 }
                 float down = 1.f;
                 if constexpr (std::is_same<T, bf16>::value) {
+                    __nv_bfloat162 top2 = __float2bfloat162_rn(0.f);
+#pragma unroll
+                    for (int k = 0; k < DP / 8; ++k)
+                        for (uint32_t w : {x[k].x, x[k].y, x[k].z, x[k].w}) top2 = __hmax2(top2, __habs2(*reinterpret_cast<__nv_bfloat162 *>(&w)));
+                    const float amax = fmaxf(to_compute(top2.x), to_compute(top2.y));
                     const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
                     if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
                         down = __uint_as_float((254u - e) << 23);
@@ -386,51 +426,71 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 const uint32_t dst = q_smem + t * C::OPERAND + r * 128;
 #pragma unroll
                 for (int k = 0; k < DP / 8; ++k) {
-                    uint32_t w[4];
+                    uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+                    if constexpr (std::is_same<T, bf16>::value) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = half2_bits(to_compute(x[k].v[2 * e]) * down, to_compute(x[k].v[2 * e + 1]) * down);
+                        for (int e = 0; e < 4; ++e) w[e] = half2_bits(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xFFFF0000u) * down);
+                    }
                     sts128(dst + (k >> 3) * C::PANEL + (((k & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
             }
             fence_async_smem();
             fence_before();  // the reads of O of the item before
             mbar_arrive(q_ready(t));
-            const int tile_first = int(min(int64_t(p.sq.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.sq.end) - 1));  // least `last` of the tile
-            const int64_t tile_after = a.window > 0 ? int64_t(p.sq.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
+            if (r == 0) ok = mbar_wait(q_ready(t), n_q & 1, abort_flag, S_QUERIES) && issue_scores(n);
+            ++n_q;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            const int tile_first = int(min(int64_t(p.it.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.it.end) - 1));  // least `last` of the tile
+            const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
 
             float m = NEG_INF, v_ref = 1.f;
             uint64_t l2 = pair(0.f, 0.f);
-            for (int step = 0; step < p.steps; ++step, ++n_info) {
+            for (int step = 0; step < p.steps; ++step, ++n) {
                 const int j0 = p.it.lo + (p.step0 + step) * KEYS;
                 if (!warp_wait(s_full(t), n_s & 1, abort_flag, S_SCORES)) { ok = false; break; }
                 ++n_s;
                 fence_after();
-                const Info &f = info[n_info % INFO];
+                const Info &f = info[n % INFO];
                 const int there = f.there;
                 v_ref = f.v_ref;
                 const bool masked = j0 + KEYS - 1 > tile_first || j0 <= tile_after || there != (1 << GROUPS) - 1;  // the same in all threads
-                const int hi = last - j0;                                                       // columns up to here are seen
-                const int lo = int(max(after - j0, int64_t(-1)));                               // from behind here
-                auto seen = [&](int col) { return col <= hi && col > lo && (there >> (col >> 4) & 1); };
-                // ---- the row's largest score ----
-                float top = NEG_INF;
+                // the columns of a run of 32 that this row sees, a bit each
+                auto seen = [&](int col) {
+                    const int hi = min(max(last - j0 - col + 1, 0), 32), lo = int(min(max(after - j0 - col + 1, int64_t(0)), int64_t(32)));
+                    const uint32_t up_to = hi == 32 ? ~0u : (1u << hi) - 1, before = lo == 32 ? ~0u : (1u << lo) - 1;
+                    const uint32_t have = ((there >> (col >> 4)) & 1 ? 0xFFFFu : 0u) | ((there >> ((col >> 4) + 1)) & 1 ? 0xFFFF0000u : 0u);
+                    return up_to & ~before & have;
+                };
+                auto hide = [&](uint32_t (&x)[32], int col) {
+                    const uint32_t bits = seen(col);
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    uint32_t x[32];
-                    tmem_ld32(s_tmem + 32 * ch, x);
+                    for (int e = 0; e < 32; ++e)
+                        if (!(bits >> e & 1)) x[e] = __float_as_uint(NEG_INF);
+                };
+                auto largest = [&](const uint32_t (&x)[32], int col) {
+                    float v[4];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        v[g] = fmaxf(__uint_as_float(x[8 * g]), __uint_as_float(x[8 * g + 1]));
+#pragma unroll
+                        for (int e = 2; e < 8; ++e) v[g] = fmaxf(v[g], __uint_as_float(x[8 * g + e]));
+                    }
+                    return fmaxf(fmaxf(v[0], v[1]) * (c_row * f.k[col >> 4]), fmaxf(v[2], v[3]) * (c_row * f.k[(col >> 4) + 1]));
+                };
+                // ---- the row's largest score: columns 64..127, then 0..63, which stay in registers ----
+                uint32_t x[2][32];
+                float top = NEG_INF;
+#pragma unroll 1
+                for (int half = 64; half >= 0; half -= 64) {
+                    tmem_ld32(s_tmem + half, x[0]);
+                    tmem_ld32(s_tmem + half + 32, x[1]);
                     wait_ld();
                     if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!seen(32 * ch + e)) x[e] = __float_as_uint(NEG_INF);
+                        hide(x[0], half);
+                        hide(x[1], half + 32);
                     }
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        float v = __uint_as_float(x[16 * g]);
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) v = fmaxf(v, __uint_as_float(x[16 * g + e]));
-                        top = fmaxf(top, v * (c_row * f.k[2 * ch + g]));
-                    }
+                    top = fmaxf(top, fmaxf(largest(x[0], half), largest(x[1], half + 32)));
                 }
                 const float turn = f.turn;
                 const bool rise = top > m + LAG;
@@ -444,46 +504,70 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     by *= turn;
                     if (step > 0) {  // the products of the step before are complete: these scores were issued behind them
 #pragma unroll 1
-                        for (int d = 0; d < DP; d += 32) {
-                            uint32_t x[32];
-                            tmem_ld32(o_tmem + d, x);
+                        for (int d = 0; d < DP; d += 16) {
+                            uint32_t y[16];
+                            tmem_ld16(o_tmem + d, y);
                             wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * by);
-                            tmem_st32(o_tmem + d, x);
+                            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * by);
+                            tmem_st16(o_tmem + d, y);
                         }
                     }
                 }
                 const float base_m = UP - (m == NEG_INF ? 0.f : m);
                 // ---- weights, over the scores that have been read ----
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    uint32_t x[32], w[16];
-                    tmem_ld32(s_tmem + 32 * ch, x);
-                    wait_ld();
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float cg = c_row * f.k[2 * ch + g], mg = base_m + f.v_log[2 * ch + g], ig = f.v_inv[2 * ch + g];
-                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float y0, y1;
-                            unpair(fma2(pair(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1])), c2, m2), y0, y1);
-                            if (masked) {
-                                y0 = seen(32 * ch + 16 * g + e) ? y0 : NEG_INF;
-                                y1 = seen(32 * ch + 16 * g + e + 1) ? y1 : NEG_INF;
-                            }
-                            y0 = exp2_approx(y0);
-                            y1 = exp2_approx(y1);
-                            l2 = fma2(pair(y0, y1), i2, l2);
-                            w[8 * g + e / 2] = half2_bits(y0, y1);
+#pragma unroll 1
+                for (int half = 0; half < KEYS; half += 64) {
+                    if (half) {
+                        tmem_ld32(s_tmem + half, x[0]);
+                        tmem_ld32(s_tmem + half + 32, x[1]);
+                        wait_ld();
+                        if (masked) {
+                            hide(x[0], half);
+                            hide(x[1], half + 32);
                         }
                     }
-                    tmem_st16(s_tmem + 16 * ch, w);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const int group16 = (half >> 4) + 2 * q + g;
+                            const float cg = c_row * f.k[group16], mg = base_m + f.v_log[group16], ig = f.v_inv[group16];
+                            const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                            for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                                float y0, y1;
+                                unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
+                                y0 = exp2_approx(y0);
+                                y1 = exp2_approx(y1);
+                                l2 = fma2(pair(y0, y1), i2, l2);
+                                w[e / 2] = half2_bits(y0, y1);
+                            }
+                        }
+                        tmem_st16(s_tmem + half / 2 + 16 * q, w);
+                    }
                 }
                 wait_st();
                 fence_before();
                 mbar_arrive(p_ready(t));
+                if (r == 0) {
+                    const int stage = n % STAGES;
+                    ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
+                    if (ok) {
+                        fence_after();
+                        const uint32_t vs = v_smem + stage * C::OPERAND;
+#pragma unroll
+                        for (int k = 0; k < KEYS / 16; ++k)
+                            mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, descriptor(vs + k * 2048, C::PANEL), pv, step != 0 || k != 0);
+                        commit(v_empty(stage));
+                        if (step + 1 < p.steps) ok = issue_scores(n + 1);
+                        else commit(o_full(t));
+                    }
+                }
+                ++n_p;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
             }
             if (!ok) break;
             // ---- the way out ----
@@ -495,7 +579,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             const float sum = l0 + l1, by = sum == 0.f ? 0.f : v_ref / sum;
             const bool whole = p.step0 == 0 && p.steps == p.it.steps;
             float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
-            T *out = static_cast<T *>(a.out) + (p.sq.row0 + i) * a.out_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+            T *out = static_cast<T *>(a.out) + (p.it.row0 + i) * a.out_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
             if (!whole && live) {
                 part[ITEM_ROWS * DP + row] = m;
                 part[ITEM_ROWS * DP + ITEM_ROWS + row] = sum;
@@ -530,77 +614,90 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                 }
             }
-            if (threadIdx.x == 0 && p.step0 > 0 && at - p.steps == begin && p.item_begin >= total * (int64_t(blockIdx.x) - 1) / blocks) {
-                join->row0 = p.sq.row0;
+            // the item's first steps are the block before's: here is where it is joined
+            if (threadIdx.x == 0 && starts_here && p.step0 > 0 && total * (int64_t(blockIdx.x) - 1) / blocks - p.item_begin <= OVERHEAD) {
+                join->row0 = p.it.row0;
                 join->first_row = p.it.first_row;
                 join->rows = p.it.rows;
                 join->head = p.head;
-                join->parts = int((p.item_end * blocks - 1) / total) - int(blockIdx.x) + 2;
+                join->parts = int(((p.item_begin + p.it.steps + OVERHEAD) * blocks - 1) / total) - int(blockIdx.x) + 2;
             }
         }
-    } else if (warp < 12) {
-        // ===== codes into halfs =====
-        const int tid = threadIdx.x & 127;
+        if (*abort_flag && r == 0) {  // products in flight: time to end before their memory is given back
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000ll) {}
+        }
+    } else {
+        // ===== codes into halfs: keys (warps 8-11) or values (12-15) =====
+        const bool is_v = warp >= 12;
         constexpr int PER_ROW = DP / 16, TURNS = KEYS * PER_ROW / 128, TURN_ROWS = 128 / PER_ROW;
-        const int ch = tid % PER_ROW, r0 = tid / PER_ROW;  // sixteen codes of row r0 + TURN_ROWS * turn
+        // sixteen codes, chunk ch of row r0 + TURN_ROWS * turn: eight lanes in a row are four chunks of an even and an odd row, whose halfs
+        // go to different banks
+        const int ch = DP == 64 ? lane & 3 : (lane & 3) | (lane >> 3 & 1) << 2;
+        const int r0 = (warp & 3) * (TURN_ROWS / 4) + (DP == 64 ? lane >> 2 : (lane >> 2 & 1) | lane >> 4 << 1);
         const bool in_dim = ch * 16 < c.dim;
-        // the two chunks of a thread, the second first in the second panel: eight lanes then touch every bank once
-        const int swap = (ch >> 2) & 1, c0 = (ch & 3) * 2 + swap, c1 = c0 ^ 1;
-        // lane g of a warp knows the page of group g of a step
-        auto page_of = [&](const Piece &p, int step) {
-            const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
-            int32_t number = -1;
-            if (step < p.steps && j < p.it.hi) {
-                number = s.table[int64_t(p.b) * s.cols + (j >> c.page_shift)];
-                if (number < 0 || number >= c.pages) {
-                    if (warp == 8 && lane < 8) raise(a.flag, FLAG_PAGE);
-                    number = -1;
-                }
-            }
-            return number;
-        };
+        const uint8_t *codes = (is_v ? c.v : c.k) + (r0 & 15) * c.dim + ch * 16;
+        const uint32_t smem = (is_v ? v_smem : k_smem) + (ch >> 2) * C::PANEL + r0 * 128;
+        const int at0 = ((ch & 3) * 2 ^ (r0 & 7)) << 4, at1 = at0 ^ 16;
         uint32_t n = 0;
         bool ok = true;
         for (int64_t at = begin; at < end && ok;) {
             const Piece p = piece_at(at);
-            at += p.steps;
-            uint4 xk[TURNS], xv[TURNS];
-            int32_t number = page_of(p, 0), next = page_of(p, 1);
-            auto load = [&](const uint8_t *codes, int step, int32_t numbers, int turn) {
-                const int row = r0 + TURN_ROWS * turn, j = p.it.lo + (p.step0 + step) * KEYS + row;
-                const int32_t page = __shfl_sync(0xffffffffu, numbers, row >> 4);  // a warp's rows of a turn are of one group
-                if (page < 0 || j >= p.it.hi || !in_dim) return make_uint4(0, 0, 0, 0);
-                return *reinterpret_cast<const uint4 *>(codes + ((int64_t(page) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim + ch * 16);
+            at = p.next;
+            if (p.steps == 0) continue;
+            // lane g of a warp knows group g of a step: its page, and where its codes begin (-1: nowhere)
+            const int32_t *table = s.table + int64_t(p.it.b) * s.cols;
+            auto page_of = [&](int step) {
+                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
+                int32_t number = -1;
+                if (step < p.steps && j < p.it.hi) {
+                    number = table[j >> c.page_shift];
+                    if (number < 0 || number >= c.pages) {
+                        if (warp == 8 && lane < 8) raise(a.flag, FLAG_PAGE);
+                        number = -1;
+                    }
+                }
+                return number;
             };
-            auto store = [&](uint32_t dst, int turn, uint4 x, auto finite) {
+            auto begin_of = [&](int step, int32_t number) {
+                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
+                return number < 0 ? int64_t(-1) : ((int64_t(number) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim;
+            };
+            uint4 x[TURNS];
+            auto load = [&](int64_t offsets, int left, int turn) {
                 const int row = r0 + TURN_ROWS * turn;
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                uint32_t h[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) decode4<FMT, decltype(finite)::value>(w[e], h[2 * e], h[2 * e + 1]);
-                const uint32_t line = dst + (ch >> 2) * C::PANEL + row * 128;
-                sts128(line + ((c0 ^ (row & 7)) << 4), swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
-                sts128(line + ((c1 ^ (row & 7)) << 4), swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
+                const int64_t off = __shfl_sync(0xffffffffu, offsets, row >> 4);  // a warp's rows of a turn are of one group
+                if (off < 0 || row >= left || !in_dim) return make_uint4(0, 0, 0, 0);
+                return *reinterpret_cast<const uint4 *>(codes + off);
             };
+            int32_t number = page_of(0), next = page_of(1);
+            {
+                const int64_t offsets = begin_of(0, number);
 #pragma unroll
-            for (int turn = 0; turn < TURNS; ++turn) xk[turn] = load(c.k, 0, number, turn);
-#pragma unroll
-            for (int turn = 0; turn < TURNS; ++turn) xv[turn] = load(c.v, 0, number, turn);
+                for (int turn = 0; turn < TURNS; ++turn) x[turn] = load(offsets, p.it.hi - p.it.lo - p.step0 * KEYS, turn);
+            }
             float v_ref = 0.f;
             for (int step = 0; step < p.steps; ++step, ++n) {
                 const int stage = n % STAGES;
-                const uint32_t empty = ((n / STAGES) & 1) ^ 1;
                 float ks = 1.f, vs = 0.f;
                 const bool there = number >= 0;
                 if (warp == 8 && there) {
                     ks = c.k_scale[int64_t(number) * c.heads + p.head];
                     vs = c.v_scale[int64_t(number) * c.heads + p.head];
                 }
-                if (!warp_wait(k_empty(stage), empty, abort_flag, S_ROOM)) { ok = false; break; }
+                const int64_t offsets = begin_of(step + 1, next);
+                const int left = p.it.hi - p.it.lo - (p.step0 + step + 1) * KEYS;
+                if (!warp_wait(is_v ? v_empty(stage) : k_empty(stage), ((n / STAGES) & 1) ^ 1, abort_flag, S_ROOM)) { ok = false; break; }
+                const uint32_t dst = smem + stage * C::OPERAND;
 #pragma unroll
                 for (int turn = 0; turn < TURNS; ++turn) {
-                    store(k_smem + stage * C::OPERAND, turn, xk[turn], std::false_type());
-                    xk[turn] = load(c.k, step + 1, next, turn);
+                    const uint32_t w[4] = {x[turn].x, x[turn].y, x[turn].z, x[turn].w};
+                    x[turn] = load(offsets, left, turn);
+                    uint32_t h[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) decode4<FMT, true>(w[e], h[2 * e], h[2 * e + 1]);
+                    sts128(dst + turn * (TURN_ROWS * 128) + at0, h[0], h[1], h[2], h[3]);
+                    sts128(dst + turn * (TURN_ROWS * 128) + at1, h[4], h[5], h[6], h[7]);
                 }
                 if (warp == 8) {
                     float top = lane < 8 ? vs : 0.f;
@@ -611,7 +708,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xFFu;
                     Info &f = info[n % INFO];
                     if (lane < 8) {
-                        f.k[lane] = ks;
+                        f.k[lane] = fmaxf(ks, 7.8886091e-31f);  // 2^-100: a factor of zero would make a hidden score not a number
                         f.v_log[lane] = log2f(unit);
                         f.v_inv[lane] = 1.f / unit;
                     }
@@ -623,74 +720,17 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     v_ref = ref;
                 }
                 fence_async_smem();
-                mbar_arrive(k_full(stage));
-                if (!warp_wait(v_empty(stage), empty, abort_flag, S_ROOM)) { ok = false; break; }
-#pragma unroll
-                for (int turn = 0; turn < TURNS; ++turn) {
-                    store(v_smem + stage * C::OPERAND, turn, xv[turn], std::true_type());
-                    xv[turn] = load(c.v, step + 1, next, turn);
-                }
-                fence_async_smem();
-                mbar_arrive(v_full(stage));
+                mbar_arrive(is_v ? v_full(stage) : k_full(stage));
                 number = next;
-                next = page_of(p, step + 2);
+                next = page_of(step + 2);
             }
-        }
-    } else if (lane == 0) {
-        // ===== the products =====
-        constexpr uint32_t qk = instruction(KEYS, false), pv = instruction(DP, true);
-        uint32_t n = 0, n_p[2] = {0, 0}, n_q[2] = {0, 0};
-        bool ok = true;
-        auto scores = [&](int t, uint32_t step) {
-            const uint32_t qs = q_smem + t * C::OPERAND, ks = k_smem + (step % STAGES) * C::OPERAND;
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
-                mma_ss(tmem + C::S_COL + 128 * t, descriptor(qs + off, 16), descriptor(ks + off, 16), qk, k != 0);
-            }
-            commit(s_full(t));
-            mbar_arrive(s_full(t));
-        };
-        for (int64_t at = begin; at < end && ok;) {
-            const Piece p = piece_at(at);
-            at += p.steps;
-            for (int t = 0; t < p.tiles && ok; ++t) ok = mbar_wait(q_ready(t), n_q[t]++ & 1, abort_flag, S_QUERIES);
-            if (ok) ok = mbar_wait(k_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_KEYS);
-            if (!ok) break;
-            fence_after();
-            for (int t = 0; t < p.tiles; ++t) scores(t, n);
-            commit(k_empty(n % STAGES));
-            for (int step = 0; step < p.steps && ok; ++step, ++n) {
-                if (!(ok = mbar_wait(v_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_VALUES))) break;
-                const bool more = step + 1 < p.steps;
-                for (int t = 0; t < p.tiles; ++t) {
-                    if (!(ok = mbar_wait(p_ready(t), n_p[t]++ & 1, abort_flag, S_WEIGHTS))) break;
-                    fence_after();
-                    const uint32_t vs = v_smem + (n % STAGES) * C::OPERAND;
-#pragma unroll
-                    for (int k = 0; k < KEYS / 16; ++k)
-                        mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, descriptor(vs + k * 2048, C::PANEL), pv, step != 0 || k != 0);
-                    if (more) {
-                        if (t == 0 && !(ok = mbar_wait(k_full((n + 1) % STAGES), ((n + 1) / STAGES) & 1, abort_flag, S_KEYS))) break;
-                        fence_after();
-                        scores(t, n + 1);
-                    } else commit(o_full(t));
-                }
-                if (!ok) break;
-                commit(v_empty(n % STAGES));
-                if (more) commit(k_empty((n + 1) % STAGES));
-            }
-        }
-        if (*abort_flag) {  // products in flight: time to end before their memory is given back
-            const long long t0 = clock64();
-            while (clock64() - t0 < 2000000ll) {}
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {

@@ -260,6 +260,15 @@ def test_attention_row_of_no_number_stays_alone(TF):
         assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page", [(14, 2, 64, 16), (8, 2, 128, 64)])
+def test_attention_of_a_mixed_batch(TF, q_heads, kv_heads, dim, page):
+    """Prompts, prompts continued and single tokens in one call: items of one tile of rows and of two in the same block, many of each."""
+    lens = [5000, 700, 3000, 900, 64, 2500, 4000, 1, 1300, 2222, 650, 3333]
+    new = [1, 700, 300, 1, 64, 37, 500, 1, 19, 1, 650, 128]
+    b = P.Batch(25, lens, new, kv_heads, dim, page, "e4m3", extra_rows=1).fill(lens)
+    check_attention(TF, b, b.rand(b.rows, q_heads, dim, dtype=torch.bfloat16), dim ** -0.5, max_new=700)
+
+
 def test_attention_many_sequences(TF):
     """More sequences than a block has threads, of very different lengths, some empty."""
     lens = [(37 * i) % 211 for i in range(700)]
