@@ -32,7 +32,10 @@ namespace {
 constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 128, GROUPS = KEYS / 16;
 constexpr int THREADS = 16 * 32;
 constexpr int STAGES = 2, INFO = 4;
-constexpr int OVERHEAD = 2;
+constexpr int OVERHEAD = 4;
+// Registers of a thread: a softmax thread holds a row's 128 scores at once.  The block is launched with 128 for every thread.
+constexpr int SOFTMAX_REGS = 184, CONVERT_REGS = 72;
+static_assert((SOFTMAX_REGS + CONVERT_REGS) * 256 <= THREADS * 128, "the split must fit what the block is launched with");
 constexpr int PLAN_CTA = 1024;
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
 enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
@@ -351,16 +354,18 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         uint32_t n = 0, n_s = 0, n_p = 0, n_q = 0, n_o = 0;  // steps of the block; phases of this tile's barriers
         bool ok = true;
         constexpr uint32_t qk = instruction(KEYS, false), pv = instruction(DP, true);
+        const uint64_t q_desc = descriptor(q_smem + t * C::OPERAND, 16), k_desc = descriptor(k_smem, 16), v_desc = descriptor(v_smem, C::PANEL);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         // By the tile's first thread: the scores of step `n`, whose keys are awaited.  What info holds of the step is visible behind its arrival.
         auto issue_scores = [&](uint32_t n) {
             const int stage = n % STAGES;
             if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
             fence_after();
-            const uint32_t qs = q_smem + t * C::OPERAND, ks = k_smem + stage * C::OPERAND;
+            const uint64_t ks = k_desc + uint64_t(stage) * (C::OPERAND >> 4);
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
-                mma_ss(tmem + C::S_COL + 128 * t, descriptor(qs + off, 16), descriptor(ks + off, 16), qk, k != 0);
+                const uint32_t off = ((k >> 2) * C::PANEL + (k & 3) * 32) >> 4;
+                mma_ss(tmem + C::S_COL + 128 * t, q_desc + off, ks + off, qk, k != 0);
             }
             commit(s_full(t));
             mbar_arrive(s_full(t));
@@ -478,20 +483,24 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                     return fmaxf(fmaxf(v[0], v[1]) * (c_row * f.k[col >> 4]), fmaxf(v[2], v[3]) * (c_row * f.k[(col >> 4) + 1]));
                 };
-                // ---- the row's largest score: columns 64..127, then 0..63, which stay in registers ----
-                uint32_t x[2][32];
-                float top = NEG_INF;
-#pragma unroll 1
-                for (int half = 64; half >= 0; half -= 64) {
-                    tmem_ld32(s_tmem + half, x[0]);
-                    tmem_ld32(s_tmem + half + 32, x[1]);
-                    wait_ld();
-                    if (masked) {
-                        hide(x[0], half);
-                        hide(x[1], half + 32);
-                    }
-                    top = fmaxf(top, fmaxf(largest(x[0], half), largest(x[1], half + 32)));
+                // ---- the row's largest score ----
+                uint32_t x[4][32];
+                tmem_ld32(s_tmem, x[0]);
+                tmem_ld32(s_tmem + 32, x[1]);
+                wait_ld();
+                tmem_ld32(s_tmem + 64, x[2]);
+                tmem_ld32(s_tmem + 96, x[3]);
+                if (masked) {
+                    hide(x[0], 0);
+                    hide(x[1], 32);
                 }
+                float top = fmaxf(largest(x[0], 0), largest(x[1], 32));
+                wait_ld();
+                if (masked) {
+                    hide(x[2], 64);
+                    hide(x[3], 96);
+                }
+                top = fmaxf(top, fmaxf(largest(x[2], 64), largest(x[3], 96)));
                 const float turn = f.turn;
                 const bool rise = top > m + LAG;
                 if (__any_sync(0xffffffffu, rise) || turn != 1.f) {
@@ -515,38 +524,25 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                 }
                 const float base_m = UP - (m == NEG_INF ? 0.f : m);
-                // ---- weights, over the scores that have been read ----
-#pragma unroll 1
-                for (int half = 0; half < KEYS; half += 64) {
-                    if (half) {
-                        tmem_ld32(s_tmem + half, x[0]);
-                        tmem_ld32(s_tmem + half + 32, x[1]);
-                        wait_ld();
-                        if (masked) {
-                            hide(x[0], half);
-                            hide(x[1], half + 32);
+                // ---- weights, into the scores' place ----
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float cg = c_row * f.k[2 * q + g], mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
+                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                            float y0, y1;
+                            unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
+                            y0 = exp2_approx(y0);
+                            y1 = exp2_approx(y1);
+                            l2 = fma2(pair(y0, y1), i2, l2);
+                            w[e / 2] = half2_bits(y0, y1);
                         }
                     }
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const int group16 = (half >> 4) + 2 * q + g;
-                            const float cg = c_row * f.k[group16], mg = base_m + f.v_log[group16], ig = f.v_inv[group16];
-                            const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
-#pragma unroll
-                            for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                                float y0, y1;
-                                unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
-                                y0 = exp2_approx(y0);
-                                y1 = exp2_approx(y1);
-                                l2 = fma2(pair(y0, y1), i2, l2);
-                                w[e / 2] = half2_bits(y0, y1);
-                            }
-                        }
-                        tmem_st16(s_tmem + half / 2 + 16 * q, w);
-                    }
+                    tmem_st16(s_tmem + 16 * q, w);
                 }
                 wait_st();
                 fence_before();
@@ -556,10 +552,10 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
                     if (ok) {
                         fence_after();
-                        const uint32_t vs = v_smem + stage * C::OPERAND;
+                        const uint64_t vs = v_desc + uint64_t(stage) * (C::OPERAND >> 4);
 #pragma unroll
                         for (int k = 0; k < KEYS / 16; ++k)
-                            mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, descriptor(vs + k * 2048, C::PANEL), pv, step != 0 || k != 0);
+                            mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, vs + k * (2048 >> 4), pv, step != 0 || k != 0);
                         commit(v_empty(stage));
                         if (step + 1 < p.steps) ok = issue_scores(n + 1);
                         else commit(o_full(t));
@@ -629,6 +625,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         }
     } else {
         // ===== codes into halfs: keys (warps 8-11) or values (12-15) =====
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         const bool is_v = warp >= 12;
         constexpr int PER_ROW = DP / 16, TURNS = KEYS * PER_ROW / 128, TURN_ROWS = 128 / PER_ROW;
         // sixteen codes, chunk ch of row r0 + TURN_ROWS * turn: eight lanes in a row are four chunks of an even and an odd row, whose halfs
