@@ -592,7 +592,7 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
     kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),
-               q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 4 == 0 && aligned_to(out, 8), static_cast<uint8_t *>(workspace), flag};
+               q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 8 == 0 && aligned_to(out, 16), static_cast<uint8_t *>(workspace), flag};
     cudaStream_t st = as_stream(stream);
     if (tiles) return kv::launch_tiles(dtype, cache->format, a, c, s, st);
 #define DX_CALL(T, FMT)                                                             \

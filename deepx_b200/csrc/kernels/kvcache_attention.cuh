@@ -14,7 +14,7 @@ struct Attn {
     int64_t q_stride, out_stride;
     int q_heads, group, window;
     float scale_log2;
-    int q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of out
+    int q_vec, out_vec;  // 16-byte loads of q and stores of out are possible
     uint8_t *ws;
     int32_t *flag;
 };

@@ -33,9 +33,6 @@ constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 128, GROUPS = KEYS / 16;
 constexpr int THREADS = 16 * 32;
 constexpr int STAGES = 2, INFO = 4;
 constexpr int OVERHEAD = 4;
-// Registers of a thread: a softmax thread holds a row's 128 scores at once.  The block is launched with 128 for every thread.
-constexpr int SOFTMAX_REGS = 184, CONVERT_REGS = 72;
-static_assert((SOFTMAX_REGS + CONVERT_REGS) * 256 <= THREADS * 128, "the split must fit what the block is launched with");
 constexpr int PLAN_CTA = 1024;
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
 enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
@@ -225,6 +222,11 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 // Two floats at a time.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t r;
@@ -262,6 +264,25 @@ struct Info {
     float turn, v_ref;
     int there;
 };
+
+// The products of a step, by one thread: all that depends on the tile and the stage is a constant, so that little stands between them.
+// `base`: the block's operands, Q of both tiles, then the stages of K, then those of V.
+template <int DP, int TILE, int STAGE> __device__ __forceinline__ void scores_of(uint32_t base) {
+    using C = Cfg<DP>;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
+        mma_ss(C::S_COL + 128 * TILE, descriptor(base + TILE * C::OPERAND + off, 16), descriptor(base + (2 + STAGE) * C::OPERAND + off, 16), instruction(KEYS, false), k != 0);
+    }
+}
+template <int DP, int TILE, int STAGE> __device__ __forceinline__ void output_of(uint32_t base, bool accumulate) {
+    using C = Cfg<DP>;
+#pragma unroll
+    for (int k = 0; k < KEYS / 16; ++k)
+        mma_ts(C::O_COL + DP * TILE, C::S_COL + 128 * TILE + 8 * k, descriptor(base + (2 + STAGES + STAGE) * C::OPERAND + k * 2048, C::PANEL), instruction(DP, true),
+               k != 0 || accumulate);
+}
+static_assert(STAGES == 2, "the stages of a product are written out");
 
 template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(Attn a, Cache c, Seqs s, Plan plan) {
     using C = Cfg<DP>;
@@ -309,7 +330,12 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot;
+    // The block has all 512 columns, so they begin at 0: written so, the products' addresses are constants of the code.
+    constexpr uint32_t tmem = 0;
+    if (tmem_slot != 0 && threadIdx.x == 0) {
+        abort_shared = 1;
+        atomicCAS(&g_status, 0, S_ROOM);
+    }
 
     // ---- this block's piece of the line ----
     Join *join = reinterpret_cast<Join *>(a.ws) + blockIdx.x;
@@ -353,20 +379,15 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         const uint32_t s_tmem = tmem + lanes + C::S_COL + 128 * t, o_tmem = tmem + lanes + C::O_COL + DP * t;
         uint32_t n = 0, n_s = 0, n_p = 0, n_q = 0, n_o = 0;  // steps of the block; phases of this tile's barriers
         bool ok = true;
-        constexpr uint32_t qk = instruction(KEYS, false), pv = instruction(DP, true);
-        const uint64_t q_desc = descriptor(q_smem + t * C::OPERAND, 16), k_desc = descriptor(k_smem, 16), v_desc = descriptor(v_smem, C::PANEL);
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         // By the tile's first thread: the scores of step `n`, whose keys are awaited.  What info holds of the step is visible behind its arrival.
         auto issue_scores = [&](uint32_t n) {
             const int stage = n % STAGES;
             if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
             fence_after();
-            const uint64_t ks = k_desc + uint64_t(stage) * (C::OPERAND >> 4);
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t off = ((k >> 2) * C::PANEL + (k & 3) * 32) >> 4;
-                mma_ss(tmem + C::S_COL + 128 * t, q_desc + off, ks + off, qk, k != 0);
-            }
+            if (t == 0 && stage == 0) scores_of<DP, 0, 0>(base);
+            else if (t == 0) scores_of<DP, 0, 1>(base);
+            else if (stage == 0) scores_of<DP, 1, 0>(base);
+            else scores_of<DP, 1, 1>(base);
             commit(s_full(t));
             mbar_arrive(s_full(t));
             commit(k_empty(stage));
@@ -401,42 +422,53 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             // ---- the row of Q as halfs into shared memory, a bfloat16 row divided by a power of two first ----
             float c_row = a.scale_log2;
             {
-                const T *q = static_cast<const T *>(a.q) + (p.it.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
-                uint4 x[DP / 8];
-                if (a.q_vec) {
+                // a warp's 32 rows come as whole lines, lanes side by side along a row, and pass through the rows' place in shared memory
+                constexpr int CHUNKS = DP / 8, AT_ONCE = 32 / CHUNKS;
+                const int64_t mine = (p.it.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+                const uint32_t rows_at = q_smem + t * C::OPERAND + (warp & 3) * (32 * 128);
+                const uint16_t *q = static_cast<const uint16_t *>(a.q);
+                const int ch = lane % CHUNKS;
+                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+                const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+                uint4 x[CHUNKS];
 #pragma unroll
-                    for (int k = 0; k < DP / 8; ++k) x[k] = live && k * 8 < c.dim ? *reinterpret_cast<const uint4 *>(q + k * 8) : make_uint4(0, 0, 0, 0);
-                } else {
+                for (int k = 0; k < CHUNKS; ++k) {
+                    const int row_k = k * AT_ONCE + lane / CHUNKS;
+                    const int64_t at_k = __shfl_sync(0xffffffffu, mine, row_k) + ch * 8;
+                    const bool in = (live_rows >> row_k & 1) && ch * 8 < c.dim;
+                    x[k] = make_uint4(0, 0, 0, 0);
+                    if (in && a.q_vec) x[k] = *reinterpret_cast<const uint4 *>(q + at_k);
+                    else if (in) {
+                        uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < DP / 8; ++k) {
-                        uint16_t h[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) h[e] = live && k * 8 < c.dim ? reinterpret_cast<const uint16_t *>(q)[k * 8 + e] : uint16_t(0);
-                        x[k] = make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16, h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
+                        for (int e = 0; e < 4; ++e) w[e] = q[at_k + 2 * e] | uint32_t(q[at_k + 2 * e + 1]) << 16;
+                        x[k] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
-                float down = 1.f;
+#pragma unroll
+                for (int k = 0; k < CHUNKS; ++k) sts128(place(k * AT_ONCE + lane / CHUNKS, ch), x[k].x, x[k].y, x[k].z, x[k].w);
+                __syncwarp();
                 if constexpr (std::is_same<T, bf16>::value) {
                     __nv_bfloat162 top2 = __float2bfloat162_rn(0.f);
 #pragma unroll
-                    for (int k = 0; k < DP / 8; ++k)
+                    for (int k = 0; k < CHUNKS; ++k) {
+                        x[k] = lds128(place(lane, k));
                         for (uint32_t w : {x[k].x, x[k].y, x[k].z, x[k].w}) top2 = __hmax2(top2, __habs2(*reinterpret_cast<__nv_bfloat162 *>(&w)));
+                    }
                     const float amax = fmaxf(to_compute(top2.x), to_compute(top2.y));
                     const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                    float down = 1.f;
                     if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
                         down = __uint_as_float((254u - e) << 23);
                         c_row *= __uint_as_float(e << 23);
                     }
-                }
-                const uint32_t dst = q_smem + t * C::OPERAND + r * 128;
 #pragma unroll
-                for (int k = 0; k < DP / 8; ++k) {
-                    uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-                    if constexpr (std::is_same<T, bf16>::value) {
+                    for (int k = 0; k < CHUNKS; ++k) {
+                        uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = half2_bits(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xFFFF0000u) * down);
+                        for (int d = 0; d < 4; ++d) w[d] = half2_bits(__uint_as_float(w[d] << 16) * down, __uint_as_float(w[d] & 0xFFFF0000u) * down);
+                        sts128(place(lane, k), w[0], w[1], w[2], w[3]);
                     }
-                    sts128(dst + (k >> 3) * C::PANEL + (((k & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
             }
             fence_async_smem();
@@ -444,7 +476,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             mbar_arrive(q_ready(t));
             if (r == 0) ok = mbar_wait(q_ready(t), n_q & 1, abort_flag, S_QUERIES) && issue_scores(n);
             ++n_q;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int tile_first = int(min(int64_t(p.it.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.it.end) - 1));  // least `last` of the tile
             const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
@@ -483,24 +515,20 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                     return fmaxf(fmaxf(v[0], v[1]) * (c_row * f.k[col >> 4]), fmaxf(v[2], v[3]) * (c_row * f.k[(col >> 4) + 1]));
                 };
-                // ---- the row's largest score ----
-                uint32_t x[4][32];
-                tmem_ld32(s_tmem, x[0]);
-                tmem_ld32(s_tmem + 32, x[1]);
-                wait_ld();
-                tmem_ld32(s_tmem + 64, x[2]);
-                tmem_ld32(s_tmem + 96, x[3]);
-                if (masked) {
-                    hide(x[0], 0);
-                    hide(x[1], 32);
+                // ---- the row's largest score: columns 64..127, then 0..63, which stay in registers ----
+                uint32_t x[2][32];
+                float top = NEG_INF;
+#pragma unroll 1
+                for (int half = 64; half >= 0; half -= 64) {
+                    tmem_ld32(s_tmem + half, x[0]);
+                    tmem_ld32(s_tmem + half + 32, x[1]);
+                    wait_ld();
+                    if (masked) {
+                        hide(x[0], half);
+                        hide(x[1], half + 32);
+                    }
+                    top = fmaxf(top, fmaxf(largest(x[0], half), largest(x[1], half + 32)));
                 }
-                float top = fmaxf(largest(x[0], 0), largest(x[1], 32));
-                wait_ld();
-                if (masked) {
-                    hide(x[2], 64);
-                    hide(x[3], 96);
-                }
-                top = fmaxf(top, fmaxf(largest(x[2], 64), largest(x[3], 96)));
                 const float turn = f.turn;
                 const bool rise = top > m + LAG;
                 if (__any_sync(0xffffffffu, rise) || turn != 1.f) {
@@ -524,25 +552,38 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                 }
                 const float base_m = UP - (m == NEG_INF ? 0.f : m);
-                // ---- weights, into the scores' place ----
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float cg = c_row * f.k[2 * q + g], mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
-                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
-#pragma unroll
-                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                            float y0, y1;
-                            unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
-                            y0 = exp2_approx(y0);
-                            y1 = exp2_approx(y1);
-                            l2 = fma2(pair(y0, y1), i2, l2);
-                            w[e / 2] = half2_bits(y0, y1);
+                // ---- weights, over the scores that have been read ----
+#pragma unroll 1
+                for (int half = 0; half < KEYS; half += 64) {
+                    if (half) {
+                        tmem_ld32(s_tmem + half, x[0]);
+                        tmem_ld32(s_tmem + half + 32, x[1]);
+                        wait_ld();
+                        if (masked) {
+                            hide(x[0], half);
+                            hide(x[1], half + 32);
                         }
                     }
-                    tmem_st16(s_tmem + 16 * q, w);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const int group16 = (half >> 4) + 2 * q + g;
+                            const float cg = c_row * f.k[group16], mg = base_m + f.v_log[group16], ig = f.v_inv[group16];
+                            const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                            for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                                float y0, y1;
+                                unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
+                                y0 = exp2_approx(y0);
+                                y1 = exp2_approx(y1);
+                                l2 = fma2(pair(y0, y1), i2, l2);
+                                w[e / 2] = half2_bits(y0, y1);
+                            }
+                        }
+                        tmem_st16(s_tmem + half / 2 + 16 * q, w);
+                    }
                 }
                 wait_st();
                 fence_before();
@@ -552,17 +593,17 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
                     if (ok) {
                         fence_after();
-                        const uint64_t vs = v_desc + uint64_t(stage) * (C::OPERAND >> 4);
-#pragma unroll
-                        for (int k = 0; k < KEYS / 16; ++k)
-                            mma_ts(tmem + C::O_COL + DP * t, tmem + C::S_COL + 128 * t + 8 * k, vs + k * (2048 >> 4), pv, step != 0 || k != 0);
+                        if (t == 0 && stage == 0) output_of<DP, 0, 0>(base, step != 0);
+                        else if (t == 0) output_of<DP, 0, 1>(base, step != 0);
+                        else if (stage == 0) output_of<DP, 1, 0>(base, step != 0);
+                        else output_of<DP, 1, 1>(base, step != 0);
                         commit(v_empty(stage));
                         if (step + 1 < p.steps) ok = issue_scores(n + 1);
                         else commit(o_full(t));
                     }
                 }
                 ++n_p;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
             }
             if (!ok) break;
@@ -575,40 +616,66 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             const float sum = l0 + l1, by = sum == 0.f ? 0.f : v_ref / sum;
             const bool whole = p.step0 == 0 && p.steps == p.it.steps;
             float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
-            T *out = static_cast<T *>(a.out) + (p.it.row0 + i) * a.out_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
-            if (!whole && live) {
-                part[ITEM_ROWS * DP + row] = m;
-                part[ITEM_ROWS * DP + ITEM_ROWS + row] = sum;
-            }
+            if (!whole) {
+                if (live) {
+                    part[ITEM_ROWS * DP + row] = m;
+                    part[ITEM_ROWS * DP + ITEM_ROWS + row] = sum;
+                }
 #pragma unroll 1
-            for (int d = 0; d < DP; d += 32) {
-                uint32_t x[32];
-                tmem_ld32(o_tmem + d, x);
-                wait_ld();
-                if (!live) continue;
+                for (int d = 0; d < DP; d += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(o_tmem + d, x);
+                    wait_ld();
+                    if (!live) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    if (d + e >= c.dim) break;
-                    float4 v;
-                    // a row that has seen nothing has multiplied nothing but zeros
-                    v.x = __uint_as_float(x[e]) * by;
-                    v.y = __uint_as_float(x[e + 1]) * by;
-                    v.z = __uint_as_float(x[e + 2]) * by;
-                    v.w = __uint_as_float(x[e + 3]) * by;
-                    if (!whole) *reinterpret_cast<float4 *>(part + row * DP + d + e) = v;
-                    else {
-                        Pack<T, 4> y;
-                        y.v[0] = from_compute<T>(v.x);
-                        y.v[1] = from_compute<T>(v.y);
-                        y.v[2] = from_compute<T>(v.z);
-                        y.v[3] = from_compute<T>(v.w);
-                        if (a.out_vec) st_stream<T, 4>(out + d + e, y);
-                        else {
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(part + row * DP + d + e) = make_float4(__uint_as_float(x[e]) * by, __uint_as_float(x[e + 1]) * by,
+                                                                                          __uint_as_float(x[e + 2]) * by, __uint_as_float(x[e + 3]) * by);
+                }
+            } else {
+                // through the place of the warp's rows of Q, which all products have read, and out as whole lines
+                constexpr int CHUNKS = DP / 8, AT_ONCE = 32 / CHUNKS;
+                const uint32_t rows_at = q_smem + t * C::OPERAND + (warp & 3) * (32 * 128);
+                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+#pragma unroll 1
+                for (int d = 0; d < DP; d += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(o_tmem + d, x);
+                    wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) out[d + e + k] = y.v[k];
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float lo = __uint_as_float(x[e + 2 * k]) * by, hi = __uint_as_float(x[e + 2 * k + 1]) * by;
+                            if constexpr (std::is_same<T, f16>::value) w[k] = half2_bits(lo, hi);
+                            else {
+                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
+                                w[k] = *reinterpret_cast<const uint32_t *>(&b2);
+                            }
                         }
+                        sts128(place(lane, (d + e) >> 3), w[0], w[1], w[2], w[3]);
                     }
                 }
+                __syncwarp();
+                const int64_t mine = (p.it.row0 + i) * a.out_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+                uint16_t *out = static_cast<uint16_t *>(a.out);
+                const int ch = lane % CHUNKS;
+                const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+#pragma unroll 4
+                for (int k = 0; k < CHUNKS; ++k) {
+                    const int row_k = k * AT_ONCE + lane / CHUNKS;
+                    const int64_t at_k = __shfl_sync(0xffffffffu, mine, row_k) + ch * 8;
+                    const uint4 v = lds128(place(row_k, ch));
+                    if (!(live_rows >> row_k & 1) || ch * 8 >= c.dim) continue;
+                    if (a.out_vec) __stcs(reinterpret_cast<uint4 *>(out + at_k), v);
+                    else {
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) out[at_k + e] = uint16_t(w[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+                __syncwarp();  // the rows are the next item's
             }
             // the item's first steps are the block before's: here is where it is joined
             if (threadIdx.x == 0 && starts_here && p.step0 > 0 && total * (int64_t(blockIdx.x) - 1) / blocks - p.item_begin <= OVERHEAD) {
@@ -625,7 +692,6 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         }
     } else {
         // ===== codes into halfs: keys (warps 8-11) or values (12-15) =====
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         const bool is_v = warp >= 12;
         constexpr int PER_ROW = DP / 16, TURNS = KEYS * PER_ROW / 128, TURN_ROWS = 128 / PER_ROW;
         // sixteen codes, chunk ch of row r0 + TURN_ROWS * turn: eight lanes in a row are four chunks of an even and an odd row, whose halfs
