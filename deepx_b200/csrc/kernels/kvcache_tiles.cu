@@ -179,6 +179,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int where) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where));
 }
+// One thread of the warp, known to be one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -265,24 +271,24 @@ struct Info {
     int there;
 };
 
-// The products of a step, by one thread: all that depends on the tile and the stage is a constant, so that little stands between them.
-// `base`: the block's operands, Q of both tiles, then the stages of K, then those of V.
-template <int DP, int TILE, int STAGE> __device__ __forceinline__ void scores_of(uint32_t base) {
+// The products of a step, by one thread.  `base`: the block's operands, Q of both tiles, then the stages of K, then those of V.
+template <int DP> __device__ __forceinline__ void scores_of(uint32_t base, int tile, int stage) {
     using C = Cfg<DP>;
+    const uint64_t q = descriptor(base + tile * C::OPERAND, 16), k = descriptor(base + (2 + stage) * C::OPERAND, 16);
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
-        mma_ss(C::S_COL + 128 * TILE, descriptor(base + TILE * C::OPERAND + off, 16), descriptor(base + (2 + STAGE) * C::OPERAND + off, 16), instruction(KEYS, false), k != 0);
+    for (int i = 0; i < DP / 16; ++i) {
+        const uint32_t off = ((i >> 2) * C::PANEL + (i & 3) * 32) >> 4;
+        mma_ss(C::S_COL + 128 * tile, q + off, k + off, instruction(KEYS, false), i != 0);
     }
 }
-template <int DP, int TILE, int STAGE> __device__ __forceinline__ void output_of(uint32_t base, bool accumulate) {
+template <int DP> __device__ __forceinline__ void output_of(uint32_t base, int tile, int stage, bool accumulate) {
     using C = Cfg<DP>;
+    const uint64_t v = descriptor(base + (2 + STAGES + stage) * C::OPERAND, C::PANEL);
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k)
-        mma_ts(C::O_COL + DP * TILE, C::S_COL + 128 * TILE + 8 * k, descriptor(base + (2 + STAGES + STAGE) * C::OPERAND + k * 2048, C::PANEL), instruction(DP, true),
-               k != 0 || accumulate);
+    for (int i = 0; i < KEYS / 16; ++i)
+        mma_ts(C::O_COL + DP * tile, C::S_COL + 128 * tile + 8 * i, v + i * (2048 >> 4), instruction(DP, true), i != 0 || accumulate);
 }
-static_assert(STAGES == 2, "the stages of a product are written out");
+static_assert(STAGES == 2, "the next stage is the other one");
 
 template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(Attn a, Cache c, Seqs s, Plan plan) {
     using C = Cfg<DP>;
@@ -293,7 +299,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     __shared__ int abort_shared;
     __shared__ int found_group;
     volatile int *abort_flag = &abort_shared;
-    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t base = __shfl_sync(0xffffffffu, (smem_u32(raw) + 1023u) & ~1023u, 0);
     const uint32_t q_smem = base, k_smem = base + 2 * C::OPERAND, v_smem = k_smem + STAGES * C::OPERAND;
     const uint32_t bar0 = smem_u32(bars);
     auto k_full = [&](int i) { return bar0 + 8u * i; };
@@ -304,7 +310,8 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     auto p_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 2 + t); };
     auto q_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 4 + t); };
     auto o_full = [&](int t) { return bar0 + 8u * (4 * STAGES + 6 + t); };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the same in all threads of a warp, and known to be: what the tensor cores are told is worked out in uniform registers
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -380,14 +387,11 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         uint32_t n = 0, n_s = 0, n_p = 0, n_q = 0, n_o = 0;  // steps of the block; phases of this tile's barriers
         bool ok = true;
         // By the tile's first thread: the scores of step `n`, whose keys are awaited.  What info holds of the step is visible behind its arrival.
-        auto issue_scores = [&](uint32_t n) {
-            const int stage = n % STAGES;
+        const bool first_warp = (warp & 3) == 0;
+        auto issue_scores = [&](uint32_t n, int stage) {
             if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
             fence_after();
-            if (t == 0 && stage == 0) scores_of<DP, 0, 0>(base);
-            else if (t == 0) scores_of<DP, 0, 1>(base);
-            else if (stage == 0) scores_of<DP, 1, 0>(base);
-            else scores_of<DP, 1, 1>(base);
+            scores_of<DP>(base, t, stage);
             commit(s_full(t));
             mbar_arrive(s_full(t));
             commit(k_empty(stage));
@@ -474,7 +478,10 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             fence_async_smem();
             fence_before();  // the reads of O of the item before
             mbar_arrive(q_ready(t));
-            if (r == 0) ok = mbar_wait(q_ready(t), n_q & 1, abort_flag, S_QUERIES) && issue_scores(n);
+            if (first_warp) {
+                const int stage = __shfl_sync(0xffffffffu, int(n % STAGES), 0);
+                if (elect_one()) ok = mbar_wait(q_ready(t), n_q & 1, abort_flag, S_QUERIES) && issue_scores(n, stage);
+            }
             ++n_q;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -482,7 +489,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
 
             float m = NEG_INF, v_ref = 1.f;
-            uint64_t l2 = pair(0.f, 0.f);
+            uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             for (int step = 0; step < p.steps; ++step, ++n) {
                 const int j0 = p.it.lo + (p.step0 + step) * KEYS;
                 if (!warp_wait(s_full(t), n_s & 1, abort_flag, S_SCORES)) { ok = false; break; }
@@ -535,9 +542,8 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     const float to = rise ? top : m;
                     float by = to == m ? 1.f : exp2_approx(m - to);
                     m = to;
-                    float l0, l1;
-                    unpair(l2, l0, l1);
-                    l2 = pair(l0 * by, l1 * by);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) l2[e] = fma2(l2[e], pair(by, by), pair(0.f, 0.f));
                     by *= turn;
                     if (step > 0) {  // the products of the step before are complete: these scores were issued behind them
 #pragma unroll 1
@@ -578,7 +584,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                                 unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
                                 y0 = exp2_approx(y0);
                                 y1 = exp2_approx(y1);
-                                l2 = fma2(pair(y0, y1), i2, l2);
+                                l2[(e >> 1) & 1] = fma2(pair(y0, y1), i2, l2[(e >> 1) & 1]);
                                 w[e / 2] = half2_bits(y0, y1);
                             }
                         }
@@ -588,18 +594,17 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 wait_st();
                 fence_before();
                 mbar_arrive(p_ready(t));
-                if (r == 0) {
-                    const int stage = n % STAGES;
-                    ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
-                    if (ok) {
-                        fence_after();
-                        if (t == 0 && stage == 0) output_of<DP, 0, 0>(base, step != 0);
-                        else if (t == 0) output_of<DP, 0, 1>(base, step != 0);
-                        else if (stage == 0) output_of<DP, 1, 0>(base, step != 0);
-                        else output_of<DP, 1, 1>(base, step != 0);
-                        commit(v_empty(stage));
-                        if (step + 1 < p.steps) ok = issue_scores(n + 1);
-                        else commit(o_full(t));
+                if (first_warp) {
+                    const int stage = __shfl_sync(0xffffffffu, int(n % STAGES), 0);
+                    if (elect_one()) {
+                        ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
+                        if (ok) {
+                            fence_after();
+                            output_of<DP>(base, t, stage, step != 0);
+                            commit(v_empty(stage));
+                            if (step + 1 < p.steps) ok = issue_scores(n + 1, stage ^ 1);
+                            else commit(o_full(t));
+                        }
                     }
                 }
                 ++n_p;
@@ -611,9 +616,10 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             if (!warp_wait(o_full(t), n_o & 1, abort_flag, S_OUTPUT)) { ok = false; break; }
             ++n_o;
             fence_after();
-            float l0, l1;
-            unpair(l2, l0, l1);
-            const float sum = l0 + l1, by = sum == 0.f ? 0.f : v_ref / sum;
+            float l0, l1, l3, l4;
+            unpair(l2[0], l0, l1);
+            unpair(l2[1], l3, l4);
+            const float sum = (l0 + l1) + (l3 + l4), by = sum == 0.f ? 0.f : v_ref / sum;
             const bool whole = p.step0 == 0 && p.steps == p.it.steps;
             float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
             if (!whole) {
