@@ -1,20 +1,19 @@
 // dx_kvcache_attention for prompts: tiles of 128 rows on tcgen05 tensor cores.
 //
-// An item is up to 256 rows (new token i, head of the key head's group: i * group + g, flattened) of one sequence and key head: two
-// tiles of 128 rows that take turns, so that the tensor cores work on one while the other's exponentials are computed.  For each step
-// of 128 keys:
-//     S = Q K^T          128 x 128, into TMEM;                                Q, K halfs in shared memory
-//     P = 2^(c S - m)    a thread has a row; halfs, over S's place in TMEM
-//     O = O + P V        128 x dim, in TMEM, P from TMEM;                     V halfs in shared memory
-// Four exponentials' worth of tensor work (512 multiply-adds) goes with each exponential at 128 dimensions: a step of both tiles costs
-// 2048 cycles of the tensor cores and 2048 of the exponential unit, so both bound this kernel; what is neither stays off their threads.
+// An item is up to 256 rows (new token i, head of the key head's group: i * group + g, flattened) of one sequence and key head, two
+// tiles of 128 rows.  For each step of 64 keys and each tile:
+//     S = Q K^T          128 x 64, into one of the tile's two places in TMEM;  Q, K halfs in shared memory
+//     P = 2^(c S - m)    a thread has a row; halfs, over S's place
+//     O = O + P V        128 x dim, in TMEM, P from TMEM;                      V halfs in shared memory
+// The scores are issued two steps ahead, so a tile's softmax finds the next ones ready when it is done with the last: with one place
+// for them it waited a third of the time.  512 multiply-adds go with each exponential at 128 dimensions: 64 keys of both tiles cost 1024
+// cycles of the tensor cores and 1024 of the exponential unit, so both bound this kernel; what is neither stays off their threads.
 //
-// Roles (16 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each, and the first thread of each issues its tile's
-// products (its P V, and behind it the scores of the next step, the moment its weights are there); 8-11 turn the codes of K into halfs,
-// 12-15 those of V (sixteen a thread and turn, loaded a step ahead).  Codes become halfs unscaled and exact; the scales of a step's
-// eight groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of the largest so far) into the
-// exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is scaled again (in TMEM, by the
-// row's thread), which after the first steps hardly happens.
+// Roles (16 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each; 8-10 turn the codes of K into halfs, 11-13 those of V
+// (sixteen a thread and turn, loaded a step ahead); a thread of warp 14 and one of 15 issue a tile's products each.  Codes become halfs
+// unscaled and exact; the scales of a step's groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of
+// the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
+// scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
 //
 // The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it, where an
 // item counts OVERHEAD steps more than it has (its queries, its way out; without that the blocks of a prompt's first rows, whose items
@@ -29,10 +28,13 @@ namespace dx {
 namespace kv {
 namespace {
 
-constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 128, GROUPS = KEYS / 16;
+constexpr int TILE_ROWS = 128, ITEM_ROWS = 256, KEYS = 64, GROUPS = KEYS / 16;
 constexpr int THREADS = 16 * 32;
-constexpr int STAGES = 2, INFO = 4;
-constexpr int OVERHEAD = 4;
+// Info of a step outlives its keys: its place is written again when the scores of four steps later are complete, which were issued
+// behind the weights of two steps later.
+constexpr int STAGES = 4, INFO = 8;
+constexpr int CONVERTERS = 3;  // warps for K, and for V
+constexpr int OVERHEAD = 6;
 constexpr int PLAN_CTA = 1024;
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
 enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
@@ -256,11 +258,13 @@ __host__ __device__ constexpr uint32_t instruction(int n, bool b_by_k) {
 }
 
 template <int DP> struct Cfg {
-    static constexpr int PANELS = DP / 64, PANEL = 128 * 128;  // 128 rows of 64 halfs
-    static constexpr int OPERAND = PANELS * PANEL;             // Q of a tile, K or V of a step
-    static constexpr int SMEM = (2 + 2 * STAGES) * OPERAND + 1024;
+    static constexpr int PANELS = DP / 64;  // of 64 halfs a row: 128 bytes
+    static constexpr int Q_PANEL = TILE_ROWS * 128, Q_TILE = PANELS * Q_PANEL;
+    static constexpr int PANEL = KEYS * 128, OPERAND = PANELS * PANEL;  // K or V of a step
+    static constexpr int SMEM = 2 * Q_TILE + 2 * STAGES * OPERAND + 1024;
     static constexpr int PART = ITEM_ROWS * DP + 2 * ITEM_ROWS;
-    static constexpr int S_COL = 0, O_COL = 256;  // TMEM columns of tile t: S_COL + 128 t, O_COL + DP t
+    // TMEM columns of tile t: scores of step n at 128 t + 64 (n % 2), O at O_COL + DP t
+    static constexpr int O_COL = 256;
 };
 
 // What the softmax needs of a step: for each group of sixteen tokens K's scale, log2 of V's in units of the largest so far and its
@@ -272,56 +276,53 @@ struct Info {
 };
 
 // The products of a step, by one thread.  `base`: the block's operands, Q of both tiles, then the stages of K, then those of V.
-template <int DP> __device__ __forceinline__ void scores_of(uint32_t base, int tile, int stage) {
+template <int DP> __device__ __forceinline__ void scores_of(uint32_t base, int tile, int place, int stage) {
     using C = Cfg<DP>;
-    const uint64_t q = descriptor(base + tile * C::OPERAND, 16), k = descriptor(base + (2 + stage) * C::OPERAND, 16);
+    const uint64_t q = descriptor(base + tile * C::Q_TILE, 16), k = descriptor(base + 2 * C::Q_TILE + stage * C::OPERAND, 16);
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-        const uint32_t off = ((i >> 2) * C::PANEL + (i & 3) * 32) >> 4;
-        mma_ss(C::S_COL + 128 * tile, q + off, k + off, instruction(KEYS, false), i != 0);
-    }
+    for (int i = 0; i < DP / 16; ++i)
+        mma_ss(128 * tile + 64 * place, q + (((i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4), k + (((i >> 2) * C::PANEL + (i & 3) * 32) >> 4), instruction(KEYS, false), i != 0);
 }
-template <int DP> __device__ __forceinline__ void output_of(uint32_t base, int tile, int stage, bool accumulate) {
+template <int DP> __device__ __forceinline__ void output_of(uint32_t base, int tile, int place, int stage, bool accumulate) {
     using C = Cfg<DP>;
-    const uint64_t v = descriptor(base + (2 + STAGES + stage) * C::OPERAND, C::PANEL);
+    const uint64_t v = descriptor(base + 2 * C::Q_TILE + (STAGES + stage) * C::OPERAND, C::PANEL);
 #pragma unroll
     for (int i = 0; i < KEYS / 16; ++i)
-        mma_ts(C::O_COL + DP * tile, C::S_COL + 128 * tile + 8 * i, v + i * (2048 >> 4), instruction(DP, true), i != 0 || accumulate);
+        mma_ts(C::O_COL + DP * tile, 128 * tile + 64 * place + 8 * i, v + i * (2048 >> 4), instruction(DP, true), i != 0 || accumulate);
 }
-static_assert(STAGES == 2, "the next stage is the other one");
 
 template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(Attn a, Cache c, Seqs s, Plan plan) {
     using C = Cfg<DP>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t bars[2 * STAGES * 2 + 4 * 2];
+    __shared__ uint64_t bars[4 * STAGES + 12];
     __shared__ Info info[INFO];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_shared;
     __shared__ int found_group;
     volatile int *abort_flag = &abort_shared;
     const uint32_t base = __shfl_sync(0xffffffffu, (smem_u32(raw) + 1023u) & ~1023u, 0);
-    const uint32_t q_smem = base, k_smem = base + 2 * C::OPERAND, v_smem = k_smem + STAGES * C::OPERAND;
+    const uint32_t q_smem = base, k_smem = base + 2 * C::Q_TILE, v_smem = k_smem + STAGES * C::OPERAND;
     const uint32_t bar0 = smem_u32(bars);
     auto k_full = [&](int i) { return bar0 + 8u * i; };
     auto k_empty = [&](int i) { return bar0 + 8u * (STAGES + i); };
     auto v_full = [&](int i) { return bar0 + 8u * (2 * STAGES + i); };
     auto v_empty = [&](int i) { return bar0 + 8u * (3 * STAGES + i); };
-    auto s_full = [&](int t) { return bar0 + 8u * (4 * STAGES + t); };
-    auto p_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 2 + t); };
-    auto q_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 4 + t); };
-    auto o_full = [&](int t) { return bar0 + 8u * (4 * STAGES + 6 + t); };
+    auto s_full = [&](int t, int place) { return bar0 + 8u * (4 * STAGES + 2 * t + place); };
+    auto p_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 4 + t); };
+    auto q_ready = [&](int t) { return bar0 + 8u * (4 * STAGES + 6 + t); };
+    auto o_full = [&](int t) { return bar0 + 8u * (4 * STAGES + 8 + t); };
     // the same in all threads of a warp, and known to be: what the tensor cores are told is worked out in uniform registers
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(k_full(i), 128);
+            mbar_init(k_full(i), 32 * CONVERTERS);
             mbar_init(k_empty(i), 2);  // one arrival for each tile
-            mbar_init(v_full(i), 128);
+            mbar_init(v_full(i), 32 * CONVERTERS);
             mbar_init(v_empty(i), 2);
         }
         for (int t = 0; t < 2; ++t) {
-            mbar_init(s_full(t), 2);  // the products' completion, and the issuing thread's own arrival, behind which info is visible
+            for (int i = 0; i < 2; ++i) mbar_init(s_full(t, i), 2);  // the products' completion, and the issuing thread's own arrival, behind which info is visible
             mbar_init(p_ready(t), 128);
             mbar_init(q_ready(t), 128);
             mbar_init(o_full(t), 1);
@@ -349,7 +350,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
     const int groups = *plan.count;
     const int64_t total = plan.before[groups];
-    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / (OVERHEAD + 2)));
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / (OVERHEAD + 4)));
     const bool work = total > 0 && int64_t(blockIdx.x) < blocks;
     const int64_t begin = work ? total * blockIdx.x / blocks : 0, end = work ? total * (blockIdx.x + 1) / blocks : 0;
     if (threadIdx.x == 0) join->parts = 0;
@@ -383,39 +384,16 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
         // ===== softmax of tile t: this thread has one row =====
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = uint32_t(warp & 3) * 32u << 16;
-        const uint32_t s_tmem = tmem + lanes + C::S_COL + 128 * t, o_tmem = tmem + lanes + C::O_COL + DP * t;
-        uint32_t n = 0, n_s = 0, n_p = 0, n_q = 0, n_o = 0;  // steps of the block; phases of this tile's barriers
+        const uint32_t s_tmem = tmem + lanes + 128 * t, o_tmem = tmem + lanes + C::O_COL + DP * t;
+        uint32_t n = 0, n_s = 0;  // steps of the block; those of this tile, whose barriers' phases they count
         bool ok = true;
-        // By the tile's first thread: the scores of step `n`, whose keys are awaited.  What info holds of the step is visible behind its arrival.
-        const bool first_warp = (warp & 3) == 0;
-        auto issue_scores = [&](uint32_t n, int stage) {
-            if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
-            fence_after();
-            scores_of<DP>(base, t, stage);
-            commit(s_full(t));
-            mbar_arrive(s_full(t));
-            commit(k_empty(stage));
-            return true;
-        };
         for (int64_t at = begin; at < end && ok;) {
             const Piece p = piece_at(at);
             const bool starts_here = at == begin;
             at = p.next;
             if (p.steps == 0) continue;
             if (t >= p.tiles) {
-                // No rows: the tile's arrivals all the same, step by step, so that its waits never fall behind or run ahead by a phase.
-                if (r == 0) {
-                    for (int step = 0; step < p.steps && ok; ++step) {
-                        const int stage = (n + step) % STAGES;
-                        const uint32_t full = ((n + step) / STAGES) & 1;
-                        ok = mbar_wait(k_full(stage), full, abort_flag, S_KEYS);
-                        mbar_arrive(k_empty(stage));
-                        ok = ok && mbar_wait(v_full(stage), full, abort_flag, S_VALUES);
-                        mbar_arrive(v_empty(stage));
-                    }
-                }
                 n += p.steps;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
                 continue;
             }
             const int row = t * TILE_ROWS + r;
@@ -429,10 +407,10 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 // a warp's 32 rows come as whole lines, lanes side by side along a row, and pass through the rows' place in shared memory
                 constexpr int CHUNKS = DP / 8, AT_ONCE = 32 / CHUNKS;
                 const int64_t mine = (p.it.row0 + i) * a.q_stride + int64_t(p.head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
-                const uint32_t rows_at = q_smem + t * C::OPERAND + (warp & 3) * (32 * 128);
+                const uint32_t rows_at = q_smem + t * C::Q_TILE + (warp & 3) * (32 * 128);
                 const uint16_t *q = static_cast<const uint16_t *>(a.q);
                 const int ch = lane % CHUNKS;
-                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::Q_PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
                 const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
                 uint4 x[CHUNKS];
 #pragma unroll
@@ -478,22 +456,15 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             fence_async_smem();
             fence_before();  // the reads of O of the item before
             mbar_arrive(q_ready(t));
-            if (first_warp) {
-                const int stage = __shfl_sync(0xffffffffu, int(n % STAGES), 0);
-                if (elect_one()) ok = mbar_wait(q_ready(t), n_q & 1, abort_flag, S_QUERIES) && issue_scores(n, stage);
-            }
-            ++n_q;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
             const int tile_first = int(min(int64_t(p.it.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.it.end) - 1));  // least `last` of the tile
             const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
 
             float m = NEG_INF, v_ref = 1.f;
             uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-            for (int step = 0; step < p.steps; ++step, ++n) {
-                const int j0 = p.it.lo + (p.step0 + step) * KEYS;
-                if (!warp_wait(s_full(t), n_s & 1, abort_flag, S_SCORES)) { ok = false; break; }
-                ++n_s;
+            for (int step = 0; step < p.steps; ++step, ++n, ++n_s) {
+                const int j0 = p.it.lo + (p.step0 + step) * KEYS, place = n_s & 1;
+                const uint32_t here = s_tmem + 64 * place;
+                if (!warp_wait(s_full(t, place), (n_s >> 1) & 1, abort_flag, S_SCORES)) { ok = false; break; }
                 fence_after();
                 const Info &f = info[n % INFO];
                 const int there = f.there;
@@ -522,21 +493,18 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     }
                     return fmaxf(fmaxf(v[0], v[1]) * (c_row * f.k[col >> 4]), fmaxf(v[2], v[3]) * (c_row * f.k[(col >> 4) + 1]));
                 };
-                // ---- the row's largest score: columns 64..127, then 0..63, which stay in registers ----
+                // ---- the row's largest score ----
                 uint32_t x[2][32];
-                float top = NEG_INF;
-#pragma unroll 1
-                for (int half = 64; half >= 0; half -= 64) {
-                    tmem_ld32(s_tmem + half, x[0]);
-                    tmem_ld32(s_tmem + half + 32, x[1]);
-                    wait_ld();
-                    if (masked) {
-                        hide(x[0], half);
-                        hide(x[1], half + 32);
-                    }
-                    top = fmaxf(top, fmaxf(largest(x[0], half), largest(x[1], half + 32)));
+                tmem_ld32(here, x[0]);
+                tmem_ld32(here + 32, x[1]);
+                wait_ld();
+                if (masked) {
+                    hide(x[0], 0);
+                    hide(x[1], 32);
                 }
+                const float top = fmaxf(largest(x[0], 0), largest(x[1], 32));
                 const float turn = f.turn;
+                bool o_known = step == 0;
                 const bool rise = top > m + LAG;
                 if (__any_sync(0xffffffffu, rise) || turn != 1.f) {
                     const float to = rise ? top : m;
@@ -545,7 +513,10 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
 #pragma unroll
                     for (int e = 0; e < 2; ++e) l2[e] = fma2(l2[e], pair(by, by), pair(0.f, 0.f));
                     by *= turn;
-                    if (step > 0) {  // the products of the step before are complete: these scores were issued behind them
+                    if (step > 0) {
+                        if (!warp_wait(o_full(t), (n_s - 1) & 1, abort_flag, S_OUTPUT)) { ok = false; break; }  // the product of the step before
+                        fence_after();
+                        o_known = true;
 #pragma unroll 1
                         for (int d = 0; d < DP; d += 16) {
                             uint32_t y[16];
@@ -559,62 +530,35 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 }
                 const float base_m = UP - (m == NEG_INF ? 0.f : m);
                 // ---- weights, over the scores that have been read ----
-#pragma unroll 1
-                for (int half = 0; half < KEYS; half += 64) {
-                    if (half) {
-                        tmem_ld32(s_tmem + half, x[0]);
-                        tmem_ld32(s_tmem + half + 32, x[1]);
-                        wait_ld();
-                        if (masked) {
-                            hide(x[0], half);
-                            hide(x[1], half + 32);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float cg = c_row * f.k[2 * q + g], mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
+                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                            float y0, y1;
+                            unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
+                            y0 = exp2_approx(y0);
+                            y1 = exp2_approx(y1);
+                            l2[(e >> 1) & 1] = fma2(pair(y0, y1), i2, l2[(e >> 1) & 1]);
+                            w[e / 2] = half2_bits(y0, y1);
                         }
                     }
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const int group16 = (half >> 4) + 2 * q + g;
-                            const float cg = c_row * f.k[group16], mg = base_m + f.v_log[group16], ig = f.v_inv[group16];
-                            const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
-#pragma unroll
-                            for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                                float y0, y1;
-                                unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
-                                y0 = exp2_approx(y0);
-                                y1 = exp2_approx(y1);
-                                l2[(e >> 1) & 1] = fma2(pair(y0, y1), i2, l2[(e >> 1) & 1]);
-                                w[e / 2] = half2_bits(y0, y1);
-                            }
-                        }
-                        tmem_st16(s_tmem + half / 2 + 16 * q, w);
-                    }
+                    tmem_st16(here + 16 * q, w);
                 }
                 wait_st();
+                // Each step sees the product of the step before complete, before it lets its own begin: so no wait on this barrier is two of
+                // its phases away.
+                if (!o_known && !warp_wait(o_full(t), (n_s - 1) & 1, abort_flag, S_OUTPUT)) { ok = false; break; }
                 fence_before();
                 mbar_arrive(p_ready(t));
-                if (first_warp) {
-                    const int stage = __shfl_sync(0xffffffffu, int(n % STAGES), 0);
-                    if (elect_one()) {
-                        ok = mbar_wait(p_ready(t), n_p & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
-                        if (ok) {
-                            fence_after();
-                            output_of<DP>(base, t, stage, step != 0);
-                            commit(v_empty(stage));
-                            if (step + 1 < p.steps) ok = issue_scores(n + 1, stage ^ 1);
-                            else commit(o_full(t));
-                        }
-                    }
-                }
-                ++n_p;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
             }
             if (!ok) break;
             // ---- the way out ----
-            if (!warp_wait(o_full(t), n_o & 1, abort_flag, S_OUTPUT)) { ok = false; break; }
-            ++n_o;
+            if (!warp_wait(o_full(t), (n_s - 1) & 1, abort_flag, S_OUTPUT)) { ok = false; break; }  // the product of the last step
             fence_after();
             float l0, l1, l3, l4;
             unpair(l2[0], l0, l1);
@@ -641,8 +585,8 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             } else {
                 // through the place of the warp's rows of Q, which all products have read, and out as whole lines
                 constexpr int CHUNKS = DP / 8, AT_ONCE = 32 / CHUNKS;
-                const uint32_t rows_at = q_smem + t * C::OPERAND + (warp & 3) * (32 * 128);
-                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
+                const uint32_t rows_at = q_smem + t * C::Q_TILE + (warp & 3) * (32 * 128);
+                auto place = [&](int row, int chunk) { return rows_at + (chunk >> 3) * C::Q_PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
 #pragma unroll 1
                 for (int d = 0; d < DP; d += 32) {
                     uint32_t x[32];
@@ -692,52 +636,48 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 join->parts = int(((p.item_begin + p.it.steps + OVERHEAD) * blocks - 1) / total) - int(blockIdx.x) + 2;
             }
         }
-        if (*abort_flag && r == 0) {  // products in flight: time to end before their memory is given back
-            const long long t0 = clock64();
-            while (clock64() - t0 < 2000000ll) {}
-        }
-    } else {
-        // ===== codes into halfs: keys (warps 8-11) or values (12-15) =====
-        const bool is_v = warp >= 12;
-        constexpr int PER_ROW = DP / 16, TURNS = KEYS * PER_ROW / 128, TURN_ROWS = 128 / PER_ROW;
-        // sixteen codes, chunk ch of row r0 + TURN_ROWS * turn: eight lanes in a row are four chunks of an even and an odd row, whose halfs
-        // go to different banks
+    } else if (warp < 8 + 2 * CONVERTERS) {
+        // ===== codes into halfs: keys or values =====
+        const bool is_v = warp >= 8 + CONVERTERS;
+        const int sub = (warp - 8) % CONVERTERS;
+        constexpr int PER_ROW = DP / 16, WARP_ROWS = 32 / PER_ROW, UNITS = KEYS / WARP_ROWS, TURNS = (UNITS + CONVERTERS - 1) / CONVERTERS;
+        // In turn i the warp takes rows WARP_ROWS * (sub + CONVERTERS * i)..., a thread sixteen codes, chunk ch of one row: eight lanes in a row are
+        // four chunks of an even and an odd row, whose halfs go to different banks.
         const int ch = DP == 64 ? lane & 3 : (lane & 3) | (lane >> 3 & 1) << 2;
-        const int r0 = (warp & 3) * (TURN_ROWS / 4) + (DP == 64 ? lane >> 2 : (lane >> 2 & 1) | lane >> 4 << 1);
+        const int r0 = DP == 64 ? lane >> 2 : (lane >> 2 & 1) | lane >> 4 << 1;
         const bool in_dim = ch * 16 < c.dim;
-        const uint8_t *codes = (is_v ? c.v : c.k) + (r0 & 15) * c.dim + ch * 16;
-        const uint32_t smem = (is_v ? v_smem : k_smem) + (ch >> 2) * C::PANEL + r0 * 128;
-        const int at0 = ((ch & 3) * 2 ^ (r0 & 7)) << 4, at1 = at0 ^ 16;
+        const uint8_t *codes = (is_v ? c.v : c.k) + ch * 16;
+        const uint32_t smem = (is_v ? v_smem : k_smem) + (ch >> 2) * C::PANEL;
         uint32_t n = 0;
         bool ok = true;
         for (int64_t at = begin; at < end && ok;) {
             const Piece p = piece_at(at);
             at = p.next;
             if (p.steps == 0) continue;
-            // lane g of a warp knows group g of a step: its page, and where its codes begin (-1: nowhere)
+            // lane g of a warp (mod GROUPS) knows group g of a step: its page, and where its codes begin (-1: nowhere)
             const int32_t *table = s.table + int64_t(p.it.b) * s.cols;
             auto page_of = [&](int step) {
-                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
+                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
                 int32_t number = -1;
                 if (step < p.steps && j < p.it.hi) {
                     number = table[j >> c.page_shift];
                     if (number < 0 || number >= c.pages) {
-                        if (warp == 8 && lane < 8) raise(a.flag, FLAG_PAGE);
+                        if (warp == 8 && lane < GROUPS) raise(a.flag, FLAG_PAGE);
                         number = -1;
                     }
                 }
                 return number;
             };
             auto begin_of = [&](int step, int32_t number) {
-                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane & 7) * 16;
+                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
                 return number < 0 ? int64_t(-1) : ((int64_t(number) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim;
             };
             uint4 x[TURNS];
             auto load = [&](int64_t offsets, int left, int turn) {
-                const int row = r0 + TURN_ROWS * turn;
-                const int64_t off = __shfl_sync(0xffffffffu, offsets, row >> 4);  // a warp's rows of a turn are of one group
-                if (off < 0 || row >= left || !in_dim) return make_uint4(0, 0, 0, 0);
-                return *reinterpret_cast<const uint4 *>(codes + off);
+                const int row = WARP_ROWS * (sub + CONVERTERS * turn) + r0;
+                const int64_t off = __shfl_sync(0xffffffffu, offsets, (row >> 4) % GROUPS);  // a warp's rows of a turn are of one group
+                if (off < 0 || row >= left || row >= KEYS || !in_dim) return make_uint4(0, 0, 0, 0);
+                return *reinterpret_cast<const uint4 *>(codes + off + (row & 15) * c.dim);
             };
             int32_t number = page_of(0), next = page_of(1);
             {
@@ -765,18 +705,22 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     uint32_t h[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) decode4<FMT, true>(w[e], h[2 * e], h[2 * e + 1]);
-                    sts128(dst + turn * (TURN_ROWS * 128) + at0, h[0], h[1], h[2], h[3]);
-                    sts128(dst + turn * (TURN_ROWS * 128) + at1, h[4], h[5], h[6], h[7]);
+                    const int row = WARP_ROWS * (sub + CONVERTERS * turn) + r0;
+                    const uint32_t at0 = dst + row * 128 + (((ch & 3) * 2 ^ (row & 7)) << 4);
+                    if (row < KEYS) {
+                        sts128(at0, h[0], h[1], h[2], h[3]);
+                        sts128(at0 ^ 16, h[4], h[5], h[6], h[7]);
+                    }
                 }
                 if (warp == 8) {
-                    float top = lane < 8 ? vs : 0.f;
+                    float top = vs;
 #pragma unroll
-                    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    top = fmaxf(__shfl_sync(0xffffffffu, top, 0), 1.17549435e-38f);
+                    for (int o = GROUPS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = fmaxf(top, 1.17549435e-38f);
                     const float ref = fmaxf(v_ref, top), unit = fmaxf(vs / ref, 8.6736174e-19f);  // 2^-60: below, values count for nothing
-                    const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xFFu;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << GROUPS) - 1);
                     Info &f = info[n % INFO];
-                    if (lane < 8) {
+                    if (lane < GROUPS) {
                         f.k[lane] = fmaxf(ks, 7.8886091e-31f);  // 2^-100: a factor of zero would make a hidden score not a number
                         f.v_log[lane] = log2f(unit);
                         f.v_inv[lane] = 1.f / unit;
@@ -793,6 +737,54 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 number = next;
                 next = page_of(step + 2);
             }
+        }
+    } else if (elect_one()) {
+        // ===== the products of tile t =====
+        const int t = warp - (8 + 2 * CONVERTERS);
+        uint32_t n = 0, n_s = 0, n_q = 0;
+        bool ok = true;
+        // The scores of the block's step n, the tile's step s: the keys are awaited; what info holds of the step is visible behind this
+        // thread's arrival.
+        auto issue_scores = [&](uint32_t n, uint32_t n_s) {
+            const int stage = n % STAGES, place = n_s & 1;
+            if (!mbar_wait(k_full(stage), (n / STAGES) & 1, abort_flag, S_KEYS)) return false;
+            fence_after();
+            scores_of<DP>(base, t, place, stage);
+            commit(s_full(t, place));
+            mbar_arrive(s_full(t, place));
+            commit(k_empty(stage));
+            return true;
+        };
+        for (int64_t at = begin; at < end && ok;) {
+            const Piece p = piece_at(at);
+            at = p.next;
+            if (p.steps == 0) continue;
+            if (t >= p.tiles) {
+                // No rows: the tile's arrivals all the same, step by step, so that its waits never run ahead by a phase.
+                for (int step = 0; step < p.steps && ok; ++step, ++n) {
+                    ok = mbar_wait(k_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_KEYS);
+                    mbar_arrive(k_empty(n % STAGES));
+                    ok = ok && mbar_wait(v_full(n % STAGES), (n / STAGES) & 1, abort_flag, S_VALUES);
+                    mbar_arrive(v_empty(n % STAGES));
+                }
+                continue;
+            }
+            ok = mbar_wait(q_ready(t), n_q++ & 1, abort_flag, S_QUERIES) && issue_scores(n, n_s);
+            if (p.steps > 1) ok = ok && issue_scores(n + 1, n_s + 1);
+            for (int step = 0; step < p.steps && ok; ++step, ++n, ++n_s) {
+                const int stage = n % STAGES;
+                ok = mbar_wait(p_ready(t), n_s & 1, abort_flag, S_WEIGHTS) && mbar_wait(v_full(stage), (n / STAGES) & 1, abort_flag, S_VALUES);
+                if (!ok) break;
+                fence_after();
+                output_of<DP>(base, t, n_s & 1, stage, step != 0);
+                commit(v_empty(stage));
+                commit(o_full(t));
+                if (step + 2 < p.steps) ok = issue_scores(n + 2, n_s + 2);
+            }
+        }
+        if (*abort_flag) {  // products in flight: time to end before their memory is given back
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000ll) {}
         }
     }
     __syncwarp();
