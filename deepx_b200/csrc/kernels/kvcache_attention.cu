@@ -177,58 +177,6 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
         const int rows = min(ROWS, int(min(int64_t(sq.n) * a.group - first_row, int64_t(ROWS))));
         const int steps = step1 - step0;
 
-        // ---- the queries: row g of each block of eight, the chunks this lane multiplies ----
-        uint32_t qb[NB][KC][4][2];
-        float c_row[NB][2];  // of the rows 2t and 2t + 1, whose scores this lane has
-        int pos[NB][2];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int r = 8 * nb + g, fr = first_row + r;
-            const bool live = r < rows;
-            const int i = live ? fr / a.group : 0;
-            const T *q = static_cast<const T *>(a.q) + (sq.row0 + i) * a.q_stride + int64_t(head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
-            Pack<T, 8> x[KC][2];
-            float amax = 0.f;
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                const int d = key_chunk<DP>(t, k) * 16;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (live && d < c.dim && a.q_vec) x[k][h] = ld_cached<T, 8>(q + d + 8 * h);
-                    else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[k][h].v[e] = live && d < c.dim ? q[d + 8 * h + e] : from_compute<T>(0.f);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k][h].v[e])));
-                }
-            }
-            float down = 1.f, c_mine = a.scale_log2;
-            if constexpr (std::is_same<T, bf16>::value) {
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-                if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
-                    down = __uint_as_float((254u - e) << 23);
-                    c_mine *= __uint_as_float(e << 23);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KC; ++k)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {  // word w of the chunk: dimensions 4w..4w+3
-                    const Pack<T, 8> &p = x[k][w >> 1];
-                    const int e = (w & 1) * 4;
-                    qb[nb][k][w][0] = half2_bits(to_compute(p.v[e]) * down, to_compute(p.v[e + 1]) * down);
-                    qb[nb][k][w][1] = half2_bits(to_compute(p.v[e + 2]) * down, to_compute(p.v[e + 3]) * down);
-                }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int col = 8 * nb + 2 * t + e;
-                c_row[nb][e] = __shfl_sync(0xffffffffu, c_mine, (2 * t + e) * 4);
-                pos[nb][e] = col < rows ? sq.first + (first_row + col) / a.group : INT32_MIN;
-            }
-        }
         const int pos_min = sq.first + first_row / a.group, pos_max = sq.first + (first_row + rows - 1) / a.group;
         const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's
 
@@ -291,6 +239,58 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
             issue(p, p, number);
         }
 
+        // ---- the queries, while the first keys are on their way: row g of each block of eight, the chunks this lane multiplies ----
+        uint32_t qb[NB][KC][4][2];
+        float c_row[NB][2];  // of the rows 2t and 2t + 1, whose scores this lane has
+        int pos[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g, fr = first_row + r;
+            const bool live = r < rows;
+            const int i = live ? fr / a.group : 0;
+            const T *q = static_cast<const T *>(a.q) + (sq.row0 + i) * a.q_stride + int64_t(head * a.group + (live ? fr - i * a.group : 0)) * c.dim;
+            Pack<T, 8> x[KC][2];
+            float amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const int d = key_chunk<DP>(t, k) * 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (live && d < c.dim && a.q_vec) x[k][h] = ld_cached<T, 8>(q + d + 8 * h);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[k][h].v[e] = live && d < c.dim ? q[d + 8 * h + e] : from_compute<T>(0.f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(to_compute(x[k][h].v[e])));
+                }
+            }
+            float down = 1.f, c_mine = a.scale_log2;
+            if constexpr (std::is_same<T, bf16>::value) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                if (amax > 0.f && amax < __int_as_float(0x7f800000)) {
+                    down = __uint_as_float((254u - e) << 23);
+                    c_mine *= __uint_as_float(e << 23);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {  // word w of the chunk: dimensions 4w..4w+3
+                    const Pack<T, 8> &p = x[k][w >> 1];
+                    const int e = (w & 1) * 4;
+                    qb[nb][k][w][0] = half2_bits(to_compute(p.v[e]) * down, to_compute(p.v[e + 1]) * down);
+                    qb[nb][k][w][1] = half2_bits(to_compute(p.v[e + 2]) * down, to_compute(p.v[e + 3]) * down);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = 8 * nb + 2 * t + e;
+                c_row[nb][e] = __shfl_sync(0xffffffffu, c_mine, (2 * t + e) * 4);
+                pos[nb][e] = col < rows ? sq.first + (first_row + col) / a.group : INT32_MIN;
+            }
+        }
         int stage = 0;
         for (int step = 0; step < steps; ++step) {
             cp_wait<K::STAGES - 2>();

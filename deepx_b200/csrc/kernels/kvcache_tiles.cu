@@ -717,16 +717,16 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
 #pragma unroll
                     for (int o = GROUPS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     top = fmaxf(top, 1.17549435e-38f);
-                    const float ref = fmaxf(v_ref, top), unit = fmaxf(vs / ref, 8.6736174e-19f);  // 2^-60: below, values count for nothing
+                    const float ref = fmaxf(v_ref, top), unit = fmaxf(__fdividef(vs, ref), 8.6736174e-19f);  // 2^-60: below, values count for nothing
                     const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << GROUPS) - 1);
                     Info &f = info[n % INFO];
                     if (lane < GROUPS) {
                         f.k[lane] = fmaxf(ks, 7.8886091e-31f);  // 2^-100: a factor of zero would make a hidden score not a number
-                        f.v_log[lane] = log2f(unit);
-                        f.v_inv[lane] = 1.f / unit;
+                        f.v_log[lane] = __log2f(unit);
+                        f.v_inv[lane] = __frcp_rn(unit);
                     }
                     if (lane == 0) {
-                        f.turn = v_ref == 0.f ? 1.f : v_ref / ref;
+                        f.turn = v_ref == 0.f || v_ref == ref ? 1.f : __fdividef(v_ref, ref);
                         f.v_ref = ref;
                         f.there = int(mask);
                     }

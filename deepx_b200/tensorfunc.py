@@ -305,24 +305,47 @@ def softmax(X: torch.Tensor, Out: torch.Tensor) -> None:
 
 
 # ---- queries, keys and the 8-bit key/value cache (no reference function) ------------------------------------
-def _on_device(*ts: torch.Tensor) -> None:
-    """All on one CUDA device; unlike _dev, rows may be strided."""
-    d = ts[0].device
+# These are called for each layer and token, with little work a call: their checks are written for few Python steps.
+def _device_index(*ts: torch.Tensor) -> int:
+    """The one CUDA device of all tensors; unlike _dev, rows may be strided."""
+    index = ts[0].get_device()
+    if index < 0:
+        raise ValueError("tensor is not on a CUDA device (this executor has no CPU path)")
     for t in ts:
-        if not t.is_cuda:
-            raise ValueError("tensor is not on a CUDA device (this executor has no CPU path)")
-        if t.device != d:
+        if t.get_device() != index:
             raise ValueError("tensors are on different devices")
+    return index
 
 
-def _token_rows(t: torch.Tensor, name: str) -> int:
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index`, its current stream."""
+    if torch.cuda.current_device() == index:
+        code = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if code:
+        N.check(code)
+
+
+def _token_rows(t: torch.Tensor, shape: torch.Size) -> int:
     """The stride between tokens of a [tokens, heads, head_dim] tensor whose rows are whole (a view of a packed projection is)."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-    n, h, d = t.shape
-    if (t.stride(2) != 1 and d > 1) or (t.stride(1) != d and h > 1):
-        raise ValueError(f"{name}: the heads of a token are not contiguous")
-    return t.stride(0) if n > 1 else builtins.max(h * d, 1)
+    n, h, d = shape
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and d > 1) or (s1 != d and h > 1):
+        raise ValueError("the heads of a token are not contiguous")
+    return s0 if n > 1 else builtins.max(h * d, 1)
+
+
+def _heads_of(*ts: torch.Tensor) -> torch.Size:
+    """The [tokens, heads, head_dim] shape that all tensors have."""
+    shape = ts[0].shape
+    if len(shape) != 3:
+        raise ValueError("expected [tokens, heads, head_dim]")
+    for t in ts[1:]:
+        if t.shape != shape:
+            raise ValueError("shape mismatch")
+    return shape
 
 
 def qknorm_rope(Q: torch.Tensor, K: torch.Tensor, q_weight, k_weight, inv_freq: torch.Tensor, positions: torch.Tensor, eps, interleaved: bool,
@@ -330,66 +353,72 @@ def qknorm_rope(Q: torch.Tensor, K: torch.Tensor, q_weight, k_weight, inv_freq: 
     """Each head of Q [tokens, q_heads, dim] and K [tokens, k_heads, dim] over sqrt(mean(x^2) + eps), times its weight [dim] or None
     (eps None: no norm), its first 2 * len(inv_freq) dimensions turned by positions[t] * inv_freq[i]: pairs (i, i + half), or
     (2i, 2i+1) when `interleaved`.  An output may be its input."""
-    _on_device(Q, K, inv_freq, positions, Qout, Kout)
-    _same_dtype(Q, K, Qout, Kout)
-    strides = [_token_rows(t, n) for t, n in ((Q, "Q"), (K, "K"), (Qout, "Qout"), (Kout, "Kout"))]
-    tokens, qh, dim = Q.shape
-    if Qout.shape != Q.shape or Kout.shape != K.shape or K.shape[0] != tokens or K.shape[2] != dim:
+    index = _device_index(Q, K, inv_freq, positions, Qout, Kout)
+    dtype = Q.dtype
+    if K.dtype is not dtype or Qout.dtype is not dtype or Kout.dtype is not dtype:
+        _same_dtype(Q, K, Qout, Kout)
+    qshape, kshape = _heads_of(Q, Qout), _heads_of(K, Kout)
+    tokens, qh, dim = qshape
+    if kshape[0] != tokens or kshape[2] != dim:
         raise ValueError("shape mismatch")
     for w in (q_weight, k_weight):
         if w is not None:
             if eps is None:
                 raise ValueError("weights belong to the norm: eps is None")
-            _dev(inv_freq, w)
-            _same_dtype(Q, w)
+            if w.get_device() != index or not w.is_contiguous():
+                _dev(inv_freq, w)
+            if w.dtype is not dtype:
+                _same_dtype(Q, w)
             if w.shape != (dim,):
                 raise ValueError("a weight holds head_dim elements")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise TypeError("inv_freq must be contiguous float32 [rotated / 2]")
     if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) or not positions.is_contiguous():
         raise TypeError("positions must be contiguous int32 or int64 [tokens]")
-    with torch.cuda.device(Q.device):
-        N.check(N.lib.dx_qknorm_rope(dtype_code(Q), Q.data_ptr(), strides[0], qh, K.data_ptr(), strides[1], K.shape[1], tokens, dim, int(eps is not None),
-                                     None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-                                     0.0 if eps is None else float(eps), inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved),
-                                     dtype_code(positions), positions.data_ptr(), Qout.data_ptr(), strides[2], Kout.data_ptr(), strides[3], _stream(Q)))
+    _call(index, N.lib.dx_qknorm_rope, dtype_code(Q), Q.data_ptr(), _token_rows(Q, qshape), qh, K.data_ptr(), _token_rows(K, kshape), kshape[1], tokens, dim,
+          eps is not None, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+          0.0 if eps is None else eps, inv_freq.data_ptr(), 2 * inv_freq.numel(), bool(interleaved), dtype_code(positions), positions.data_ptr(),
+          Qout.data_ptr(), _token_rows(Qout, qshape), Kout.data_ptr(), _token_rows(Kout, kshape))
 
 
 _CACHE_FORMATS = {torch.int8: N.CACHE_I8, torch.float8_e4m3fn: N.CACHE_E4M3}
 
 
-def _kvcache(rows: int, k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag) -> tuple:
-    """The two descriptors of a call over the cache, its tensors checked."""
-    _dev(k_cache, v_cache, k_scale, v_scale, starts, lens, table)
-    if k_cache.dtype not in _CACHE_FORMATS or v_cache.dtype != k_cache.dtype:
-        raise TypeError("a cache is int8 or float8_e4m3fn, keys and values alike")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+def _kvcache(rows: int, shape: torch.Size, k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag) -> tuple:
+    """The two descriptors of a call over the cache, its tensors checked; `shape` is that of the cache."""
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("a cache is [pages, kv_heads, page_tokens, head_dim], keys and values alike")
-    pages, heads, page, dim = k_cache.shape
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+    if k_cache.dtype not in _CACHE_FORMATS or v_cache.dtype is not k_cache.dtype:
+        raise TypeError("a cache is int8 or float8_e4m3fn, keys and values alike")
+    pages, heads, page, dim = shape
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
         raise TypeError("scales are float32")
     if k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
         raise ValueError("scales are [pages, kv_heads]")
-    if starts.dtype != torch.int32 or lens.dtype != torch.int32 or table.dtype != torch.int32:
+    int32 = torch.int32
+    if starts.dtype is not int32 or lens.dtype is not int32 or table.dtype is not int32:
         raise TypeError("starts, lens and table are int32")
-    batch = lens.shape[0] if lens.dim() == 1 else -1
-    if starts.shape != (batch + 1,) or table.dim() != 2 or table.shape[0] != batch:
+    tshape = table.shape
+    if len(tshape) != 2 or lens.shape != tshape[:1] or starts.shape != (tshape[0] + 1,):
         raise ValueError("starts is [batch + 1], lens [batch], table [batch, columns]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and starts.is_contiguous()
+            and lens.is_contiguous() and table.is_contiguous()):
+        raise ValueError("tensor is not contiguous")
     if oob_flag is not None:
         _dev(k_cache, oob_flag)
-        if oob_flag.dtype != torch.int32 or oob_flag.numel() < 1:
+        if oob_flag.dtype is not int32 or oob_flag.numel() < 1:
             raise TypeError("oob_flag is an int32 tensor")
-    return (N.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page, dim, _CACHE_FORMATS[k_cache.dtype]),
-            N.KvSeqs(starts.data_ptr(), lens.data_ptr(), table.data_ptr(), batch, table.shape[1], rows))
+    return (N.KvSeqs(starts.data_ptr(), lens.data_ptr(), table.data_ptr(), tshape[0], tshape[1], rows),
+            N.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page, dim, _CACHE_FORMATS[k_cache.dtype]))
 
 
-def _kv_rows(K: torch.Tensor, V: torch.Tensor, k_cache: torch.Tensor) -> tuple[int, int]:
-    _on_device(K, V, k_cache)
-    _same_dtype(K, V)
-    strides = _token_rows(K, "K"), _token_rows(V, "V")
-    if K.shape != V.shape or k_cache.dim() != 4 or K.shape[1] != k_cache.shape[1] or K.shape[2] != k_cache.shape[3]:
+def _kv_rows(K: torch.Tensor, V: torch.Tensor, cshape: torch.Size) -> torch.Size:
+    if K.dtype is not V.dtype:
+        _same_dtype(K, V)
+    shape = _heads_of(K, V)
+    if len(cshape) != 4 or shape[1] != cshape[1] or shape[2] != cshape[3]:
         raise ValueError("K and V must be [rows, kv_heads, head_dim] of the cache")
-    return strides
+    return shape
 
 
 def kvcache_write(K: torch.Tensor, V: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor,
@@ -397,21 +426,23 @@ def kvcache_write(K: torch.Tensor, V: torch.Tensor, starts: torch.Tensor, lens: 
     """The new tokens' keys and values [rows, kv_heads, head_dim] into the pages of the cache [pages, kv_heads, page_tokens, head_dim], in
     8 bits with one power-of-two scale for each page and head.  Sequence b's new tokens are the rows starts[b]..starts[b+1], the
     last ones of its lens[b] tokens; table[b] names its pages."""
-    ks, vs = _kv_rows(K, V, k_cache)
-    cache, seqs = _kvcache(K.shape[0], k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
-    with torch.cuda.device(K.device):
-        N.check(N.lib.dx_kvcache_write(dtype_code(K), K.data_ptr(), ks, V.data_ptr(), vs, seqs, cache, None if oob_flag is None else oob_flag.data_ptr(),
-                                       _stream(K)))
+    index = _device_index(K, V, k_cache, v_cache, k_scale, v_scale, starts, lens, table)
+    cshape = k_cache.shape
+    shape = _kv_rows(K, V, cshape)
+    seqs, cache = _kvcache(shape[0], cshape, k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
+    _call(index, N.lib.dx_kvcache_write, dtype_code(K), K.data_ptr(), _token_rows(K, shape), V.data_ptr(), _token_rows(V, shape), seqs, cache,
+          None if oob_flag is None else oob_flag.data_ptr())
 
 
 def kvcache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, starts: torch.Tensor,
                  lens: torch.Tensor, table: torch.Tensor, K: torch.Tensor, V: torch.Tensor, oob_flag: torch.Tensor | None = None) -> None:
     """The last starts[b+1] - starts[b] tokens of each sequence as values, into the rows of K and V."""
-    ks, vs = _kv_rows(K, V, k_cache)
-    cache, seqs = _kvcache(K.shape[0], k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
-    with torch.cuda.device(K.device):
-        N.check(N.lib.dx_kvcache_read(dtype_code(K), seqs, cache, K.data_ptr(), ks, V.data_ptr(), vs, None if oob_flag is None else oob_flag.data_ptr(),
-                                      _stream(K)))
+    index = _device_index(K, V, k_cache, v_cache, k_scale, v_scale, starts, lens, table)
+    cshape = k_cache.shape
+    shape = _kv_rows(K, V, cshape)
+    seqs, cache = _kvcache(shape[0], cshape, k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
+    _call(index, N.lib.dx_kvcache_read, dtype_code(K), seqs, cache, K.data_ptr(), _token_rows(K, shape), V.data_ptr(), _token_rows(V, shape),
+          None if oob_flag is None else oob_flag.data_ptr())
 
 
 def kvcache_attention(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -420,19 +451,19 @@ def kvcache_attention(Q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """Out = softmax(scale * Q K^T) V of the new tokens (whose keys are in the cache) over each sequence's tokens up to their own
     position, the last `window` of them if window > 0.  Q and Out are [rows, q_heads, head_dim], q_heads a multiple of the
     cache's heads.  max_new: the most new tokens of a sequence (0: not known); it decides how the work is split, not what comes out."""
-    _on_device(Q, Out, k_cache)
-    _same_dtype(Q, Out)
-    qs, os = _token_rows(Q, "Q"), _token_rows(Out, "Out")
-    if Q.shape != Out.shape or k_cache.dim() != 4 or Q.shape[2] != k_cache.shape[3]:
+    index = _device_index(Q, Out, k_cache, v_cache, k_scale, v_scale, starts, lens, table)
+    if Q.dtype is not Out.dtype:
+        _same_dtype(Q, Out)
+    shape, cshape = _heads_of(Q, Out), k_cache.shape
+    if len(cshape) != 4 or shape[2] != cshape[3]:
         raise ValueError("Q and Out must be [rows, q_heads, head_dim] of the cache")
-    cache, seqs = _kvcache(Q.shape[0], k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
-    code, heads = dtype_code(Q), Q.shape[1]
-    with torch.cuda.device(Q.device):
-        need = N.lib.dx_kvcache_attention_workspace_bytes(code, heads, seqs, cache, int(max_new))
-        # from the caching allocator for each call: a call captured into a graph then has scratch of its own graph's pool
-        ws = torch.empty(need, dtype=torch.uint8, device=Q.device) if need else None
-        N.check(N.lib.dx_kvcache_attention(code, Q.data_ptr(), qs, heads, seqs, cache, float(scale), int(max_new), int(window), Out.data_ptr(), os,
-                                           None if ws is None else ws.data_ptr(), need, None if oob_flag is None else oob_flag.data_ptr(), _stream(Q)))
+    seqs, cache = _kvcache(shape[0], cshape, k_cache, v_cache, k_scale, v_scale, starts, lens, table, oob_flag)
+    code, heads = dtype_code(Q), shape[1]
+    need = N.lib.dx_kvcache_attention_workspace_bytes(code, heads, seqs, cache, max_new)
+    # from the caching allocator for each call: a call captured into a graph then has scratch of its own graph's pool
+    ws = torch.empty(need, dtype=torch.uint8, device=Q.device) if need else None
+    _call(index, N.lib.dx_kvcache_attention, code, Q.data_ptr(), _token_rows(Q, shape), heads, seqs, cache, scale, max_new, window, Out.data_ptr(),
+          _token_rows(Out, shape), None if ws is None else ws.data_ptr(), need, None if oob_flag is None else oob_flag.data_ptr())
 
 
 # ---- changeshape -----------------------------------------------------------------------------------------
