@@ -109,7 +109,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     __shared__ int found_b;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     griddep_wait_cta();
-    if (blockIdx.x == 0) check_seqs(s, c, a.flag);
+    if (blockIdx.x == gridDim.x - 1) check_seqs(s, c, a.flag);  // a block that has no piece when there is little to do
 
     // ---- this block's piece of the line ----
     const int per = (s.batch + CTA - 1) / CTA;
@@ -161,6 +161,13 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     // the sixteen bytes of a tile that this lane loads first; the others lie whole rows further
     const int lane_row = lane / (DP / 16), lane_chunk = lane % (DP / 16), lane_src = lane_row * c.dim + lane_chunk * 16, row_step = (512 / DP) * c.dim;
     const bool lane_in = lane_chunk * 16 < c.dim;
+    // where this lane's parts of a tile lie in a stage: to load (rows of either parity of 512 / DP), keys, values of even and odd tokens
+    const uint32_t load_at = place<DP>(lane_row, lane_chunk), load_odd = load_at ^ 64;
+    const uint32_t key_at = place<DP>(g, key_chunk<DP>(t, 0));
+    const int value_half = DP == 64 ? (g & 1) * 8 : 0;
+    const uint32_t value_at = place<DP>(2 * t, DP == 64 ? g >> 1 : g) + value_half, value_odd = place<DP>(2 * t + 1, DP == 64 ? g >> 1 : g) + value_half;
+    auto later = [](uint32_t at) { return (DP == 64 ? at ^ 64 : at) + 8 * DP; };  // the same of the token eight further
+    const int64_t page_bytes = int64_t(c.heads) * c.page * c.dim;
     for (int64_t at = begin; at < end;) {
         const Seq sq = seq_at(s, c, b);
         const Line ln = line_of<ROWS>(sq, a);
@@ -194,6 +201,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
 
         // ---- keys and values in flight ----
         const int32_t *table = s.table + int64_t(b) * s.cols;
+        const int64_t head_bytes = int64_t(head) * c.page * c.dim;
         auto token0 = [&](int step) { return ln.lo + (step0 + step) * STEP + warp * WT; };
         auto page_number = [&](int step) {
             const int j = token0(step);
@@ -205,14 +213,13 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                 const int left = seen_end - j;  // tokens to load
                 const bool ok = left > 0 && number >= 0 && number < c.pages;
                 if (left > 0 && !ok && lane == 0) raise(a.flag, FLAG_PAGE);
-                const int64_t ph = ok ? int64_t(number) * c.heads + head : 0;
-                const int64_t base = ok ? (ph * c.page + (j & (c.page - 1))) * c.dim + lane_src : 0;
                 const uint32_t dst = ring_u + stage * 2 * K::TILE;
-                const uint8_t *ksrc = c.k + base, *vsrc = c.v + base;
+                const int64_t base = ok ? number * page_bytes + head_bytes + (j & (c.page - 1)) * c.dim : 0;
+                const uint8_t *ksrc = c.k + (base + lane_src), *vsrc = c.v + (base + lane_src);
                 if (ok && left >= WT && c.dim == DP) {
 #pragma unroll
                     for (int i = 0; i < K::TILE / 512; ++i) {
-                        const uint32_t at = dst + place<DP>(i * (512 / DP) + lane_row, lane_chunk);
+                        const uint32_t at = dst + (DP == 256 ? place<DP>(i * 2 + lane_row, lane_chunk) : (i & 1 ? load_odd : load_at) + i * 512);
                         cp_async16(at, ksrc + i * 512, true);
                         cp_async16(at + K::TILE, vsrc + i * 512, true);
                     }
@@ -226,6 +233,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                         cp_async16(at + K::TILE, in ? vsrc + off : c.v, in);
                     }
                 }
+                const int64_t ph = ok ? int64_t(number) * c.heads + head : 0;
                 if (lane < 2) cp_async4(smem_u32(&scales[warp][stage][lane]), (lane ? c.v_scale : c.k_scale) + ph, ok);
                 if (lane == 2) in_cache[warp][stage] = ok;
             }
@@ -315,7 +323,9 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                 for (int e = 0; e < 4; ++e) x[nb][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
-                const uint4 w0 = lds128(ks + place<DP>(g, key_chunk<DP>(t, k))), w1 = lds128(ks + place<DP>(g + 8, key_chunk<DP>(t, k)));
+                // the second chunk is the first one's neighbour, the third and fourth lie 128 bytes further
+                const uint32_t at = (key_at ^ ((k & 1) << 4)) + (k >> 1) * 128;
+                const uint4 w0 = lds128(ks + at), w1 = lds128(ks + later(at));
                 const uint32_t lo[4] = {w0.x, w0.y, w0.z, w0.w}, hi[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -330,7 +340,8 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[nb][e] *= c_row[nb][e & 1] * k_scale;
-            if (j0 + WT - 1 > pos_min || j0 + WT > sq.end || (a.window > 0 && j0 <= int64_t(pos_max) - a.window)) {
+            const bool masked = j0 + WT - 1 > pos_min || j0 + WT > sq.end || (a.window > 0 && j0 <= int64_t(pos_max) - a.window);
+            if (masked) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -400,36 +411,38 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                         p[nb][i] = *reinterpret_cast<const uint32_t *>(&w);
                     }
             }
-            auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
-                uint32_t v0[4], v1[4];  // of dimensions 2 tile, 2 tile + 1 and the two after: tokens 2t.., tokens 2t + 8..
-                decode4<FMT, true>(__byte_perm(wa, wb, 0x5140), v0[0], v0[1]);
-                decode4<FMT, true>(__byte_perm(wc, wd, 0x5140), v0[2], v0[3]);
-                decode4<FMT, true>(__byte_perm(wa, wb, 0x7362), v1[0], v1[1]);
-                decode4<FMT, true>(__byte_perm(wc, wd, 0x7362), v1[2], v1[3]);
+            // FINITE: some of the tile's tokens are masked for some rows; what lies there must not be no number.
+            auto values = [&](auto finite) {
+                auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
+                    uint32_t v0[4], v1[4];  // of dimensions 2 tile, 2 tile + 1 and the two after: tokens 2t.., tokens 2t + 8..
+                    decode4<FMT, decltype(finite)::value>(__byte_perm(wa, wb, 0x5140), v0[0], v0[1]);
+                    decode4<FMT, decltype(finite)::value>(__byte_perm(wc, wd, 0x5140), v0[2], v0[3]);
+                    decode4<FMT, decltype(finite)::value>(__byte_perm(wa, wb, 0x7362), v1[0], v1[1]);
+                    decode4<FMT, decltype(finite)::value>(__byte_perm(wc, wd, 0x7362), v1[2], v1[3]);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    mma(o[nb][tile], v0, p[nb][0], p[nb][1]);
-                    mma(o[nb][tile + 1], v1, p[nb][0], p[nb][1]);
+                    for (int nb = 0; nb < NB; ++nb) {
+                        mma(o[nb][tile], v0, p[nb][0], p[nb][1]);
+                        mma(o[nb][tile + 1], v1, p[nb][0], p[nb][1]);
+                    }
+                };
+                if constexpr (DP == 64) {
+                    const uint2 wa = lds64(vs + value_at), wb = lds64(vs + value_odd), wc = lds64(vs + later(value_at)), wd = lds64(vs + later(value_odd));
+                    four(wa.x, wb.x, wc.x, wd.x, 0);
+                    four(wa.y, wb.y, wc.y, wd.y, 2);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < VC; ++h) {
+                        const uint4 wa = lds128(vs + value_at + 128 * h), wb = lds128(vs + value_odd + 128 * h);
+                        const uint4 wc = lds128(vs + later(value_at) + 128 * h), wd = lds128(vs + later(value_odd) + 128 * h);
+                        four(wa.x, wb.x, wc.x, wd.x, 8 * h);
+                        four(wa.y, wb.y, wc.y, wd.y, 8 * h + 2);
+                        four(wa.z, wb.z, wc.z, wd.z, 8 * h + 4);
+                        four(wa.w, wb.w, wc.w, wd.w, 8 * h + 6);
+                    }
                 }
             };
-            if constexpr (DP == 64) {
-                const int half = (g & 1) * 8;
-                const uint2 wa = lds64(vs + place<DP>(2 * t, g >> 1) + half), wb = lds64(vs + place<DP>(2 * t + 1, g >> 1) + half);
-                const uint2 wc = lds64(vs + place<DP>(2 * t + 8, g >> 1) + half), wd = lds64(vs + place<DP>(2 * t + 9, g >> 1) + half);
-                four(wa.x, wb.x, wc.x, wd.x, 0);
-                four(wa.y, wb.y, wc.y, wd.y, 2);
-            } else {
-#pragma unroll
-                for (int h = 0; h < VC; ++h) {
-                    const int ch = g + 8 * h;
-                    const uint4 wa = lds128(vs + place<DP>(2 * t, ch)), wb = lds128(vs + place<DP>(2 * t + 1, ch));
-                    const uint4 wc = lds128(vs + place<DP>(2 * t + 8, ch)), wd = lds128(vs + place<DP>(2 * t + 9, ch));
-                    four(wa.x, wb.x, wc.x, wd.x, 8 * h);
-                    four(wa.y, wb.y, wc.y, wd.y, 8 * h + 2);
-                    four(wa.z, wb.z, wc.z, wd.z, 8 * h + 4);
-                    four(wa.w, wb.w, wc.w, wd.w, 8 * h + 6);
-                }
-            }
+            if (FMT == DX_CACHE_E4M3 && masked) values(std::true_type());
+            else values(std::false_type());
         }
         cp_wait<0>();
         __syncthreads();  // every warp is done with its ring

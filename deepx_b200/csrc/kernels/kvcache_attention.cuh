@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
 // with its item and does not end it part 2i + 1.  Sixteen warps share sixteen of the item's rows; the warps of a row share its parts.
 template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
-    constexpr int V = DP / 32, PART = ROWS * DP + 2 * ROWS;
+    constexpr int V = DP / 32, VW = V < 4 ? V : 4, PART = ROWS * DP + 2 * ROWS;
     __shared__ float sh[JOIN_CTA / 32][DP];
     griddep_wait_cta();
     const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
@@ -94,9 +94,9 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
 #pragma unroll 4
             for (int p = sub; p < n; p += each) {
                 const float by = __shfl_sync(0xffffffffu, w, p);
-                const float *src = at(p0 + p) + row * DP + lane * V;
+                const Pack<float, VW> *src = reinterpret_cast<const Pack<float, VW> *>(at(p0 + p) + row * DP + lane * V);
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e];
+                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e / VW].v[e % VW];
             }
         }
     }
