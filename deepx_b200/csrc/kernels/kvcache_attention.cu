@@ -20,15 +20,15 @@ namespace kv {
 namespace {
 
 constexpr int WARPS = 4, CTA = WARPS * 32;
-constexpr int WT = 16;     // tokens a warp takes at a time: never more than one page
-constexpr int STEP = WARPS * WT;
-constexpr int MIN_STEPS = 2;  // of a block: fewer would cost more in joining than they save
+constexpr int MIN_TOKENS = 128;  // of a block: fewer would cost more in joining than they save
 
-// DP: the head's dimensions, padded; NB: blocks of eight rows of an item.
-template <int DP, int NB> struct Cfg {
-    static constexpr int ROWS = 8 * NB;
-    static constexpr int STAGES = DP == 64 ? 4 : 3;
-    static constexpr int BLOCKS = DP == 256 ? 2 : NB == 1 ? 4 : 3;  // resident on an SM
+// DP: the head's dimensions, padded; NB: blocks of eight rows of an item; WT: tokens a warp takes at a time, of one page.  What a turn of
+// the loop costs besides its tokens (addresses, the wait, the vote on the maximum) is half of it at 16 tokens, so 32 are taken where the
+// pages and the registers allow it (one token after 262100: 110 us with 16, 102 us with 32).
+template <int DP, int NB, int WT> struct Cfg {
+    static constexpr int ROWS = 8 * NB, STEP = WARPS * WT;
+    static constexpr int STAGES = WT == 32 ? (DP == 64 ? 3 : 2) : DP == 64 ? 4 : 3;
+    static constexpr int BLOCKS = DP == 256 ? 2 : NB == 1 && WT == 16 ? 4 : 3;  // resident on an SM
     static constexpr int TILE = WT * DP;                                            // bytes of a warp's keys (or values) of a stage
     static constexpr int RING = STAGES * 2 * TILE;                                  // of a warp; holds its ROWS x DP floats at the end
     static constexpr int SMEM = WARPS * RING;
@@ -78,7 +78,7 @@ template <int DP> __device__ __forceinline__ int key_chunk(int t, int i) { retur
 struct Line {
     int lo, steps, tiles;  // first token of the range (a multiple of STEP), steps of a tile of rows, tiles of rows of a head
 };
-template <int ROWS> __device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
+template <int ROWS, int STEP> __device__ __forceinline__ Line line_of(const Seq &q, const Attn &a) {
     Line l;
     const int64_t hi = min(int64_t(q.end), int64_t(q.first) + q.n);
     const int64_t lo = a.window > 0 ? max(int64_t(0), int64_t(q.first) - a.window + 1) : 0;
@@ -87,16 +87,17 @@ template <int ROWS> __device__ __forceinline__ Line line_of(const Seq &q, const 
     l.tiles = int((int64_t(q.n) * a.group + ROWS - 1) / ROWS);
     return l;
 }
-template <int ROWS> __device__ __forceinline__ int64_t steps_of(const Seqs &s, const Cache &c, const Attn &a, int b) {
+template <int ROWS, int STEP> __device__ __forceinline__ int64_t steps_of(const Seqs &s, const Cache &c, const Attn &a, int b) {
     const Seq q = seq_at(s, c, b);
     if (q.n == 0) return 0;
-    const Line l = line_of<ROWS>(q, a);
+    const Line l = line_of<ROWS, STEP>(q, a);
     return int64_t(l.steps) * l.tiles * c.heads;
 }
 
-template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__(CTA, Cfg<DP, NB>::BLOCKS) attention_kernel(Attn a, Cache c, Seqs s) {
-    using K = Cfg<DP, NB>;
-    constexpr int ROWS = K::ROWS;
+template <typename T, int FMT, int DP, int NB, int WT>
+__global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel(Attn a, Cache c, Seqs s) {
+    using K = Cfg<DP, NB, WT>;
+    constexpr int ROWS = K::ROWS, STEP = K::STEP, TT = WT / 16;  // TT: tiles of sixteen tokens
     constexpr int MT = DP / 16;            // tiles of sixteen dimensions of the output
     constexpr int KC = DP / 64;            // chunks of a key that a lane multiplies
     constexpr int VC = DP == 256 ? 2 : 1;  // chunks of a value that a lane multiplies (half of one at DP 64)
@@ -115,7 +116,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     const int per = (s.batch + CTA - 1) / CTA;
     {
         int64_t mine = 0;
-        for (int b = threadIdx.x * per; b < min(s.batch, int(threadIdx.x + 1) * per); ++b) mine += steps_of<ROWS>(s, c, a, b);
+        for (int b = threadIdx.x * per; b < min(s.batch, int(threadIdx.x + 1) * per); ++b) mine += steps_of<ROWS, STEP>(s, c, a, b);
         int64_t sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -132,7 +133,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
         __syncthreads();
     }
     const int64_t total = total_steps;
-    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / MIN_STEPS));
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total * STEP / MIN_TOKENS));
     Join *join = reinterpret_cast<Join *>(a.ws) + blockIdx.x;
     float *parts = reinterpret_cast<float *>(a.ws + gridDim.x * sizeof(Join));
     if (total == 0 || int64_t(blockIdx.x) >= blocks) {
@@ -144,7 +145,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
         int64_t at = before[threadIdx.x];
         int b = threadIdx.x * per;
         for (; b < s.batch; ++b) {
-            const int64_t n = steps_of<ROWS>(s, c, a, b);
+            const int64_t n = steps_of<ROWS, STEP>(s, c, a, b);
             if (at + n > begin) break;
             at += n;
         }
@@ -170,7 +171,7 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     const int64_t page_bytes = int64_t(c.heads) * c.page * c.dim;
     for (int64_t at = begin; at < end;) {
         const Seq sq = seq_at(s, c, b);
-        const Line ln = line_of<ROWS>(sq, a);
+        const Line ln = line_of<ROWS, STEP>(sq, a);
         const int64_t seq_steps = sq.n ? int64_t(ln.steps) * ln.tiles * c.heads : 0;
         if (at >= seq_begin + seq_steps) {  // on to the next sequence
             seq_begin += seq_steps;
@@ -315,41 +316,56 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
             if (++stage == K::STAGES) stage = 0;
             if (!ok) continue;  // no token of a page: nothing to see
 
-            // ---- scores: lane (g, t) holds tokens g, g+8 of rows 2t, 2t+1 ----
-            float x[NB][4];
+            // ---- scores: lane (g, t) holds tokens g, g+8 (of each sixteen) of rows 2t, 2t+1 ----
+            float x[NB][TT][4];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[nb][e] = 0.f;
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[nb][tt][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
                 // the second chunk is the first one's neighbour, the third and fourth lie 128 bytes further
                 const uint32_t at = (key_at ^ ((k & 1) << 4)) + (k >> 1) * 128;
-                const uint4 w0 = lds128(ks + at), w1 = lds128(ks + later(at));
-                const uint32_t lo[4] = {w0.x, w0.y, w0.z, w0.w}, hi[4] = {w1.x, w1.y, w1.z, w1.w};
+                uint4 w0[TT], w1[TT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t ka[4];
-                    decode4<FMT, false>(lo[i], ka[0], ka[2]);
-                    decode4<FMT, false>(hi[i], ka[1], ka[3]);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) mma(x[nb], ka, qb[nb][k][i][0], qb[nb][k][i][1]);
+                for (int tt = 0; tt < TT; ++tt) {
+                    w0[tt] = lds128(ks + at + tt * 16 * DP);
+                    w1[tt] = lds128(ks + later(at) + tt * 16 * DP);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) {
+                        const uint32_t lo[4] = {w0[tt].x, w0[tt].y, w0[tt].z, w0[tt].w}, hi[4] = {w1[tt].x, w1[tt].y, w1[tt].z, w1[tt].w};
+                        uint32_t ka[4];
+                        decode4<FMT, false>(lo[i], ka[0], ka[2]);
+                        decode4<FMT, false>(hi[i], ka[1], ka[3]);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) mma(x[nb][tt], ka, qb[nb][k][i][0], qb[nb][k][i][1]);
+                    }
             }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int nb = 0; nb < NB; ++nb) {
+                const float c0 = c_row[nb][0] * k_scale, c1 = c_row[nb][1] * k_scale;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[nb][e] *= c_row[nb][e & 1] * k_scale;
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[nb][tt][e] *= e & 1 ? c1 : c0;
+            }
             const bool masked = j0 + WT - 1 > pos_min || j0 + WT > sq.end || (a.window > 0 && j0 <= int64_t(pos_max) - a.window);
             if (masked) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = j0 + g + 8 * (e >> 1), p = pos[nb][e & 1];
-                        const bool seen = j <= p && j < sq.end && (a.window <= 0 || j > int64_t(p) - a.window);
-                        if (!seen) x[nb][e] = NEG_INF;
-                    }
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = j0 + 16 * tt + g + 8 * (e >> 1), p = pos[nb][e & 1];
+                            const bool seen = j <= p && j < sq.end && (a.window <= 0 || j > int64_t(p) - a.window);
+                            if (!seen) x[nb][tt][e] = NEG_INF;
+                        }
             }
             // ---- running maximum: a row's rises when a score is 2^8 above it ----
             float top[NB][2];
@@ -358,7 +374,9 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float v = fmaxf(x[nb][e], x[nb][e + 2]);
+                    float v = fmaxf(x[nb][0][e], x[nb][0][e + 2]);
+#pragma unroll
+                    for (int tt = 1; tt < TT; ++tt) v = fmaxf(v, fmaxf(x[nb][tt][e], x[nb][tt][e + 2]));
                     rise |= v > m[nb][e] + LAG;
                     top[nb][e] = v;
                 }
@@ -389,14 +407,17 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                     }
                 }
             }
-            uint32_t p[NB][2];
+            uint32_t p[NB][TT][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float m0 = (m[nb][0] == NEG_INF ? 0.f : m[nb][0]) - UP, m1 = (m[nb][1] == NEG_INF ? 0.f : m[nb][1]) - UP;
-                p[nb][0] = transpose8(half2_bits(exp2_approx(x[nb][0] - m0), exp2_approx(x[nb][1] - m1)));
-                p[nb][1] = transpose8(half2_bits(exp2_approx(x[nb][2] - m0), exp2_approx(x[nb][3] - m1)));
                 const uint32_t one[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-                mma(l[nb], one, p[nb][0], p[nb][1]);  // the sum of the very weights that multiply the values
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+                    p[nb][tt][0] = transpose8(half2_bits(exp2_approx(x[nb][tt][0] - m0), exp2_approx(x[nb][tt][1] - m1)));
+                    p[nb][tt][1] = transpose8(half2_bits(exp2_approx(x[nb][tt][2] - m0), exp2_approx(x[nb][tt][3] - m1)));
+                    mma(l[nb], one, p[nb][tt][0], p[nb][tt][1]);  // the sum of the very weights that multiply the values
+                }
             }
 
             // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
@@ -406,14 +427,14 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const __half2 w = __hmul2(*reinterpret_cast<const __half2 *>(&p[nb][i]), unit);
-                        p[nb][i] = *reinterpret_cast<const uint32_t *>(&w);
+                    for (int i = 0; i < 2 * TT; ++i) {
+                        const __half2 w = __hmul2(*reinterpret_cast<const __half2 *>(&p[nb][i >> 1][i & 1]), unit);
+                        p[nb][i >> 1][i & 1] = *reinterpret_cast<const uint32_t *>(&w);
                     }
             }
             // FINITE: some of the tile's tokens are masked for some rows; what lies there must not be no number.
             auto values = [&](auto finite) {
-                auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
+                auto four = [&](int tt, uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
                     uint32_t v0[4], v1[4];  // of dimensions 2 tile, 2 tile + 1 and the two after: tokens 2t.., tokens 2t + 8..
                     decode4<FMT, decltype(finite)::value>(__byte_perm(wa, wb, 0x5140), v0[0], v0[1]);
                     decode4<FMT, decltype(finite)::value>(__byte_perm(wc, wd, 0x5140), v0[2], v0[3]);
@@ -421,23 +442,27 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
                     decode4<FMT, decltype(finite)::value>(__byte_perm(wc, wd, 0x7362), v1[2], v1[3]);
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        mma(o[nb][tile], v0, p[nb][0], p[nb][1]);
-                        mma(o[nb][tile + 1], v1, p[nb][0], p[nb][1]);
+                        mma(o[nb][tile], v0, p[nb][tt][0], p[nb][tt][1]);
+                        mma(o[nb][tile + 1], v1, p[nb][tt][0], p[nb][tt][1]);
                     }
                 };
-                if constexpr (DP == 64) {
-                    const uint2 wa = lds64(vs + value_at), wb = lds64(vs + value_odd), wc = lds64(vs + later(value_at)), wd = lds64(vs + later(value_odd));
-                    four(wa.x, wb.x, wc.x, wd.x, 0);
-                    four(wa.y, wb.y, wc.y, wd.y, 2);
-                } else {
 #pragma unroll
-                    for (int h = 0; h < VC; ++h) {
-                        const uint4 wa = lds128(vs + value_at + 128 * h), wb = lds128(vs + value_odd + 128 * h);
-                        const uint4 wc = lds128(vs + later(value_at) + 128 * h), wd = lds128(vs + later(value_odd) + 128 * h);
-                        four(wa.x, wb.x, wc.x, wd.x, 8 * h);
-                        four(wa.y, wb.y, wc.y, wd.y, 8 * h + 2);
-                        four(wa.z, wb.z, wc.z, wd.z, 8 * h + 4);
-                        four(wa.w, wb.w, wc.w, wd.w, 8 * h + 6);
+                for (int tt = 0; tt < TT; ++tt) {
+                    const uint32_t even = vs + tt * 16 * DP + value_at, odd = vs + tt * 16 * DP + value_odd;
+                    const uint32_t even8 = vs + tt * 16 * DP + later(value_at), odd8 = vs + tt * 16 * DP + later(value_odd);
+                    if constexpr (DP == 64) {
+                        const uint2 wa = lds64(even), wb = lds64(odd), wc = lds64(even8), wd = lds64(odd8);
+                        four(tt, wa.x, wb.x, wc.x, wd.x, 0);
+                        four(tt, wa.y, wb.y, wc.y, wd.y, 2);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < VC; ++h) {
+                            const uint4 wa = lds128(even + 128 * h), wb = lds128(odd + 128 * h), wc = lds128(even8 + 128 * h), wd = lds128(odd8 + 128 * h);
+                            four(tt, wa.x, wb.x, wc.x, wd.x, 8 * h);
+                            four(tt, wa.y, wb.y, wc.y, wd.y, 8 * h + 2);
+                            four(tt, wa.z, wb.z, wc.z, wd.z, 8 * h + 4);
+                            four(tt, wa.w, wb.w, wc.w, wd.w, 8 * h + 6);
+                        }
                     }
                 }
             };
@@ -530,34 +555,32 @@ template <typename T, int FMT, int DP, int NB> __global__ void __launch_bounds__
     }
 }
 
-template <typename T, int FMT, int DP, int NB> int launch_rows(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
-    using K = Cfg<DP, NB>;
+template <typename T, int FMT, int DP, int NB, int WT> int launch_tokens(const Attn &a, const Cache &c, const Seqs &s, cudaStream_t st) {
+    using K = Cfg<DP, NB, WT>;
     static std::atomic<uint64_t> prepared{0};  // one bit for each device
-    if (int e = allow_shared(attention_kernel<T, FMT, DP, NB>, K::SMEM, &prepared)) return e;
+    if (int e = allow_shared(attention_kernel<T, FMT, DP, NB, WT>, K::SMEM, &prepared)) return e;
     const unsigned grid = unsigned(sm_count() * K::BLOCKS);
-    launch_pdl(attention_kernel<T, FMT, DP, NB>, dim3(grid), dim3(CTA), K::SMEM, st, a, c, s);
+    launch_pdl(attention_kernel<T, FMT, DP, NB, WT>, dim3(grid), dim3(CTA), K::SMEM, st, a, c, s);
     if (int e = check_launch("kvcache_attention")) return e;
     launch_pdl(join_kernel<T, DP, K::ROWS>, dim3(grid), dim3(JOIN_CTA), 0, st, a, c);
     return check_launch("kvcache_attention (join)");
 }
+// Up to eight rows of up to 128 dimensions leave registers for 32 tokens at a time; pages of sixteen hold no 32.
 template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c, const Seqs &s, int64_t rows, cudaStream_t st) {
-    if (rows <= 8) return launch_rows<T, FMT, DP, 1>(a, c, s, st);
-    return launch_rows<T, FMT, DP, 2>(a, c, s, st);
+    if (rows > 8) return launch_tokens<T, FMT, DP, 2, 16>(a, c, s, st);
+    if constexpr (DP <= 128)
+        if (c.page >= 32) return launch_tokens<T, FMT, DP, 1, 32>(a, c, s, st);
+    return launch_tokens<T, FMT, DP, 1, 16>(a, c, s, st);
 }
 
-template <int DP, int NB> size_t workspace_of() {
-    using K = Cfg<DP, NB>;
-    return size_t(sm_count()) * K::BLOCKS * (sizeof(Join) + 2 * K::PART * sizeof(float));
+// Large enough for every variant of the head's dimensions.
+template <int DP> size_t workspace_of() {
+    const size_t one = Cfg<DP, 1, 16>::BLOCKS * (sizeof(Join) + 2 * Cfg<DP, 1, 16>::PART * sizeof(float));
+    const size_t two = Cfg<DP, 2, 16>::BLOCKS * (sizeof(Join) + 2 * Cfg<DP, 2, 16>::PART * sizeof(float));
+    return size_t(sm_count()) * (one > two ? one : two);
 }
-template <int DP> size_t workspace_rows(int64_t rows) { return rows <= 8 ? workspace_of<DP, 1>() : workspace_of<DP, 2>(); }
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-size_t workspace(int dim, int64_t rows) {
-    switch (padded(dim)) {
-        case 64: return workspace_rows<64>(rows);
-        case 128: return workspace_rows<128>(rows);
-        default: return workspace_rows<256>(rows);
-    }
-}
+size_t workspace(int dim) { return dim <= 64 ? workspace_of<64>() : dim <= 128 ? workspace_of<128>() : workspace_of<256>(); }
 // Whether a call goes to the tiles of 128 rows: as soon as a sequence may have more rows than one item here.
 bool by_tiles(const Cache &c, int64_t rows) { return c.dim <= 128 && rows > 16; }
 // The most rows of a sequence that share a key head, as far as the caller says.
@@ -576,7 +599,7 @@ extern "C" size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_head
     if (kv::check("kvcache_attention", cache, seqs, &c, &s) || s.rows == 0 || s.batch == 0) return 0;
     if (q_heads < 1 || q_heads % c.heads) return 0;
     const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
-    return kv::by_tiles(c, rows) ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim, rows);
+    return kv::by_tiles(c, rows) ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim);
 }
 
 extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache,
@@ -601,7 +624,7 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
         return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
     const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
     const bool tiles = kv::by_tiles(c, rows);
-    const size_t need = tiles ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim, rows);
+    const size_t need = tiles ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim);
     if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
     kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),

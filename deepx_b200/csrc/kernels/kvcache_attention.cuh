@@ -79,7 +79,12 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
     float acc[V] = {}, sum = 0.f;
     if (r < rows) {
         float top = NEG_INF;
-        for (int p = lane; p < j.parts; p += 32) top = fmaxf(top, at(p)[ROWS * DP + row]);
+        for (int p0 = lane; p0 < j.parts; p0 += 128) {
+            float m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = p0 + 32 * k < j.parts ? at(p0 + 32 * k)[ROWS * DP + row] : NEG_INF;
+            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float base = top == NEG_INF ? 0.f : top;
@@ -91,12 +96,20 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             sum += s;
             const int n = min(32, j.parts - p0);
-#pragma unroll 4
-            for (int p = sub; p < n; p += each) {
-                const float by = __shfl_sync(0xffffffffu, w, p);
-                const Pack<float, VW> *src = reinterpret_cast<const Pack<float, VW> *>(at(p0 + p) + row * DP + lane * V);
+            for (int p1 = sub; p1 < n; p1 += 8 * each) {  // eight loads in flight
+                Pack<float, VW> x[8][V / VW];
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] += by == 0.f ? 0.f : by * src[e / VW].v[e % VW];
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int e = 0; e < V / VW; ++e)
+                        if (p1 + k * each < n) x[k][e] = reinterpret_cast<const Pack<float, VW> *>(at(p0 + p1 + k * each) + row * DP + lane * V)[e];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float by = __shfl_sync(0xffffffffu, w, min(p1 + k * each, 31));
+                    if (p1 + k * each >= n || by == 0.f) continue;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += by * x[k][e / VW].v[e % VW];
+                }
             }
         }
     }
