@@ -997,6 +997,141 @@ struct SoftmaxTF : TF {
     }
 };
 
+// ---- a transformer layer's attention over an 8-bit key/value cache (no reference counterpart) ------------------------------
+// The cache is four tensors: k and v, int8 [pages kv_heads page_tokens head_dim] (the codes; the format says int8 or e4m3), and their
+// scales, float32 [pages kv_heads].  starts [batch+1], lens [batch] and table [batch columns] are int32 (dx_kernels.h says what they hold).
+struct QkNormRopeTF : TF {
+    bool norm;
+    std::string formula;
+    QkNormRopeTF(bool norm_, std::vector<Param> a, std::vector<Param> r)
+        : norm(norm_), formula(norm_ ? "T5,T6=rotate(W1*T1/rms(T1), W2*T2/rms(T2), positions)" : "T5,T6=rotate(T1, T2, positions)") {
+        name = "qknorm_rope"; metadata.author = "b200"; tftype = "fused"; args = std::move(a); returns = std::move(r);
+    }
+    DX_TF_BOILERPLATE(QkNormRopeTF)
+    int run(Mem &mem, std::string &error) override {
+        const int fi = norm ? 4 : 2, pi = fi + 1;
+        std::vector<std::string> names{args[0].textvalue, args[1].textvalue, args[fi].textvalue, args[pi].textvalue, returns[0].textvalue, returns[1].textvalue};
+        if (norm) { names.push_back(args[2].textvalue); names.push_back(args[3].textvalue); }
+        if (!check_tensors(names, mem, error)) return 1;
+        auto Q = mem.get_tensor(args[0].textvalue), K = mem.get_tensor(args[1].textvalue), F = mem.get_tensor(args[fi].textvalue), P = mem.get_tensor(args[pi].textvalue);
+        auto QO = mem.get_tensor(returns[0].textvalue), KO = mem.get_tensor(returns[1].textvalue);
+        TensorPtr WQ = norm ? mem.get_tensor(args[2].textvalue) : nullptr, WK = norm ? mem.get_tensor(args[3].textvalue) : nullptr;
+        refuse_partitioned(name, {Q, K, F, P, QO, KO, WQ, WK});
+        for (const TensorPtr &t : {K, QO, KO, norm ? WQ : Q, norm ? WK : Q})
+            if (t->shape.dtype != Q->shape.dtype) { error = type_mismatch({Q->shape.dtype, t->shape.dtype}); return 1; }
+        if (Q->shape.dim() != 3 || K->shape.dim() != 3 || Q->shape.shape != QO->shape.shape || K->shape.shape != KO->shape.shape ||
+            Q->shape.shape[0] != K->shape.shape[0] || Q->shape.shape[2] != K->shape.shape[2])
+            throw TensorShapeError(name + ": q and k are [tokens heads head_dim], outputs alike");
+        const int64_t tokens = Q->shape.shape[0], dim = Q->shape.shape[2];
+        if (F->shape.dtype != P_F32 || F->shape.dim() != 1 || (P->shape.dtype != P_I32 && P->shape.dtype != P_I64) || P->shape.size != tokens)
+            throw TensorShapeError(name + ": inv_freq is float32 [rotated/2], positions int32 or int64 [tokens]");
+        if (norm && (WQ->shape.size != dim || WK->shape.size != dim)) throw TensorShapeError(name + ": a weight holds head_dim elements");
+        const double eps = norm ? double(var_f32(pi + 1, mem)) : 0.0;
+        const bool interleaved = var_bool(norm ? pi + 2 : pi + 1);
+        const int64_t qs = Q->shape.shape[1] * dim, ks = K->shape.shape[1] * dim;
+        dx_check(dx_qknorm_rope(Q->dx(), Q->data, qs, Q->shape.shape[1], K->data, ks, K->shape.shape[1], tokens, dim, norm, norm ? WQ->data : nullptr,
+                                norm ? WK->data : nullptr, eps, static_cast<const float *>(F->data), 2 * F->shape.size, interleaved, P->dx(), P->data,
+                                QO->data, qs, KO->data, ks, mem.stream()));
+        return 0;
+    }
+};
+
+// The descriptors of a cache operator: tensors k, v, k_scale, v_scale, then starts, lens, table, by name; `rows` packed rows.
+struct KvOperands {
+    dx_kvcache cache{};
+    dx_kvseqs seqs{};
+    KvOperands(const std::string &op, Mem &mem, const std::vector<std::string> &cache_names, const std::vector<std::string> &seq_names, const std::string &format,
+               int64_t rows) {
+        TensorPtr c[4], s[3];
+        for (int i = 0; i < 4; ++i) c[i] = mem.get_tensor(cache_names[i]);
+        for (int i = 0; i < 3; ++i) s[i] = mem.get_tensor(seq_names[i]);
+        refuse_partitioned(op, {c[0], c[1], c[2], c[3], s[0], s[1], s[2]});
+        if (c[0]->shape.dtype != P_I8 || c[1]->shape.dtype != P_I8 || c[2]->shape.dtype != P_F32 || c[3]->shape.dtype != P_F32)
+            throw std::invalid_argument(op + ": a cache is int8, its scales float32");
+        if (c[0]->shape.dim() != 4 || c[0]->shape.shape != c[1]->shape.shape)
+            throw TensorShapeError(op + ": a cache is [pages kv_heads page_tokens head_dim], keys and values alike");
+        const std::vector<int64_t> &sh = c[0]->shape.shape, scales{sh[0], sh[1]};
+        if (c[2]->shape.shape != scales || c[3]->shape.shape != scales) throw TensorShapeError(op + ": scales are [pages kv_heads]");
+        for (const TensorPtr &t : s)
+            if (t->shape.dtype != P_I32) throw std::invalid_argument(op + ": starts, lens and table are int32");
+        if (s[1]->shape.dim() != 1 || s[2]->shape.dim() != 2 || s[0]->shape.dim() != 1 || s[0]->shape.size != s[1]->shape.size + 1 || s[2]->shape.shape[0] != s[1]->shape.size)
+            throw TensorShapeError(op + ": starts is [batch+1], lens [batch], table [batch columns]");
+        if (format != "int8" && format != "e4m3") throw std::invalid_argument(op + ": the format is int8 or e4m3, not " + format);
+        cache = dx_kvcache{c[0]->data, c[1]->data, static_cast<float *>(c[2]->data), static_cast<float *>(c[3]->data), sh[0], sh[1], sh[2], sh[3],
+                           format == "int8" ? DX_CACHE_I8 : DX_CACHE_E4M3};
+        seqs = dx_kvseqs{static_cast<const int32_t *>(s[0]->data), static_cast<const int32_t *>(s[1]->data), static_cast<const int32_t *>(s[2]->data),
+                         s[1]->shape.size, s[2]->shape.shape[1], rows};
+    }
+};
+std::vector<std::string> texts(const std::vector<Param> &ps, int from, int count) {
+    std::vector<std::string> v;
+    for (int i = from; i < from + count; ++i) v.push_back(ps[i].textvalue);
+    return v;
+}
+
+struct KvCacheWriteTF : TF {
+    std::string formula = "cache[starts,lens,table]=quantise(T1,T2)";
+    KvCacheWriteTF(std::vector<Param> a, std::vector<Param> r) { name = "kvcache_write"; metadata.author = "b200"; tftype = "fused"; args = std::move(a); returns = std::move(r); }
+    DX_TF_BOILERPLATE(KvCacheWriteTF)
+    int run(Mem &mem, std::string &error) override {
+        std::vector<std::string> all = texts(args, 0, 5);
+        for (const auto &n : texts(returns, 0, 4)) all.push_back(n);
+        if (!check_tensors(all, mem, error)) return 1;
+        auto K = mem.get_tensor(args[0].textvalue), V = mem.get_tensor(args[1].textvalue);
+        refuse_partitioned(name, {K, V});
+        if (K->shape.dtype != V->shape.dtype) { error = type_mismatch({K->shape.dtype, V->shape.dtype}); return 1; }
+        if (K->shape.dim() != 3 || K->shape.shape != V->shape.shape) throw TensorShapeError(name + ": keys and values are [rows kv_heads head_dim]");
+        const KvOperands o(name, mem, texts(returns, 0, 4), texts(args, 2, 3), args[5].textvalue, K->shape.shape[0]);
+        if (K->shape.shape[1] != o.cache.kv_heads || K->shape.shape[2] != o.cache.head_dim) throw TensorShapeError(name + ": keys and values of other heads than the cache's");
+        const int64_t stride = K->shape.shape[1] * K->shape.shape[2];
+        dx_check(dx_kvcache_write(K->dx(), K->data, stride, V->data, stride, &o.seqs, &o.cache, nullptr, mem.stream()));
+        return 0;
+    }
+};
+
+struct KvCacheReadTF : TF {
+    std::string formula = "T1,T2=cache[starts,lens,table]";
+    KvCacheReadTF(std::vector<Param> a, std::vector<Param> r) { name = "kvcache_read"; metadata.author = "b200"; tftype = "fused"; args = std::move(a); returns = std::move(r); }
+    DX_TF_BOILERPLATE(KvCacheReadTF)
+    int run(Mem &mem, std::string &error) override {
+        std::vector<std::string> all = texts(args, 0, 7);
+        for (const auto &n : texts(returns, 0, 2)) all.push_back(n);
+        if (!check_tensors(all, mem, error)) return 1;
+        auto K = mem.get_tensor(returns[0].textvalue), V = mem.get_tensor(returns[1].textvalue);
+        refuse_partitioned(name, {K, V});
+        if (K->shape.dtype != V->shape.dtype) { error = type_mismatch({K->shape.dtype, V->shape.dtype}); return 1; }
+        if (K->shape.dim() != 3 || K->shape.shape != V->shape.shape) throw TensorShapeError(name + ": keys and values are [rows kv_heads head_dim]");
+        const KvOperands o(name, mem, texts(args, 0, 4), texts(args, 4, 3), args[7].textvalue, K->shape.shape[0]);
+        if (K->shape.shape[1] != o.cache.kv_heads || K->shape.shape[2] != o.cache.head_dim) throw TensorShapeError(name + ": keys and values of other heads than the cache's");
+        const int64_t stride = K->shape.shape[1] * K->shape.shape[2];
+        dx_check(dx_kvcache_read(K->dx(), &o.seqs, &o.cache, K->data, stride, V->data, stride, nullptr, mem.stream()));
+        return 0;
+    }
+};
+
+struct KvCacheAttentionTF : TF {
+    std::string formula = "T2=softmax(scale*T1@cache.k)@cache.v";
+    KvCacheAttentionTF(std::vector<Param> a, std::vector<Param> r) { name = "kvcache_attention"; metadata.author = "b200"; tftype = "fused"; args = std::move(a); returns = std::move(r); }
+    DX_TF_BOILERPLATE(KvCacheAttentionTF)
+    int run(Mem &mem, std::string &error) override {
+        std::vector<std::string> all = texts(args, 0, 8);
+        all.push_back(returns[0].textvalue);
+        if (!check_tensors(all, mem, error)) return 1;
+        auto Q = mem.get_tensor(args[0].textvalue), O = mem.get_tensor(returns[0].textvalue);
+        refuse_partitioned(name, {Q, O});
+        if (Q->shape.dtype != O->shape.dtype) { error = type_mismatch({Q->shape.dtype, O->shape.dtype}); return 1; }
+        if (Q->shape.dim() != 3 || Q->shape.shape != O->shape.shape) throw TensorShapeError(name + ": queries are [rows q_heads head_dim], the output alike");
+        const KvOperands o(name, mem, texts(args, 1, 4), texts(args, 5, 3), args[11].textvalue, Q->shape.shape[0]);
+        if (Q->shape.shape[2] != o.cache.head_dim) throw TensorShapeError(name + ": queries of another head_dim than the cache's");
+        const double scale = var_f32(8, mem);
+        const int64_t max_new = var_int(9, mem), window = var_int(10, mem), heads = Q->shape.shape[1], stride = heads * Q->shape.shape[2];
+        const size_t need = dx_kvcache_attention_workspace_bytes(Q->dx(), heads, &o.seqs, &o.cache, max_new);
+        void *ws = need ? mem.scratch(need) : nullptr;
+        dx_check(dx_kvcache_attention(Q->dx(), Q->data, stride, heads, &o.seqs, &o.cache, scale, max_new, window, O->data, stride, ws, need, nullptr, mem.stream()));
+        return 0;
+    }
+};
+
 // ---- registration helpers ---------------------------------------------------------------------------------------------------
 Param T(const char *n, uint16_t p = P_ANY) { return Param(n, CAT_TENSOR, p); }
 Param V(const char *n, uint16_t p = P_ANY) { return Param(n, CAT_VAR, p); }
@@ -1083,12 +1218,23 @@ int register_all(TfFactory &f) {
     return 0;
 }
 
-// Ops beyond the reference's table: the single-kernel forms of the RMSNorm and softmax chains.
+// Ops beyond the reference's table: the single-kernel forms of the RMSNorm and softmax chains, and the attention of a layer over a cache.
 int register_fused(TfFactory &f) {
     const uint16_t F4 = P_F64 | P_F32 | P_F16 | P_BF16;
     f.add_tf(std::make_shared<RmsNormTF>(true, PV{T("x", F4), T("weight", F4), V("divisor"), V("eps")}, PV{T("out", F4)}));
     f.add_tf(std::make_shared<RmsNormTF>(false, PV{T("x", F4), V("divisor"), V("eps")}, PV{T("out", F4)}));
     f.add_tf(std::make_shared<SoftmaxTF>(PV{T("x", F4)}, PV{T("out", F4)}));
+    const uint16_t F3 = P_F32 | P_F16 | P_BF16, F16S = P_F16 | P_BF16, IDX = P_I32 | P_I64;
+    f.add_tf(std::make_shared<QkNormRopeTF>(true, PV{T("q", F3), T("k", F3), T("q_weight", F3), T("k_weight", F3), T("inv_freq", P_F32), T("positions", IDX), V("eps"), V("interleaved", P_BOOL)},
+                                            PV{T("q_out", F3), T("k_out", F3)}));
+    f.add_tf(std::make_shared<QkNormRopeTF>(false, PV{T("q", F3), T("k", F3), T("inv_freq", P_F32), T("positions", IDX), V("interleaved", P_BOOL)}, PV{T("q_out", F3), T("k_out", F3)}));
+    f.add_tf(std::make_shared<KvCacheWriteTF>(PV{T("keys", F3), T("values", F3), T("starts", P_I32), T("lens", P_I32), T("table", P_I32), V("format", P_STRING)},
+                                              PV{T("k", P_I8), T("v", P_I8), T("k_scale", P_F32), T("v_scale", P_F32)}));
+    f.add_tf(std::make_shared<KvCacheReadTF>(PV{T("k", P_I8), T("v", P_I8), T("k_scale", P_F32), T("v_scale", P_F32), T("starts", P_I32), T("lens", P_I32), T("table", P_I32), V("format", P_STRING)},
+                                             PV{T("keys", F3), T("values", F3)}));
+    f.add_tf(std::make_shared<KvCacheAttentionTF>(PV{T("q", F16S), T("k", P_I8), T("v", P_I8), T("k_scale", P_F32), T("v_scale", P_F32), T("starts", P_I32), T("lens", P_I32), T("table", P_I32),
+                                                     V("scale"), V("max_new", P_I32), V("window", P_I32), V("format", P_STRING)},
+                                                  PV{T("out", F16S)}));
     return 0;
 }
 
