@@ -103,9 +103,9 @@ template <typename T> struct Eight {
 
 template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_bounds__(CTA) qknorm_rope_kernel(RopeArgs a, int per_block, FastDiv by_heads) {
     extern __shared__ __align__(16) float shared[];
-    // two weights of 16 * LANES, then [per_block][rotated / 2] pairs of cosine and sine
-    float *weights = shared;
-    float2 *cs = reinterpret_cast<float2 *>(shared + 2 * 16 * LANES);
+    // What a lane reads together lies LANES apart in fours, so that the lanes of a team touch different banks: two weights [4][LANES], then
+    // for each token [4][LANES] of two (cosine, sine).
+    float4 *const weights = reinterpret_cast<float4 *>(shared), *const cs = weights + 2 * 4 * LANES;
     griddep_wait_cta();
     const int heads = a.q_heads + a.k_heads, half = a.rotated / 2;
     const int64_t token0 = int64_t(blockIdx.x) * per_block;
@@ -134,14 +134,17 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
     if (a.norm) {
         for (int i = threadIdx.x; i < 2 * a.dim; i += CTA) {
             const bool is_k = i >= a.dim;
-            const int d = i - (is_k ? a.dim : 0);
+            const int d = i - (is_k ? a.dim : 0), chunk = d / 8;
             const T *w = static_cast<const T *>(is_k ? a.kw : a.qw);
-            weights[(is_k ? 16 * LANES : 0) + d] = w ? to_compute(w[d]) : 1.f;
+            // of which unit's first or second chunk it is
+            const bool split = chunk < 2 * rotated_units;
+            const int unit = split ? chunk % rotated_units : chunk / 2, which = split ? chunk / rotated_units : chunk & 1;
+            reinterpret_cast<float *>(weights + ((is_k ? 4 : 0) + 2 * which + d % 8 / 4) * LANES + unit)[d % 4] = w ? to_compute(w[d]) : 1.f;
         }
     }
     for (int i = threadIdx.x; i < tokens * half; i += CTA) {
-        const int t = i / half, f = i - t * half;
-        cs[i] = turn_of(position(a, token0 + t), a.inv_freq[f]);
+        const int t = i / half, f = i - t * half, unit = f / 8, e = f % 8;  // pair f: both orders have eight pairs of a unit in order
+        reinterpret_cast<float2 *>(cs + (t * 4 + e / 2) * LANES + unit)[e & 1] = turn_of(position(a, token0 + t), a.inv_freq[f]);
     }
     __syncthreads();
     // every thread of a warp takes the same number of turns: the sums are warp shuffles
@@ -163,10 +166,10 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float r = 1.f / sqrtf(sum / float(a.dim) + a.eps);
-            const float *w = weights + (is_q ? 0 : 16 * LANES);
+            const float4 *w = weights + (is_q ? 0 : 4 * LANES) + u;
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                const float4 w0 = *reinterpret_cast<const float4 *>(w + (has0 ? first : 0) * 8 + e), w1 = *reinterpret_cast<const float4 *>(w + (has1 ? second : 0) * 8 + e);
+                const float4 w0 = w[e / 4 * LANES], w1 = w[(2 + e / 4) * LANES];
                 const float m0[4] = {w0.x, w0.y, w0.z, w0.w}, m1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
@@ -176,13 +179,13 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
             }
         }
         if (!live) continue;
-        const float2 *turn = cs + t * half;
+        const float4 *turn = cs + t * 4 * LANES + u;
         if constexpr (INTERLEAVED) {
-            auto rotate = [&](float (&y)[8], int chunk) {
+            auto rotate = [&](float (&y)[8], int chunk, int from) {
                 if (chunk * 8 >= a.rotated) return;
 #pragma unroll
                 for (int p = 0; p < 4; p += 2) {
-                    const float4 c = *reinterpret_cast<const float4 *>(turn + chunk * 4 + p);
+                    const float4 c = turn[(from + p / 2) * LANES];
                     const float s = y[2 * p], v = y[2 * p + 1], z = y[2 * p + 2], w = y[2 * p + 3];
                     y[2 * p] = s * c.x - v * c.y;
                     y[2 * p + 1] = v * c.x + s * c.y;
@@ -190,12 +193,12 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
                     y[2 * p + 3] = w * c.z + z * c.w;
                 }
             };
-            rotate(y0, first);
-            rotate(y1, second);
+            rotate(y0, first, 0);
+            rotate(y1, second, 2);
         } else if (apart) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const float4 c = *reinterpret_cast<const float4 *>(turn + u * 8 + e);
+                const float4 c = turn[e / 2 * LANES];
                 const float s = y0[e], v = y1[e], z = y0[e + 1], w = y1[e + 1];
                 y0[e] = s * c.x - v * c.y;
                 y1[e] = v * c.x + s * c.y;
@@ -218,9 +221,9 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
 template <typename T, int LANES> void launch_lanes(const RopeArgs &a, cudaStream_t st) {
     // enough blocks for every SM's eight, then up to sixteen tokens each
     int per_block = 1;
-    while (per_block < 16 && a.tokens > int64_t(sm_count()) * 8 * per_block) per_block *= 2;
+    while (per_block < (LANES > 16 ? 8 : 16) && a.tokens > int64_t(sm_count()) * 8 * per_block) per_block *= 2;
     const unsigned grid = unsigned((a.tokens + per_block - 1) / per_block);
-    const size_t smem = 2 * 16 * LANES * sizeof(float) + size_t(per_block) * (a.rotated / 2) * sizeof(float2);
+    const size_t smem = size_t(2 + per_block) * 4 * LANES * sizeof(float4);
     const FastDiv by_heads = make_fastdiv(unsigned(a.q_heads + a.k_heads));
     if (a.interleaved) launch_pdl(qknorm_rope_kernel<T, LANES, true>, dim3(grid), dim3(CTA), smem, st, a, per_block, by_heads);
     else launch_pdl(qknorm_rope_kernel<T, LANES, false>, dim3(grid), dim3(CTA), smem, st, a, per_block, by_heads);
