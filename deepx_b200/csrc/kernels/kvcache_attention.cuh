@@ -47,7 +47,7 @@ template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_
 // largest is still a half.
 constexpr float LAG = 8.f, UP = 7.f;
 constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr int JOIN_CTA = 512, JOIN_ROWS = 16;
+constexpr int JOIN_CTA = 512;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 // 2^x, off by 2^-22 of it; what is below 2^-126 becomes zero (without that, every call would be four instructions instead of one).
@@ -63,67 +63,131 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 // Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
 // of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
-// with its item and does not end it part 2i + 1.  Sixteen warps share sixteen of the item's rows; the warps of a row share its parts.
+// with its item and does not end it part 2i + 1.  Two cases.  Items of many rows are as a rule split in a few parts, and there are many
+// of them: a warp takes two rows and has every load of theirs in flight at once, without waiting for a maximum.  (With the other way,
+// of 2 x 4096 tokens, 32 heads of 128, the join was 30 us of 427.)  Otherwise sixteen warps take sixteen of the item's rows at a time, the
+// warps of a row share its parts, and FLIGHT of a warp's parts are on their way at once.
+__host__ __device__ constexpr int join_rows(int rows) { return rows > 128 ? 32 : 16; }  // of a block
+
 template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
-    constexpr int V = DP / 32, VW = V < 4 ? V : 4, PART = ROWS * DP + 2 * ROWS;
+    constexpr int V = DP / 32, VW = V < 4 ? V : 4, PART = ROWS * DP + 2 * ROWS, STEP = 16, FEW = 4;
+    constexpr int FLIGHT = ROWS > 128 ? 2 : 8;
     __shared__ float sh[JOIN_CTA / 32][DP];
     griddep_wait_cta();
     const Join j = reinterpret_cast<const Join *>(a.ws)[blockIdx.x];
-    const int row0 = blockIdx.y * JOIN_ROWS, rows = min(j.rows - row0, JOIN_ROWS);
-    if (j.parts == 0 || rows <= 0) return;
+    const int first = blockIdx.y * join_rows(ROWS), last = min(j.rows, first + join_rows(ROWS));
+    if (j.parts == 0 || first >= last) return;
     const float *parts = reinterpret_cast<const float *>(a.ws + gridDim.x * sizeof(Join));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int each = rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;  // warps of a row
-    const int r = warp / each, row = row0 + r, sub = warp % each;
     auto at = [&](int p) { return parts + (int64_t(blockIdx.x - 1 + p) * 2 + (p == 0 ? 1 : 0)) * PART; };
-    float acc[V] = {}, sum = 0.f;
-    if (r < rows) {
-        float top = NEG_INF;
-        for (int p0 = lane; p0 < j.parts; p0 += 128) {
-            float m[4];
+    auto out_row = [&](int row) {
+        const int fr = j.first_row + row, i = fr / a.group;
+        return static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
+    };
+    if constexpr (ROWS > 128) {
+        if (j.parts <= FEW) {
+            constexpr int EACH = join_rows(ROWS) / 16;
+            Pack<float, VW> x[EACH][FEW][V / VW];
+            float m[EACH][FEW], l[EACH][FEW];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) m[k] = p0 + 32 * k < j.parts ? at(p0 + 32 * k)[ROWS * DP + row] : NEG_INF;
-            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+            for (int k = 0; k < EACH; ++k) {
+                const int row = first + k * 16 + warp;
+#pragma unroll
+                for (int p = 0; p < FEW; ++p) {
+                    m[k][p] = NEG_INF, l[k][p] = 0.f;
+                    if (row < last && p < j.parts) {
+                        m[k][p] = at(p)[ROWS * DP + row];
+                        l[k][p] = at(p)[ROWS * DP + ROWS + row];
+#pragma unroll
+                        for (int e = 0; e < V / VW; ++e) x[k][p][e] = reinterpret_cast<const Pack<float, VW> *>(at(p) + row * DP + lane * V)[e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                const int row = first + k * 16 + warp;
+                if (row >= last) continue;
+                float top = m[k][0], sum = 0.f, acc[V] = {};
+#pragma unroll
+                for (int p = 1; p < FEW; ++p) top = fmaxf(top, m[k][p]);
+                const float base = top == NEG_INF ? 0.f : top;
+#pragma unroll
+                for (int p = 0; p < FEW; ++p) {
+                    const float w = l[k][p] * exp2_approx(m[k][p] - base);
+                    sum += w;
+                    if (p < j.parts && w != 0.f)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[e] += w * x[k][p][e / VW].v[e % VW];
+                }
+                const float by = sum == 0.f ? 0.f : 1.f / sum;
+                T *out = out_row(row) + lane * V;
+                if (lane * V >= c.dim) continue;  // dim is a multiple of 16, V a power of two up to 4: the lane's values are all of the row or none
+                Pack<T, V> o;
+#pragma unroll
+                for (int e = 0; e < V; ++e) o.v[e] = from_compute<T>(acc[e] * by);
+                if (reinterpret_cast<uintptr_t>(out) % sizeof(o) == 0) *reinterpret_cast<Pack<T, V> *>(out) = o;
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e) out[e] = o.v[e];
+            }
+            return;
         }
+    }
+#pragma unroll 1
+    for (int row0 = first; row0 < last; row0 += STEP) {
+        const int rows = min(last - row0, STEP);
+        const int each = rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;  // warps of a row
+        const int r = warp / each, row = row0 + r, sub = warp % each;
+        float acc[V] = {}, sum = 0.f;
+        if (r < rows) {
+            float top = NEG_INF;
+            for (int p0 = lane; p0 < j.parts; p0 += 128) {
+                float m[4];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float base = top == NEG_INF ? 0.f : top;
-        for (int p0 = 0; p0 < j.parts; p0 += 32) {
-            float w = 0.f;
-            if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
-            float s = w;
+                for (int k = 0; k < 4; ++k) m[k] = p0 + 32 * k < j.parts ? at(p0 + 32 * k)[ROWS * DP + row] : NEG_INF;
+                top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+            }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            sum += s;
-            const int n = min(32, j.parts - p0);
-            for (int p1 = sub; p1 < n; p1 += 8 * each) {  // eight loads in flight
-                Pack<float, VW> x[8][V / VW];
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float base = top == NEG_INF ? 0.f : top;
+            for (int p0 = 0; p0 < j.parts; p0 += 32) {
+                float w = 0.f;
+                if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
+                float s = w;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                sum += s;
+                const int n = min(32, j.parts - p0);
+                for (int p1 = sub; p1 < n; p1 += FLIGHT * each) {
+                    Pack<float, VW> x[FLIGHT][V / VW];
 #pragma unroll
-                    for (int e = 0; e < V / VW; ++e)
-                        if (p1 + k * each < n) x[k][e] = reinterpret_cast<const Pack<float, VW> *>(at(p0 + p1 + k * each) + row * DP + lane * V)[e];
+                    for (int k = 0; k < FLIGHT; ++k)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float by = __shfl_sync(0xffffffffu, w, min(p1 + k * each, 31));
-                    if (p1 + k * each >= n || by == 0.f) continue;
+                        for (int e = 0; e < V / VW; ++e)
+                            if (p1 + k * each < n) x[k][e] = reinterpret_cast<const Pack<float, VW> *>(at(p0 + p1 + k * each) + row * DP + lane * V)[e];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) acc[e] += by * x[k][e / VW].v[e % VW];
+                    for (int k = 0; k < FLIGHT; ++k) {
+                        const float by = __shfl_sync(0xffffffffu, w, min(p1 + k * each, 31));
+                        if (p1 + k * each >= n || by == 0.f) continue;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[e] += by * x[k][e / VW].v[e % VW];
+                    }
                 }
             }
         }
-    }
 #pragma unroll
-    for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
-    __syncthreads();
-    if (r >= rows || sub) return;
-    const float by = sum == 0.f ? 0.f : 1.f / sum;
-    const int fr = j.first_row + row, i = fr / a.group;
-    T *out = static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
-    for (int d = lane; d < c.dim; d += 32) {
-        float v = 0.f;
-        for (int w = 0; w < each; ++w) v += sh[warp + w][d];
-        out[d] = from_compute<T>(v * by);
+        for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
+        __syncthreads();
+        if (r < rows && sub == 0) {
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            T *out = out_row(row);
+            for (int d = lane; d < c.dim; d += 32) {
+                float v = 0.f;
+                for (int w = 0; w < each; ++w) v += sh[warp + w][d];
+                out[d] = from_compute<T>(v * by);
+            }
+        }
+        __syncthreads();
     }
 }
 #endif

@@ -804,7 +804,7 @@ template <typename T, int FMT, int DP> int launch(const Attn &a, const Cache &c,
     if (int e = check_launch("kvcache_attention (plan)")) return e;
     launch_pdl(tiles_kernel<T, FMT, DP>, dim3(grid), dim3(THREADS), C::SMEM, st, a, c, s, plan);
     if (int e = check_launch("kvcache_attention (tiles)")) return e;
-    launch_pdl(join_kernel<T, DP, ITEM_ROWS>, dim3(grid, ITEM_ROWS / JOIN_ROWS), dim3(JOIN_CTA), 0, st, a, c);
+    launch_pdl(join_kernel<T, DP, ITEM_ROWS>, dim3(grid, ITEM_ROWS / join_rows(ITEM_ROWS)), dim3(JOIN_CTA), 0, st, a, c);
     return check_launch("kvcache_attention (join)");
 }
 
