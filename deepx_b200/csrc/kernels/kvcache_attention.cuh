@@ -63,13 +63,14 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 // Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
 // of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
-// with its item and does not end it part 2i + 1.  Two cases.  Items of many rows are as a rule split in a few parts, and there are many
-// of them: a warp takes two rows and has every load of theirs in flight at once, without waiting for a maximum.  (With the other way,
-// of 2 x 4096 tokens, 32 heads of 128, the join was 30 us of 427.)  Otherwise sixteen warps take sixteen of the item's rows at a time, the
-// warps of a row share its parts, and FLIGHT of a warp's parts are on their way at once.
+// with its item and does not end it part 2i + 1.  What it costs is waiting for memory, one load after the other, so there are two ways.
+// Up to FEW parts: a warp takes a row (two where items have many) and has every load of it in flight at once, without waiting for a
+// maximum.  (With the other way alone the join of 64 single tokens after 300 to 8192, 8 key heads of 128, took 13 us in place of 7, that
+// of 2 x 4096 tokens, 32 heads, 30 in place of 14.)  More: sixteen warps take sixteen of the item's rows at a time, the warps of a row
+// share its parts, and FLIGHT of a warp's parts are on their way at once.
 __host__ __device__ constexpr int join_rows(int rows) { return rows > 128 ? 32 : 16; }  // of a block
 
-template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_CTA) join_kernel(Attn a, Cache c) {
+template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_CTA, DP > 128 ? 1 : 2) join_kernel(Attn a, Cache c) {
     constexpr int V = DP / 32, VW = V < 4 ? V : 4, PART = ROWS * DP + 2 * ROWS, STEP = 16, FEW = 4;
     constexpr int FLIGHT = ROWS > 128 ? 2 : 8;
     __shared__ float sh[JOIN_CTA / 32][DP];
@@ -84,54 +85,52 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
         const int fr = j.first_row + row, i = fr / a.group;
         return static_cast<T *>(a.out) + (j.row0 + i) * a.out_stride + int64_t(j.head * a.group + fr - i * a.group) * c.dim;
     };
-    if constexpr (ROWS > 128) {
-        if (j.parts <= FEW) {
-            constexpr int EACH = join_rows(ROWS) / 16;
-            Pack<float, VW> x[EACH][FEW][V / VW];
-            float m[EACH][FEW], l[EACH][FEW];
+    if (j.parts <= FEW) {
+        constexpr int EACH = join_rows(ROWS) / 16;
+        Pack<float, VW> x[EACH][FEW][V / VW];
+        float m[EACH][FEW], l[EACH][FEW];
 #pragma unroll
-            for (int k = 0; k < EACH; ++k) {
-                const int row = first + k * 16 + warp;
+        for (int k = 0; k < EACH; ++k) {
+            const int row = first + k * 16 + warp;
 #pragma unroll
-                for (int p = 0; p < FEW; ++p) {
-                    m[k][p] = NEG_INF, l[k][p] = 0.f;
-                    if (row < last && p < j.parts) {
-                        m[k][p] = at(p)[ROWS * DP + row];
-                        l[k][p] = at(p)[ROWS * DP + ROWS + row];
+            for (int p = 0; p < FEW; ++p) {
+                m[k][p] = NEG_INF, l[k][p] = 0.f;
+                if (row < last && p < j.parts) {
+                    m[k][p] = at(p)[ROWS * DP + row];
+                    l[k][p] = at(p)[ROWS * DP + ROWS + row];
 #pragma unroll
-                        for (int e = 0; e < V / VW; ++e) x[k][p][e] = reinterpret_cast<const Pack<float, VW> *>(at(p) + row * DP + lane * V)[e];
-                    }
+                    for (int e = 0; e < V / VW; ++e) x[k][p][e] = reinterpret_cast<const Pack<float, VW> *>(at(p) + row * DP + lane * V)[e];
                 }
             }
-#pragma unroll
-            for (int k = 0; k < EACH; ++k) {
-                const int row = first + k * 16 + warp;
-                if (row >= last) continue;
-                float top = m[k][0], sum = 0.f, acc[V] = {};
-#pragma unroll
-                for (int p = 1; p < FEW; ++p) top = fmaxf(top, m[k][p]);
-                const float base = top == NEG_INF ? 0.f : top;
-#pragma unroll
-                for (int p = 0; p < FEW; ++p) {
-                    const float w = l[k][p] * exp2_approx(m[k][p] - base);
-                    sum += w;
-                    if (p < j.parts && w != 0.f)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) acc[e] += w * x[k][p][e / VW].v[e % VW];
-                }
-                const float by = sum == 0.f ? 0.f : 1.f / sum;
-                T *out = out_row(row) + lane * V;
-                if (lane * V >= c.dim) continue;  // dim is a multiple of 16, V a power of two up to 4: the lane's values are all of the row or none
-                Pack<T, V> o;
-#pragma unroll
-                for (int e = 0; e < V; ++e) o.v[e] = from_compute<T>(acc[e] * by);
-                if (reinterpret_cast<uintptr_t>(out) % sizeof(o) == 0) *reinterpret_cast<Pack<T, V> *>(out) = o;
-                else
-#pragma unroll
-                    for (int e = 0; e < V; ++e) out[e] = o.v[e];
-            }
-            return;
         }
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int row = first + k * 16 + warp;
+            if (row >= last) continue;
+            float top = m[k][0], sum = 0.f, acc[V] = {};
+#pragma unroll
+            for (int p = 1; p < FEW; ++p) top = fmaxf(top, m[k][p]);
+            const float base = top == NEG_INF ? 0.f : top;
+#pragma unroll
+            for (int p = 0; p < FEW; ++p) {
+                const float w = l[k][p] * exp2_approx(m[k][p] - base);
+                sum += w;
+                if (p < j.parts && w != 0.f)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += w * x[k][p][e / VW].v[e % VW];
+            }
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            T *out = out_row(row) + lane * V;
+            if (lane * V >= c.dim) continue;  // dim is a multiple of 16, V a power of two up to 4: the lane's values are all of the row or none
+            Pack<T, V> o;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o.v[e] = from_compute<T>(acc[e] * by);
+            if (reinterpret_cast<uintptr_t>(out) % sizeof(o) == 0) *reinterpret_cast<Pack<T, V> *>(out) = o;
+            else
+#pragma unroll
+                for (int e = 0; e < V; ++e) out[e] = o.v[e];
+        }
+        return;
     }
 #pragma unroll 1
     for (int row0 = first; row0 < last; row0 += STEP) {
