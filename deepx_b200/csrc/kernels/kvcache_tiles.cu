@@ -639,8 +639,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     } else if (warp < 8 + 2 * CONVERTERS) {
         // ===== codes into halfs: keys or values =====
         const bool is_v = warp >= 8 + CONVERTERS;
-        const int sub = (warp - 8) % CONVERTERS;
+        const int sub = (warp - 7) % CONVERTERS;  // the first warp, which has the steps' info to see to as well, is not the one with a turn more
         constexpr int PER_ROW = DP / 16, WARP_ROWS = 32 / PER_ROW, UNITS = KEYS / WARP_ROWS, TURNS = (UNITS + CONVERTERS - 1) / CONVERTERS;
+        auto has = [&](int turn) { return turn + 1 < TURNS || sub < UNITS - CONVERTERS * (TURNS - 1); };  // the same in all threads of the warp
         // In turn i the warp takes rows WARP_ROWS * (sub + CONVERTERS * i)..., a thread sixteen codes, chunk ch of one row: eight lanes in a row are
         // four chunks of an even and an odd row, whose halfs go to different banks.
         const int ch = DP == 64 ? lane & 3 : (lane & 3) | (lane >> 3 & 1) << 2;
@@ -673,17 +674,19 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 return number < 0 ? int64_t(-1) : ((int64_t(number) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim;
             };
             uint4 x[TURNS];
-            auto load = [&](int64_t offsets, int left, int turn) {
+            // Rows from p.it.hi on in a group that is there are read like the others: no row sees them.
+            auto load = [&](int64_t offsets, int turn) {
                 const int row = WARP_ROWS * (sub + CONVERTERS * turn) + r0;
                 const int64_t off = __shfl_sync(0xffffffffu, offsets, (row >> 4) % GROUPS);  // a warp's rows of a turn are of one group
-                if (off < 0 || row >= left || row >= KEYS || !in_dim) return make_uint4(0, 0, 0, 0);
+                if (off < 0 || !in_dim) return make_uint4(0, 0, 0, 0);
                 return *reinterpret_cast<const uint4 *>(codes + off + (row & 15) * c.dim);
             };
             int32_t number = page_of(0), next = page_of(1);
             {
                 const int64_t offsets = begin_of(0, number);
 #pragma unroll
-                for (int turn = 0; turn < TURNS; ++turn) x[turn] = load(offsets, p.it.hi - p.it.lo - p.step0 * KEYS, turn);
+                for (int turn = 0; turn < TURNS; ++turn)
+                    if (has(turn)) x[turn] = load(offsets, turn);
             }
             float v_ref = 0.f;
             for (int step = 0; step < p.steps; ++step, ++n) {
@@ -695,22 +698,20 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     vs = c.v_scale[int64_t(number) * c.heads + p.head];
                 }
                 const int64_t offsets = begin_of(step + 1, next);
-                const int left = p.it.hi - p.it.lo - (p.step0 + step + 1) * KEYS;
                 if (!warp_wait(is_v ? v_empty(stage) : k_empty(stage), ((n / STAGES) & 1) ^ 1, abort_flag, S_ROOM)) { ok = false; break; }
                 const uint32_t dst = smem + stage * C::OPERAND;
 #pragma unroll
                 for (int turn = 0; turn < TURNS; ++turn) {
+                    if (!has(turn)) continue;
                     const uint32_t w[4] = {x[turn].x, x[turn].y, x[turn].z, x[turn].w};
-                    x[turn] = load(offsets, left, turn);
+                    x[turn] = load(offsets, turn);
                     uint32_t h[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) decode4<FMT, true>(w[e], h[2 * e], h[2 * e + 1]);
                     const int row = WARP_ROWS * (sub + CONVERTERS * turn) + r0;
                     const uint32_t at0 = dst + row * 128 + (((ch & 3) * 2 ^ (row & 7)) << 4);
-                    if (row < KEYS) {
-                        sts128(at0, h[0], h[1], h[2], h[3]);
-                        sts128(at0 ^ 16, h[4], h[5], h[6], h[7]);
-                    }
+                    sts128(at0, h[0], h[1], h[2], h[3]);
+                    sts128(at0 ^ 16, h[4], h[5], h[6], h[7]);
                 }
                 if (warp == 8) {
                     float top = vs;
@@ -723,7 +724,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     if (lane < GROUPS) {
                         f.k[lane] = fmaxf(ks, 7.8886091e-31f);  // 2^-100: a factor of zero would make a hidden score not a number
                         f.v_log[lane] = __log2f(unit);
-                        f.v_inv[lane] = __frcp_rn(unit);
+                        f.v_inv[lane] = __fdividef(1.f, unit);
                     }
                     if (lane == 0) {
                         f.turn = v_ref == 0.f || v_ref == ref ? 1.f : __fdividef(v_ref, ref);
