@@ -13,6 +13,11 @@
 // block takes an equal piece of it, whatever the lengths are (they are known on the device alone).  A piece may begin or end
 // inside an item (one tile of rows, one head); such items' parts meet in the workspace and a second kernel joins them, always
 // in the order of the keys: the same bits every time.
+//
+// Measured (B200, 32 query and 8 key heads of 128): one token after 262100, int8, f16: 95 to 102 us, 5.3 to 5.6 TB/s of the copy's 6.5; 64 single
+// tokens after 300 to 8192, e4m3, bf16: 72 us, 4.6 TB/s, 7 of them the join; one token after 1500: 11 us on the device, two launches and
+// the chain from the lengths to the pages to the keys.  More than the copy's time goes into each block's way to its first keys, the
+// joints between items and turning codes into halfs with twelve warps an SM.
 #include "kvcache_attention.cuh"
 
 namespace dx {
@@ -24,7 +29,7 @@ constexpr int MIN_TOKENS = 128;  // of a block: fewer would cost more in joining
 
 // DP: the head's dimensions, padded; NB: blocks of eight rows of an item; WT: tokens a warp takes at a time, of one page.  What a turn of
 // the loop costs besides its tokens (addresses, the wait, the vote on the maximum) is half of it at 16 tokens, so 32 are taken where the
-// pages and the registers allow it (one token after 262100: 110 us with 16, 102 us with 32).
+// pages and the registers allow it (one token after 262100: 110 us with 16, 102 us with 32, on one card).
 template <int DP, int NB, int WT> struct Cfg {
     static constexpr int ROWS = 8 * NB, STEP = WARPS * WT;
     static constexpr int STAGES = WT == 32 ? (DP == 64 ? 3 : 2) : DP == 64 ? 4 : 3;
@@ -581,8 +586,11 @@ template <int DP> size_t workspace_of() {
 }
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 size_t workspace(int dim) { return dim <= 64 ? workspace_of<64>() : dim <= 128 ? workspace_of<128>() : workspace_of<256>(); }
-// Whether a call goes to the tiles of 128 rows: as soon as a sequence may have more rows than one item here.
-bool by_tiles(const Cache &c, int64_t rows) { return c.dim <= 128 && rows > 16; }
+// Whether a call goes to the tiles of 128 rows, whose time hardly depends on the rows: here every sixteen rows of a sequence and key head
+// read its cache again.  64 sequences of 4096 tokens, 8 key heads, here against the tiles: 32 rows of 128 dimensions 265 us against 385,
+// 48 rows 387 against 387, 64 rows 506 against 390; of 64 dimensions 64 rows 337 against 369, 96 rows 502 against 371.  (Eight
+// sequences: 48 rows of 128 dimensions 62 against 51 us, 64 rows of 64 52 against 48.)
+bool by_tiles(const Cache &c, int64_t rows) { return c.dim <= 128 && rows > (c.dim <= 64 ? 64 : 32); }
 // The most rows of a sequence that share a key head, as far as the caller says.
 int64_t rows_of(int64_t q_heads, const Cache &c, const Seqs &s, int64_t max_new) {
     return (max_new > 0 && max_new < s.rows ? max_new : s.rows) * (q_heads / c.heads);

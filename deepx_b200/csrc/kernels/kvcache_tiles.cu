@@ -5,9 +5,9 @@
 //     S = Q K^T          128 x 64, into one of the tile's two places in TMEM;  Q, K halfs in shared memory
 //     P = 2^(c S - m)    a thread has a row; halfs, over S's place
 //     O = O + P V        128 x dim, in TMEM, P from TMEM;                      V halfs in shared memory
-// The scores are issued two steps ahead, so a tile's softmax finds the next ones ready when it is done with the last: with one place
-// for them it waited a third of the time.  512 multiply-adds go with each exponential at 128 dimensions: 64 keys of both tiles cost 1024
-// cycles of the tensor cores and 1024 of the exponential unit, so both bound this kernel; what is neither stays off their threads.
+// The scores are issued two steps ahead, so a tile's softmax finds the next ones ready when it is done with the last.  512 multiply-adds
+// go with each exponential at 128 dimensions: 64 keys of both tiles cost 1024 cycles of the tensor cores and 1024 of the exponential
+// unit, so both would bound a perfect kernel; what is neither stays off their threads.
 //
 // Roles (16 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each; 8-10 turn the codes of K into halfs, 11-13 those of V
 // (sixteen a thread and turn, loaded a step ahead); a thread of warp 14 and one of 15 issue a tile's products each.  Codes become halfs
@@ -15,9 +15,16 @@
 // the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
 // scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
 //
+// Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 401 us with the plan and the join (14 us), 686 TFLOP/s,
+// 0.43 of a large matrix product's rate; 12 sequences of 1 to 700 new tokens up to 5000, 14 and 2 heads of 64: 91 us.  A step of 64 keys takes
+// about 2800 cycles: 1300 the exponentials and weights of a row, 560 its maximum, 380 and 270 the waits before and after, while the first
+// converter's way through a step is nearly as long (with the exponentials left out the kernel waits for keys and gains 4 %, with the
+// conversion left out 2 %).  Not taken, as slower: two threads a row (16 softmax warps of 80 registers: 520 us), the tiles in turns, loading
+// the next scores early.
+//
 // The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it, where an
-// item counts OVERHEAD steps more than it has (its queries, its way out; without that the blocks of a prompt's first rows, whose items
-// have few steps, took twice the others' time); items that more than one block works on are joined as in kvcache_attention.cu.
+// item counts OVERHEAD steps more than it has (its queries, its way out: about 10,000 cycles; without that the blocks of a prompt's first
+// rows, whose items have few steps, took twice the others' time); items that more than one block works on are joined as in kvcache_attention.cu.
 //
 // Every wait is bounded by a clock; when one runs out a status word is set (dx_kvcache_status), all roles leave, TMEM is freed.
 #include <mutex>
@@ -657,17 +664,16 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             if (p.steps == 0) continue;
             // lane g of a warp (mod GROUPS) knows group g of a step: its page, and where its codes begin (-1: nowhere)
             const int32_t *table = s.table + int64_t(p.it.b) * s.cols;
-            auto page_of = [&](int step) {
+            // A page's number is asked for a step before it is looked at: nothing waits for it.
+            auto entry_of = [&](int step) {
                 const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
-                int32_t number = -1;
-                if (step < p.steps && j < p.it.hi) {
-                    number = table[j >> c.page_shift];
-                    if (number < 0 || number >= c.pages) {
-                        if (warp == 8 && lane < GROUPS) raise(a.flag, FLAG_PAGE);
-                        number = -1;
-                    }
-                }
-                return number;
+                return step < p.steps && j < p.it.hi ? table[j >> c.page_shift] : -1;
+            };
+            auto page_of = [&](int step, int32_t entry) {
+                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
+                if (uint32_t(entry) < uint64_t(c.pages)) return entry;
+                if (warp == 8 && lane < GROUPS && step < p.steps && j < p.it.hi) raise(a.flag, FLAG_PAGE);
+                return -1;
             };
             auto begin_of = [&](int step, int32_t number) {
                 const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
@@ -681,22 +687,29 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 if (off < 0 || !in_dim) return make_uint4(0, 0, 0, 0);
                 return *reinterpret_cast<const uint4 *>(codes + off + (row & 15) * c.dim);
             };
-            int32_t number = page_of(0), next = page_of(1);
+            int32_t entry = entry_of(2), number = page_of(0, entry_of(0)), next = page_of(1, entry_of(1));
             {
                 const int64_t offsets = begin_of(0, number);
 #pragma unroll
                 for (int turn = 0; turn < TURNS; ++turn)
                     if (has(turn)) x[turn] = load(offsets, turn);
             }
+            // The scales of a step's groups, like its codes, a step ahead.
+            float ks_next = 1.f, vs_next = 0.f;
+            auto scales_of = [&](int32_t of) {
+                ks_next = 1.f, vs_next = 0.f;
+                if (warp == 8 && of >= 0) {
+                    ks_next = c.k_scale[int64_t(of) * c.heads + p.head];
+                    vs_next = c.v_scale[int64_t(of) * c.heads + p.head];
+                }
+            };
+            scales_of(number);
             float v_ref = 0.f;
             for (int step = 0; step < p.steps; ++step, ++n) {
                 const int stage = n % STAGES;
-                float ks = 1.f, vs = 0.f;
                 const bool there = number >= 0;
-                if (warp == 8 && there) {
-                    ks = c.k_scale[int64_t(number) * c.heads + p.head];
-                    vs = c.v_scale[int64_t(number) * c.heads + p.head];
-                }
+                const float ks = ks_next, vs = vs_next;
+                scales_of(next);
                 const int64_t offsets = begin_of(step + 1, next);
                 if (!warp_wait(is_v ? v_empty(stage) : k_empty(stage), ((n / STAGES) & 1) ^ 1, abort_flag, S_ROOM)) { ok = false; break; }
                 const uint32_t dst = smem + stage * C::OPERAND;
@@ -736,7 +749,8 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 fence_async_smem();
                 mbar_arrive(is_v ? v_full(stage) : k_full(stage));
                 number = next;
-                next = page_of(step + 2);
+                next = page_of(step + 2, entry);
+                entry = entry_of(step + 3);
             }
         }
     } else if (elect_one()) {

