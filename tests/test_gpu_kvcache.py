@@ -269,6 +269,26 @@ def test_attention_of_a_mixed_batch(TF, q_heads, kv_heads, dim, page):
     check_attention(TF, b, b.rand(b.rows, q_heads, dim, dtype=torch.bfloat16), dim ** -0.5, max_new=700)
 
 
+@pytest.mark.parametrize("dim,group", [(128, 4), (64, 8), (96, 1), (64, 1)])
+def test_attention_of_many_short_sequences(TF, dim, group):
+    """Short sequences with few new tokens each, without a hint of how few, so that they go the prompts' way too: rows that see nothing,
+    one tile of rows or hardly any of it, a step or two of keys; and with the hint, the other way."""
+    lens = [0, 1, 2, 15, 16, 17, 63, 64, 65, 128, 200, 129, 31] * 4
+    new = [2, 1, 3, 1, 16, 5, 1, 2, 33, 1, 64, 4, 0] * 4
+    b = P.Batch(26, lens, new, 2, dim, 16, "int8", extra_rows=3).fill(lens)
+    Q = b.rand(b.rows, 2 * group, dim, dtype=torch.float16)
+    for hint in (0, max(new)):
+        check_attention(TF, b, Q, dim ** -0.5, max_new=hint)
+
+
+@pytest.mark.parametrize("dim,new", [(128, 8), (128, 9), (64, 16), (64, 17), (96, 8), (80, 9)])
+def test_attention_where_the_ways_part(TF, dim, new):
+    """Four rows for each new token: the last number that goes the way of few rows, the first that goes the prompts' way."""
+    lens = [500, 40, new]
+    b = P.Batch(27, lens, [new] * 3, 1, dim, 64, "e4m3").fill(lens)
+    check_attention(TF, b, b.rand(b.rows, 4, dim, dtype=torch.bfloat16), dim ** -0.5, max_new=new)
+
+
 def test_attention_many_sequences(TF):
     """More sequences than a block has threads, of very different lengths, some empty."""
     lens = [(37 * i) % 211 for i in range(700)]
