@@ -6,9 +6,9 @@
 // works them out once into shared memory: position * inv_freq is a float64 product (a float32 one is off by a tenth of a
 // radian at a position of a million), reduced to a fraction of a turn there and turned into sine and cosine in float32.
 //
-// Measured (B200, inputs of other passes in between): 16384 tokens of 32 + 8 heads of 128, bf16: 76 us, 4.4 TB/s of the copy's 6.5; what
-// is above the copy's time is the wait between a head's loads and the sum of its squares, which as many rows in flight as registers
-// allow do not hide.  64 tokens: 3.6 us on the device, a launch's latency.
+// Measured (B200, inputs of other passes in between): 16384 tokens of 32 + 8 heads of 128, bf16: 62.9 us, 5.3 TB/s of the copy's 6.5.  A row's
+// loads come while the row before is worked on (76 -> 71 us, with the short root), and two values are rounded with one instruction
+// (71 -> 63 us): issue slots count here as much as bytes.  64 tokens: 3.6 us on the device, a launch's latency.
 #include "common.cuh"
 
 namespace dx {
@@ -93,16 +93,19 @@ template <typename T> struct Eight {
 #pragma unroll
         for (int i = 0; i < P; ++i) p[i] = ld_stream<T, N>(x + i * N);
     }
-    __device__ __forceinline__ void load_weight(const T *x) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) p[i] = ld_cached<T, N>(x + i * N);
-    }
     __device__ __forceinline__ void store(T *x) const {
 #pragma unroll
         for (int i = 0; i < P; ++i) st_stream<T, N>(x + i * N, p[i]);
     }
     __device__ __forceinline__ float get(int e) const { return to_compute(p[e / N].v[e % N]); }
-    __device__ __forceinline__ void set(int e, float f) { p[e / N].v[e % N] = from_compute<T>(f); }
+    __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {  // two at a time: one conversion
+            if constexpr (std::is_same<T, bf16>::value) *reinterpret_cast<__nv_bfloat162 *>(&p[e / N].v[e % N]) = __floats2bfloat162_rn(f[e], f[e + 1]);
+            else if constexpr (std::is_same<T, f16>::value) *reinterpret_cast<__half2 *>(&p[e / N].v[e % N]) = __floats2half2_rn(f[e], f[e + 1]);
+            else p[e / N].v[e % N] = f[e], p[(e + 1) / N].v[(e + 1) % N] = f[e + 1];
+        }
+    }
 };
 
 template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_bounds__(CTA) qknorm_rope_kernel(RopeArgs a, int per_block, FastDiv by_heads) {
@@ -123,11 +126,9 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
     const T *const q = static_cast<const T *>(a.q) + token0 * a.q_stride, *const k = static_cast<const T *>(a.k) + token0 * a.k_stride;
     T *const qo = static_cast<T *>(a.qo) + token0 * a.qo_stride, *const ko = static_cast<T *>(a.ko) + token0 * a.ko_stride;
     Eight<T> x0, x1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {  // what a short last unit does not have stays zero
-        x0.set(e, 0.f);
-        x1.set(e, 0.f);
-    }
+    const float zeros[8] = {};
+    x0.set(zeros);  // what a short last unit does not have stays zero
+    x1.set(zeros);
     auto load = [&](int row) {
         const int t = int(fd_div(uint32_t(row), by_heads)), h = row - t * heads;
         const T *x = h < a.q_heads ? q + t * a.q_stride + h * a.dim : k + t * a.k_stride + (h - a.q_heads) * a.dim;
@@ -142,7 +143,7 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
             const T *w = static_cast<const T *>(is_k ? a.kw : a.qw);
             // of which unit's first or second chunk it is
             const bool split = chunk < 2 * rotated_units;
-            const int unit = split ? chunk % rotated_units : chunk / 2, which = split ? chunk / rotated_units : chunk & 1;
+            const int unit = split && chunk >= rotated_units ? chunk - rotated_units : split ? chunk : chunk / 2, which = split ? chunk >= rotated_units : chunk & 1;
             reinterpret_cast<float *>(weights + ((is_k ? 4 : 0) + 2 * which + d % 8 / 4) * LANES + unit)[d % 4] = w ? to_compute(w[d]) : 1.f;
         }
     }
@@ -151,11 +152,11 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
         reinterpret_cast<float2 *>(cs + (t * 4 + e / 2) * LANES + unit)[e & 1] = turn_of(position(a, token0 + t), a.inv_freq[f]);
     }
     __syncthreads();
+    const float by_dim = 1.f / float(a.dim);
     // every thread of a warp takes the same number of turns: the sums are warp shuffles
     for (int row0 = 0; row0 < rows; row0 += CTA / LANES) {
         const int row = row0 + team;
         const bool live = row < rows;
-        if (row0 > 0 && live) load(row);
         float y0[8], y1[8], sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -164,12 +165,14 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
             sum += y0[e] * y0[e];
             sum += y1[e] * y1[e];
         }
+        if (row + CTA / LANES < rows) load(row + CTA / LANES);  // the next row comes while this one is worked on
         const int t = int(fd_div(uint32_t(row), by_heads)), h = row - t * heads;
         const bool is_q = h < a.q_heads;
         if (a.norm) {
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float r = 1.f / sqrtf(sum / float(a.dim) + a.eps);
+            // 16-bit results do not show the 2^-22 that the short form is off by; the long one is two dozen instructions
+            const float mean = sum * by_dim + a.eps, r = sizeof(T) == 4 ? 1.f / sqrtf(mean) : rsqrtf(mean);
             const float4 *w = weights + (is_q ? 0 : 4 * LANES) + u;
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
@@ -212,11 +215,8 @@ template <typename T, int LANES, bool INTERLEAVED> __global__ void __launch_boun
         }
         T *o = is_q ? qo + t * a.qo_stride + h * a.dim : ko + t * a.ko_stride + (h - a.q_heads) * a.dim;
         Eight<T> z0, z1;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            z0.set(e, y0[e]);
-            z1.set(e, y1[e]);
-        }
+        z0.set(y0);
+        z1.set(y1);
         if (has0) z0.store(o + first * 8);
         if (has1) z1.store(o + second * 8);
     }
