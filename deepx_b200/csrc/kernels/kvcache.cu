@@ -83,6 +83,17 @@ template <typename T> struct Sixteen {
             for (int e = 0; e < 16; ++e) x[e] = v[e];
         }
     }
+    __device__ __forceinline__ void set4(int i, float a, float b, float c, float d) {  // values 4i.., two at a time: one conversion
+        if constexpr (std::is_same<T, bf16>::value) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+            w[2 * i] = *reinterpret_cast<const uint32_t *>(&x), w[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+        } else if constexpr (std::is_same<T, f16>::value) {
+            const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+            w[2 * i] = *reinterpret_cast<const uint32_t *>(&x), w[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+        } else {
+            w[4 * i] = __float_as_uint(a), w[4 * i + 1] = __float_as_uint(b), w[4 * i + 2] = __float_as_uint(c), w[4 * i + 3] = __float_as_uint(d);
+        }
+    }
     __device__ __forceinline__ float get(int e) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
         else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
@@ -307,10 +318,7 @@ __global__ void __launch_bounds__(CTA) read_kernel(Cache c, Seqs s, T *k, int64_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 lo = __half22float2(decode2<FMT>(words[e] & 0xFFFFu)), hi = __half22float2(decode2<FMT>(words[e] >> 16));
-            o.v[4 * e] = from_compute<T>(lo.x * f);
-            o.v[4 * e + 1] = from_compute<T>(lo.y * f);
-            o.v[4 * e + 2] = from_compute<T>(hi.x * f);
-            o.v[4 * e + 3] = from_compute<T>(hi.y * f);
+            o.set4(e, lo.x * f, lo.y * f, hi.x * f, hi.y * f);
         }
         o.store((is_v ? v + (row0 + r) * v_stride : k + (row0 + r) * k_stride) + int64_t(u) * 16, width);
     }
