@@ -2,7 +2,7 @@
 //
 // Both are bound by memory: a value is read (written) once at its type's size, its code written (read) once.  Measured (B200): writing four
 // prompts of 5000 to 8192 tokens, 8 heads of 128, bf16 to e4m3: 37.3 us, 4.6 TB/s of the copy's 6.5; reading eight histories of 3000 to
-// 9000 tokens, 8 heads of 64, e4m3 to f16: 32.7 us, 4.7 TB/s.  Sixteen values a thread, moved 32 bytes at a time where the rows allow it
+// 9000 tokens, 8 heads of 64, e4m3 to f16: 32.2 us, 4.7 TB/s.  Sixteen values a thread, moved 32 bytes at a time where the rows allow it
 // (eight at 16 bytes: 41 and 35 us); 64 single tokens: 3.6 us on the device, a launch's latency.
 #include "kvcache.cuh"
 
@@ -363,7 +363,7 @@ void launch_write(const void *k, int64_t ks, const void *v, int64_t vs, const Ca
 }
 template <typename T, int FMT>
 void launch_read(const Cache &c, const Seqs &s, void *k, int64_t ks, void *v, int64_t vs, int32_t *flag, cudaStream_t st) {
-    int chunk = 1;
+    int chunk = 1;  // rows of a block: up to 16 (with 32 or 64 the case above takes 34 and 35 us)
     while (chunk < 16 && s.rows > int64_t(sm_count()) * 8 * chunk) chunk *= 2;
     launch_pdl(read_kernel<T, FMT>, dim3(unsigned((s.rows + chunk - 1) / chunk)), dim3(CTA), 0, st, c, s, static_cast<T *>(k), ks, static_cast<T *>(v), vs, chunk,
                make_fastdiv(unsigned(c.heads * (c.dim / 16))), make_fastdiv(c.dim / 16), width_of<T>(k, ks, v, vs), flag);

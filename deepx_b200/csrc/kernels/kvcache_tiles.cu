@@ -15,7 +15,7 @@
 // the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
 // scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
 //
-// Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 401 us with the plan and the join (14 us), 686 TFLOP/s,
+// Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 394 to 404 us with the plan and the join (14 us), 690 TFLOP/s,
 // 0.43 of a large matrix product's rate; 12 sequences of 1 to 700 new tokens up to 5000, 14 and 2 heads of 64: 91 us.  A step of 64 keys takes
 // about 2800 cycles: 1300 the exponentials and weights of a row, 560 its maximum, 380 and 270 the waits before and after, while the first
 // converter's way through a step is nearly as long (with the exponentials left out the kernel waits for keys and gains 4 %, with the
