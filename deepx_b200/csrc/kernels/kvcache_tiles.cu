@@ -490,6 +490,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     for (int e = 0; e < 32; ++e)
                         if (!(bits >> e & 1)) x[e] = __float_as_uint(NEG_INF);
                 };
+                // From a score of group g to its exponent.  Hidden scores are infinite before they are multiplied: the factor is never zero, however
+                // small the row and the keys' scale are (a score that the least normal number stands for is zero beside any other).
+                auto factor = [&](int g) { return fmaxf(c_row * f.k[g], 1.17549435e-38f); };
                 auto largest = [&](const uint32_t (&x)[32], int col) {
                     float v[4];
 #pragma unroll
@@ -498,7 +501,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
 #pragma unroll
                         for (int e = 2; e < 8; ++e) v[g] = fmaxf(v[g], __uint_as_float(x[8 * g + e]));
                     }
-                    return fmaxf(fmaxf(v[0], v[1]) * (c_row * f.k[col >> 4]), fmaxf(v[2], v[3]) * (c_row * f.k[(col >> 4) + 1]));
+                    return fmaxf(fmaxf(v[0], v[1]) * factor(col >> 4), fmaxf(v[2], v[3]) * factor((col >> 4) + 1));
                 };
                 // ---- the row's largest score ----
                 uint32_t x[2][32];
@@ -542,7 +545,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     uint32_t w[16];
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const float cg = c_row * f.k[2 * q + g], mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
+                        const float cg = factor(2 * q + g), mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
                         const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
 #pragma unroll
                         for (int e = 16 * g; e < 16 * g + 16; e += 2) {
@@ -735,7 +738,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << GROUPS) - 1);
                     Info &f = info[n % INFO];
                     if (lane < GROUPS) {
-                        f.k[lane] = fmaxf(ks, 7.8886091e-31f);  // 2^-100: a factor of zero would make a hidden score not a number
+                        f.k[lane] = ks;
                         f.v_log[lane] = __log2f(unit);
                         f.v_inv[lane] = __fdividef(1.f, unit);
                     }

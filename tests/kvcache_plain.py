@@ -157,6 +157,48 @@ def attention(batch, Q, scale, window=0):
     return out, bound
 
 
+def attention_rows(batch, Q, scale, window=0):
+    """(out, bound) as `attention`, with a bound that depends on nothing but what a row weighs: its weights p, and the values v = s * code
+    of the tokens it sees, s the scale of a token's page.
+
+    A weight times its page's scale is held in 16 bits, so that the largest of a row is 2^7 or more times (a maximum may be rounded up to a whole
+    power of two: 2^6): relative to its own size each is off by 2^-11, or by the fixed half step 2^-25 of what is below 2^-14, which is 2^-31 of
+    the row's largest p * s.  A code is at most 127 (448): together 2^-11 of A = sum p|v|, and 2^-31 * keys * 127 (448) * max(p * s).
+    The sum that divides is of weights in 32 bits.  Scores, sums and exponentials as in `attention`; the arguments of the exponentials
+    that count are below 256, and there are three of them for a weight (its own, that of its group's factor, that of the parts' maxima): 3 * 2^-17
+    is inside 2^-15."""
+    heads = Q.shape[1]
+    group = heads // batch.heads
+    out = torch.zeros(Q.shape, dtype=torch.float64, device=Q.device)
+    bound = torch.zeros_like(out)
+    for b, (n, m) in enumerate(zip(batch.lens, batch.new)):
+        if m == 0 or n == 0:
+            continue
+        pages = batch.host_table[b, torch.arange(n) // batch.page].to(Q.device)
+        slot = torch.arange(n, device=Q.device) % batch.page
+        key = torch.arange(n, device=Q.device)[None, :]
+        pos = torch.arange(n - m, n, device=Q.device)[:, None]
+        seen = key <= pos
+        if window:
+            seen &= key > pos - window
+        row = batch.host_starts[b]
+        for h in range(heads):
+            kv = h // group
+            ks, vs = (x[pages, kv].double() for x in (batch.ks, batch.vs))
+            kh = torch.nan_to_num(batch.k[pages, kv, slot].double()) * torch.nan_to_num(ks)[:, None]
+            vh = torch.nan_to_num(batch.v[pages, kv, slot].double()) * torch.nan_to_num(vs)[:, None]
+            q = Q[row: row + m, h].double()
+            s = ((q @ kh.T) * scale).masked_fill(~seen, -torch.inf)
+            p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300))
+            total = p.sum(-1, keepdim=True)
+            p = torch.where(total > 0, p / total, torch.zeros_like(p))
+            out[row: row + m, h] = p @ vh
+            score = ((q.abs() @ kh.abs().T) * scale * seen).amax(-1, keepdim=True)
+            fixed = 2.0**-31 * seen.double().sum(-1, keepdim=True) * LARGEST[batch.fmt] * (p * torch.nan_to_num(vs)).amax(-1, keepdim=True)
+            bound[row: row + m, h] = fixed + (p @ vh.abs()) * (2.0**-11 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
+    return out, bound
+
+
 def rope(x, weight, inv_freq, positions, eps, interleaved):
     """(y, scale): the norm and rotation of [tokens, heads, dim] in float64, and the size of the pair each element is of."""
     y = x.double()
