@@ -193,16 +193,15 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
         const int pos_min = sq.first + first_row / a.group, pos_max = sq.first + (first_row + rows - 1) / a.group;
         const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's
 
-        float o[NB][MT][4], l[NB][4], m[NB][2], v_ref = 0.f;
+        float o[NB][MT][4], l[NB][2], m[NB][2], big[NB][2];  // output, sum (of this lane's tokens), the maxima for the sum and for the output
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            m[nb][0] = m[nb][1] = NEG_INF;
+            m[nb][0] = m[nb][1] = big[nb][0] = big[nb][1] = NEG_INF;
+            l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                l[nb][e] = 0.f;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int d = 0; d < MT; ++d) o[nb][d][e] = 0.f;
-            }
         }
 
         // ---- keys and values in flight ----
@@ -372,7 +371,8 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                             if (!seen) x[nb][tt][e] = NEG_INF;
                         }
             }
-            // ---- running maximum: a row's rises when a score is 2^8 above it ----
+            // ---- running maxima: a row's rise when a score is 2^8 above one of them ----
+            const float v_log = scale_log2(v_scale);
             float top[NB][2];
             bool rise = false;
 #pragma unroll
@@ -382,13 +382,10 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                     float v = fmaxf(x[nb][0][e], x[nb][0][e + 2]);
 #pragma unroll
                     for (int tt = 1; tt < TT; ++tt) v = fmaxf(v, fmaxf(x[nb][tt][e], x[nb][tt][e + 2]));
-                    rise |= v > m[nb][e] + LAG;
+                    rise |= v > m[nb][e] + LAG || v + v_log > big[nb][e] + LAG;
                     top[nb][e] = v;
                 }
-            const bool scale_up = v_scale > v_ref;
-            if (__any_sync(0xffffffffu, rise) || scale_up) {
-                const float turn = scale_up ? v_ref / v_scale : 1.f;  // values in units of the largest scale so far
-                if (scale_up) v_ref = v_scale;
+            if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     float by[2];
@@ -397,11 +394,11 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                         float v = top[nb][e];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                        v = v > m[nb][e] + LAG ? v : m[nb][e];
-                        by[e] = v == m[nb][e] ? 1.f : exp2_approx(m[nb][e] - v);
-                        m[nb][e] = v;
-                        l[nb][e] *= by[e];
-                        by[e] *= turn;
+                        const float to = v > m[nb][e] + LAG ? ceilf(v) : m[nb][e], big_to = v + v_log > big[nb][e] + LAG ? ceilf(v + v_log) : big[nb][e];
+                        l[nb][e] *= to == m[nb][e] ? 1.f : exp2_approx(m[nb][e] - to);
+                        by[e] = big_to == big[nb][e] ? 1.f : exp2_approx(big[nb][e] - big_to);
+                        m[nb][e] = to;
+                        big[nb][e] = big_to;
                     }
 #pragma unroll
                     for (int d = 0; d < MT; ++d) {
@@ -415,28 +412,24 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
             uint32_t p[NB][TT][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const float m0 = (m[nb][0] == NEG_INF ? 0.f : m[nb][0]) - UP, m1 = (m[nb][1] == NEG_INF ? 0.f : m[nb][1]) - UP;
-                const uint32_t one[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+                float a[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) a[e] = fmaxf(v_log - or_zero(big[nb][e]) + UP, -CAP - or_zero(m[nb][e]));
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
-                    p[nb][tt][0] = transpose8(half2_bits(exp2_approx(x[nb][tt][0] - m0), exp2_approx(x[nb][tt][1] - m1)));
-                    p[nb][tt][1] = transpose8(half2_bits(exp2_approx(x[nb][tt][2] - m0), exp2_approx(x[nb][tt][3] - m1)));
-                    mma(l[nb], one, p[nb][tt][0], p[nb][tt][1]);  // the sum of the very weights that multiply the values
+                    float y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = exp2_approx(x[nb][tt][e] + a[e & 1]);
+                    sum[0] += y[0] + y[2];
+                    sum[1] += y[1] + y[3];
+                    p[nb][tt][0] = transpose8(half2_bits(y[0], y[1]));
+                    p[nb][tt][1] = transpose8(half2_bits(y[2], y[3]));
                 }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) l[nb][e] += sum[e] * exp2_approx(-a[e] - or_zero(m[nb][e]));
             }
 
             // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
-            // Values are in units of the largest scale so far; a page of a smaller one has the difference in its weights, a power of two.
-            if (v_scale != v_ref) {
-                const __half2 unit = __float2half2_rn(v_scale / v_ref);
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int i = 0; i < 2 * TT; ++i) {
-                        const __half2 w = __hmul2(*reinterpret_cast<const __half2 *>(&p[nb][i >> 1][i & 1]), unit);
-                        p[nb][i >> 1][i & 1] = *reinterpret_cast<const uint32_t *>(&w);
-                    }
-            }
             // FINITE: some of the tile's tokens are masked for some rows; what lies there must not be no number.
             auto values = [&](auto finite) {
                 auto four = [&](int tt, uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, int tile) {
@@ -485,7 +478,11 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float sum = l[nb][e], by = sum == 0.f ? 0.f : v_ref / sum;
+                float sum = l[nb][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const Out by = way_out(big[nb][e], m[nb][e], sum);
+                auto result = [&](float x) { return x * by.first * by.second; };
                 const int row = 8 * nb + 2 * t + e;
                 if (g == 0) {
                     sm_m[warp][row] = m[nb][e];
@@ -497,7 +494,7 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                     for (int i = 0; i < W; i += 4) {
                         const int d = h * 128 + g * W + i, tile = h * 8 + i / 2;
                         *reinterpret_cast<float4 *>(mine + in_part(row, d)) =
-                            make_float4(o[nb][tile][e] * by, o[nb][tile][2 + e] * by, o[nb][tile + 1][e] * by, o[nb][tile + 1][2 + e] * by);
+                            make_float4(result(o[nb][tile][e]), result(o[nb][tile][2 + e]), result(o[nb][tile + 1][e]), result(o[nb][tile + 1][2 + e]));
                     }
             }
         __syncthreads();

@@ -11,8 +11,8 @@
 //
 // Roles (16 warps, one block an SM): warps 0-3 and 4-7 the softmax of a tile each; 8-10 turn the codes of K into halfs, 11-13 those of V
 // (sixteen a thread and turn, loaded a step ahead); a thread of warp 14 and one of 15 issue a tile's products each.  Codes become halfs
-// unscaled and exact; the scales of a step's groups of sixteen tokens go to the softmax threads, K's into the factor c, V's (in units of
-// the largest so far) into the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
+// unscaled and exact; the scales of a step's groups of sixteen tokens go to the softmax threads, K's into the factor c, V's into
+// the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
 // scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
 //
 // Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 394 to 404 us with the plan and the join (14 us), 690 TFLOP/s,
@@ -274,11 +274,9 @@ template <int DP> struct Cfg {
     static constexpr int O_COL = 256;
 };
 
-// What the softmax needs of a step: for each group of sixteen tokens K's scale, log2 of V's in units of the largest so far and its
-// inverse; by how much O in units of the largest before shrinks, the largest; which groups are there.
+// What the softmax needs of a step: for each group of sixteen tokens K's scale, log2 of V's and V's inverse; which groups are there.
 struct Info {
     float k[GROUPS], v_log[GROUPS], v_inv[GROUPS];
-    float turn, v_ref;
     int there;
 };
 
@@ -466,7 +464,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             const int tile_first = int(min(int64_t(p.it.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.it.end) - 1));  // least `last` of the tile
             const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
 
-            float m = NEG_INF, v_ref = 1.f;
+            float m = NEG_INF, big = NEG_INF, unit = 1.f;  // the maxima for the sum and for the output; 2^(big - m - UP)
             uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             for (int step = 0; step < p.steps; ++step, ++n, ++n_s) {
                 const int j0 = p.it.lo + (p.step0 + step) * KEYS, place = n_s & 1;
@@ -475,7 +473,6 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 fence_after();
                 const Info &f = info[n % INFO];
                 const int there = f.there;
-                v_ref = f.v_ref;
                 const bool masked = j0 + KEYS - 1 > tile_first || j0 <= tile_after || there != (1 << GROUPS) - 1;  // the same in all threads
                 // the columns of a run of 32 that this row sees, a bit each
                 auto seen = [&](int col) {
@@ -493,6 +490,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 // From a score of group g to its exponent.  Hidden scores are infinite before they are multiplied: the factor is never zero, however
                 // small the row and the keys' scale are (a score that the least normal number stands for is zero beside any other).
                 auto factor = [&](int g) { return fmaxf(c_row * f.k[g], 1.17549435e-38f); };
+                float top = NEG_INF, top_v = NEG_INF;  // of the row's scores, and with the values' scales
                 auto largest = [&](const uint32_t (&x)[32], int col) {
                     float v[4];
 #pragma unroll
@@ -501,7 +499,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
 #pragma unroll
                         for (int e = 2; e < 8; ++e) v[g] = fmaxf(v[g], __uint_as_float(x[8 * g + e]));
                     }
-                    return fmaxf(fmaxf(v[0], v[1]) * factor(col >> 4), fmaxf(v[2], v[3]) * factor((col >> 4) + 1));
+                    const float lo = fmaxf(v[0], v[1]) * factor(col >> 4), hi = fmaxf(v[2], v[3]) * factor((col >> 4) + 1);
+                    top = fmaxf(top, fmaxf(lo, hi));
+                    top_v = fmaxf(top_v, fmaxf(lo + f.v_log[col >> 4], hi + f.v_log[(col >> 4) + 1]));
                 };
                 // ---- the row's largest score ----
                 uint32_t x[2][32];
@@ -512,18 +512,19 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     hide(x[0], 0);
                     hide(x[1], 32);
                 }
-                const float top = fmaxf(largest(x[0], 0), largest(x[1], 32));
-                const float turn = f.turn;
+                largest(x[0], 0);
+                largest(x[1], 32);
                 bool o_known = step == 0;
-                const bool rise = top > m + LAG;
-                if (__any_sync(0xffffffffu, rise) || turn != 1.f) {
-                    const float to = rise ? top : m;
-                    float by = to == m ? 1.f : exp2_approx(m - to);
+                const bool rise = top > m + LAG || top_v > big + LAG;
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float to = top > m + LAG ? ceilf(top) : m, big_to = top_v > big + LAG ? ceilf(top_v) : big;
+                    const float by_l = to == m ? 1.f : exp2_approx(m - to), by = big_to == big ? 1.f : exp2_approx(big - big_to);
                     m = to;
+                    big = big_to;
+                    unit = big == NEG_INF ? 1.f : ldexpf(1.f, int(big - m - UP));
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) l2[e] = fma2(l2[e], pair(by, by), pair(0.f, 0.f));
-                    by *= turn;
-                    if (step > 0) {
+                    for (int e = 0; e < 2; ++e) l2[e] = fma2(l2[e], pair(by_l, by_l), pair(0.f, 0.f));
+                    if (step > 0 && __any_sync(0xffffffffu, by != 1.f)) {
                         if (!warp_wait(o_full(t), (n_s - 1) & 1, abort_flag, S_OUTPUT)) { ok = false; break; }  // the product of the step before
                         fence_after();
                         o_known = true;
@@ -538,14 +539,14 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                         }
                     }
                 }
-                const float base_m = UP - (m == NEG_INF ? 0.f : m);
+                const float base = UP - or_zero(big), least = -CAP - or_zero(m);
                 // ---- weights, over the scores that have been read ----
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     uint32_t w[16];
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const float cg = factor(2 * q + g), mg = base_m + f.v_log[2 * q + g], ig = f.v_inv[2 * q + g];
+                        const float cg = factor(2 * q + g), mg = fmaxf(f.v_log[2 * q + g] + base, least), ig = fminf(unit * f.v_inv[2 * q + g], 0x1p100f);  // 2^CAP
                         const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
 #pragma unroll
                         for (int e = 16 * g; e < 16 * g + 16; e += 2) {
@@ -573,7 +574,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             float l0, l1, l3, l4;
             unpair(l2[0], l0, l1);
             unpair(l2[1], l3, l4);
-            const float sum = (l0 + l1) + (l3 + l4), by = sum == 0.f ? 0.f : v_ref / sum;
+            const float sum = (l0 + l1) + (l3 + l4);
+            const Out by = way_out(big, m, sum);
+            auto result = [&](uint32_t x) { return __uint_as_float(x) * by.first * by.second; };
             const bool whole = p.step0 == 0 && p.steps == p.it.steps;
             float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
             if (!whole) {
@@ -589,8 +592,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     if (!live) continue;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(part + row * DP + d + e) = make_float4(__uint_as_float(x[e]) * by, __uint_as_float(x[e + 1]) * by,
-                                                                                          __uint_as_float(x[e + 2]) * by, __uint_as_float(x[e + 3]) * by);
+                        *reinterpret_cast<float4 *>(part + row * DP + d + e) = make_float4(result(x[e]), result(x[e + 1]), result(x[e + 2]), result(x[e + 3]));
                 }
             } else {
                 // through the place of the warp's rows of Q, which all products have read, and out as whole lines
@@ -607,7 +609,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                         uint32_t w[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const float lo = __uint_as_float(x[e + 2 * k]) * by, hi = __uint_as_float(x[e + 2 * k + 1]) * by;
+                            const float lo = result(x[e + 2 * k]), hi = result(x[e + 2 * k + 1]);
                             if constexpr (std::is_same<T, f16>::value) w[k] = half2_bits(lo, hi);
                             else {
                                 const __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
@@ -707,7 +709,6 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 }
             };
             scales_of(number);
-            float v_ref = 0.f;
             for (int step = 0; step < p.steps; ++step, ++n) {
                 const int stage = n % STAGES;
                 const bool there = number >= 0;
@@ -730,24 +731,14 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     sts128(at0 ^ 16, h[4], h[5], h[6], h[7]);
                 }
                 if (warp == 8) {
-                    float top = vs;
-#pragma unroll
-                    for (int o = GROUPS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    top = fmaxf(top, 1.17549435e-38f);
-                    const float ref = fmaxf(v_ref, top), unit = fmaxf(__fdividef(vs, ref), 8.6736174e-19f);  // 2^-60: below, values count for nothing
                     const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << GROUPS) - 1);
                     Info &f = info[n % INFO];
                     if (lane < GROUPS) {
                         f.k[lane] = ks;
-                        f.v_log[lane] = __log2f(unit);
-                        f.v_inv[lane] = __fdividef(1.f, unit);
+                        f.v_log[lane] = scale_log2(vs);
+                        f.v_inv[lane] = exp2f(-f.v_log[lane]);
                     }
-                    if (lane == 0) {
-                        f.turn = v_ref == 0.f || v_ref == ref ? 1.f : __fdividef(v_ref, ref);
-                        f.v_ref = ref;
-                        f.there = int(mask);
-                    }
-                    v_ref = ref;
+                    if (lane == 0) f.there = int(mask);
                 }
                 fence_async_smem();
                 mbar_arrive(is_v ? v_full(stage) : k_full(stage));

@@ -330,8 +330,10 @@ int dx_kvcache_read(int dtype, const dx_kvseqs *seqs, const dx_kvcache *cache, v
 /* Attention of the new tokens over the cache: out[t,h] = sum_j p_j v_j with p = softmax_j(scale * q[t,h] . k_j) over the
  * positions j <= the token's own, and j > own - window when window > 0; key head h / (q_heads / kv_heads).  The new tokens'
  * keys are in the cache already (dx_kvcache_write).  A row that sees no key is zero.  q and out: [rows][q_heads][head_dim],
- * DX_F16 or DX_BF16; scale > 0.  Codes are multiplied exactly; the softmax's weights are rounded to halfs (2^-11 of each), a row of
- * a bfloat16 q keeps its 8 bits down to 2^-17 of its largest element; sums are float32, the output is rounded once.
+ * DX_F16 or DX_BF16; scale > 0.  Codes are multiplied exactly; what multiplies them, a token's weight times its page's v_scale, is
+ * rounded to a half (2^-11 of itself; what is less than 2^-20 of the row's largest, 2^-31 of that one); a row of
+ * a bfloat16 q keeps its 8 bits down to 2^-17 of its largest element; sums are float32, the sum that divides is that of the
+ * unrounded weights, the output is rounded once.  Scores have to be float32 numbers, scales finite and not below zero.
  * max_new: the most new tokens of a sequence, 0 if not known; it chooses the kernels and with them the speed, never what is
  * computed.  The workspace serves one stream at a time; its size depends on the shapes alone. */
 size_t dx_kvcache_attention_workspace_bytes(int dtype, int64_t q_heads, const dx_kvseqs *seqs, const dx_kvcache *cache, int64_t max_new);

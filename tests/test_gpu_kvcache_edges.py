@@ -79,3 +79,73 @@ def test_tiny_scale_of_float16_queries(TF, new):
     zero_keys(b, 0, 3, 2.0**-126)
     zero_keys(b, 0, 18, 2.0**-126)
     check(TF, b, b.rand(b.rows, 4, 128, dtype=torch.float16), 1e-36, max_new=new)
+
+
+# ---- values of pages whose scales lie far apart ------------------------------------------------------------------
+def apart(seed, lens, new, heads, dim, page, fmt, exponents, gap, favoured):
+    """A batch whose pages have the value scales 2^exponents[column % len]; keys such that a query of ones scores `gap` (natural
+    logarithm; up to twice that) less on every page but the columns of `favoured`."""
+    b = P.Batch(seed, lens, new, heads, dim, page, fmt).fill(lens)
+    plus, minus = (0x01, 0xFF) if fmt == "int8" else (0x38, 0xB8)  # the codes of 1 and -1
+    for i, n in enumerate(lens):
+        for c in range(-(-n // page)):
+            at = int(b.host_table[i, c])
+            b.k.view(torch.uint8)[at] = plus if c % len(exponents) in favoured else minus
+            b.ks[at] = gap / 2 / dim / 0.125
+            b.vs[at] = 2.0 ** exponents[c % len(exponents)]
+    b.ks.copy_(torch.ldexp(torch.ones_like(b.ks), torch.frexp(b.ks.nan_to_num(1.0))[1]))
+    return b
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 3, 140])
+@pytest.mark.parametrize("exponents,favoured", [
+    ((0, -26), (1,)), ((-26, 0), (0,)), ((0, -40), (1,)), ((-24, 10, -24), (0,)), ((30, -90), (1,)), ((-126, 20), (0,)), ((100, -126), (1,)),
+    ((-10, -126, -10), (1,)), ((-6, -8, -30, -7), (2, 3)), ((-126,), (0,)), ((-126, -100), (0,))])
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128)])
+def test_values_of_scales_far_apart(TF, fmt, new, exponents, favoured, page, dim):
+    """A row keeps the bits of the page it weighs, whatever scale the pages beside it have."""
+    lens = [600, 333]
+    for gap in (60.0, 6.0):
+        b = apart(35 + page, lens, [new, new], 1, dim, page, fmt, exponents, gap, favoured)
+        check(TF, b, torch.ones(b.rows, 4, dim, dtype=torch.bfloat16, device="cuda"), 0.125, max_new=new)
+        check(TF, b, b.rand(b.rows, 4, dim, dtype=torch.bfloat16), 0.125, max_new=new)
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_written_values_of_scales_far_apart(TF, new):
+    """The same through kvcache_write: a token of 10^9 in a history of values of 10^-3, behind every row's attention or before it."""
+    lens, dim, page = [500], 64, 16
+    for where in (5, 250, 350, 499):
+        b = P.Batch(36, lens, lens, 1, dim, page, "int8")
+        K, V = b.rand(500, 1, dim), b.rand(500, 1, dim) * 1e-3
+        V[where] *= 1e12
+        K[where] = -4.0
+        TF.kvcache_write(K, V, *b.seqs(), *b.cache(), b.flag)
+        b.new, b.host_starts, b.rows = [new], [0, new], new
+        b.starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        Q = torch.full((new, 2, dim), 3.0, device="cuda").bfloat16()
+        check(TF, b, Q, 0.125, max_new=new)
+
+
+@pytest.mark.parametrize("new", [1, 5, 140])
+def test_rows_do_not_depend_on_pages_they_do_not_see(TF, new):
+    """What stands in the pages in front of a row's window and behind the row (its scales too) does not change one bit of it."""
+    lens, window = [400], 48
+    b = P.Batch(37, lens, [new], 1, 64, 16, "e4m3").fill(lens, (-30, -2))
+    Q = b.rand(b.rows, 4, 64, dtype=torch.bfloat16)
+    clean = attend(TF, b, Q, 0.125, window, new)
+    first = max(0, 400 - new - window + 1) // 16
+    for c in range(first):
+        at = int(b.host_table[0, c])
+        b.vs[at], b.ks[at] = 2.0 ** (c % 40), 2.0**-100
+    assert torch.equal(clean, attend(TF, b, Q, 0.125, window, new)) and int(b.flag) == 0
+    # rows in front of the last page: its scale is not theirs
+    if new > 16:
+        b.vs[int(b.host_table[0, 24])] = 2.0**60  # tokens 384-399
+        out = attend(TF, b, Q, 0.125, window, new)
+        check_rows = new - 16
+        want, bound = P.attention_rows(b, Q, 0.125, window)
+        want, bound = want[:check_rows], bound[:check_rows]
+        off = (out[:check_rows].double() - want).abs()
+        assert bool((off <= bound + P.half_step(Q.dtype) * (want.abs() + bound) + torch.finfo(Q.dtype).tiny).all())
