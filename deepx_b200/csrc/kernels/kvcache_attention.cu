@@ -506,23 +506,21 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
             float top = NEG_INF, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w][row]);
-            const float base = top == NEG_INF ? 0.f : top;
+            const float base = or_zero(top);
+            float share[WARPS];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum += share[w] = sm_l[w][row] * exp2_approx(sm_m[w][row] - base);
+            const float all = sum == 0.f ? 0.f : 1.f / sum;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float by = sm_l[w][row] * exp2_approx(sm_m[w][row] - base);
+                const float by = share[w] * all;  // shares of one: a sum that is divided afterwards could be out of range
                 const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring + w * K::RING) + in_part(row, d));
-                sum += by;
                 v.x += by * x.x;
                 v.y += by * x.y;
                 v.z += by * x.z;
                 v.w += by * x.w;
             }
-            const float by = sum == 0.f ? 0.f : 1.f / sum;
-            v.x *= by;
-            v.y *= by;
-            v.z *= by;
-            v.w *= by;
             if (whole) {
                 const int fr = first_row + row, i = fr / a.group;
                 T *out = static_cast<T *>(a.out) + (sq.row0 + i) * a.out_stride + int64_t(head * a.group + fr - i * a.group) * c.dim + d;

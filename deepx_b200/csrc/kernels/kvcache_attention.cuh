@@ -81,8 +81,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Joins the parts of an item that several blocks worked on: weights from all parts' maxima and sums, then their outputs in the order
-// of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
+// Joins the parts of an item that several blocks worked on: each part's share of one from all parts' maxima and sums, then their outputs in the
+// order of the keys.  A part is ROWS x DP floats of output, ROWS maxima and ROWS sums; block i's first piece leaves part 2i, one that begins
 // with its item and does not end it part 2i + 1.  What it costs is waiting for memory, one load after the other, so there are two ways.
 // Up to FEW parts: a warp takes a row (two where items have many) and has every load of it in flight at once, without waiting for a
 // maximum.  (With the other way alone the join of 64 single tokens after 300 to 8192, 8 key heads of 128, took 13 us in place of 7, that
@@ -130,21 +130,22 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
             float top = m[k][0], sum = 0.f, acc[V] = {};
 #pragma unroll
             for (int p = 1; p < FEW; ++p) top = fmaxf(top, m[k][p]);
-            const float base = top == NEG_INF ? 0.f : top;
+            const float base = or_zero(top);
+#pragma unroll
+            for (int p = 0; p < FEW; ++p) sum += l[k][p] *= exp2_approx(m[k][p] - base);
+            const float all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
             for (int p = 0; p < FEW; ++p) {
-                const float w = l[k][p] * exp2_approx(m[k][p] - base);
-                sum += w;
-                if (p < j.parts && w != 0.f)
+                const float by = l[k][p] * all;  // shares of one: a sum that is divided afterwards could be out of range
+                if (p < j.parts && by != 0.f)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) acc[e] += w * x[k][p][e / VW].v[e % VW];
+                    for (int e = 0; e < V; ++e) acc[e] += by * x[k][p][e / VW].v[e % VW];
             }
-            const float by = sum == 0.f ? 0.f : 1.f / sum;
             T *out = out_row(row) + lane * V;
             if (lane * V >= c.dim) continue;  // dim is a multiple of 16, V a power of two up to 4: the lane's values are all of the row or none
             Pack<T, V> o;
 #pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = from_compute<T>(acc[e] * by);
+            for (int e = 0; e < V; ++e) o.v[e] = from_compute<T>(acc[e]);
             if (reinterpret_cast<uintptr_t>(out) % sizeof(o) == 0) *reinterpret_cast<Pack<T, V> *>(out) = o;
             else
 #pragma unroll
@@ -157,25 +158,34 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
         const int rows = min(last - row0, STEP);
         const int each = rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;  // warps of a row
         const int r = warp / each, row = row0 + r, sub = warp % each;
-        float acc[V] = {}, sum = 0.f;
+        float acc[V] = {};
         if (r < rows) {
-            float top = NEG_INF;
+            float top = NEG_INF, sum = 0.f;
             for (int p0 = lane; p0 < j.parts; p0 += 128) {
-                float m[4];
+                float m[4], l[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m[k] = p0 + 32 * k < j.parts ? at(p0 + 32 * k)[ROWS * DP + row] : NEG_INF;
-                top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = p0 + 32 * k < j.parts;
+                    m[k] = in ? at(p0 + 32 * k)[ROWS * DP + row] : NEG_INF;
+                    l[k] = in ? at(p0 + 32 * k)[ROWS * DP + ROWS + row] : 0.f;
+                }
+                const float to = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), base = or_zero(to);
+                sum *= exp2_approx(top - base);
+                top = to;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum += l[k] * exp2_approx(m[k] - base);
             }
+            float most = top;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float base = top == NEG_INF ? 0.f : top;
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float base = or_zero(most);
+            sum *= exp2_approx(top - base);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float all = sum == 0.f ? 0.f : 1.f / sum;
             for (int p0 = 0; p0 < j.parts; p0 += 32) {
                 float w = 0.f;
-                if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base);
-                float s = w;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                sum += s;
+                if (p0 + lane < j.parts) w = at(p0 + lane)[ROWS * DP + ROWS + row] * exp2_approx(at(p0 + lane)[ROWS * DP + row] - base) * all;
                 const int n = min(32, j.parts - p0);
                 for (int p1 = sub; p1 < n; p1 += FLIGHT * each) {
                     Pack<float, VW> x[FLIGHT][V / VW];
@@ -198,12 +208,11 @@ template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(JOIN_C
         for (int e = 0; e < V; ++e) sh[warp][lane * V + e] = acc[e];
         __syncthreads();
         if (r < rows && sub == 0) {
-            const float by = sum == 0.f ? 0.f : 1.f / sum;
             T *out = out_row(row);
             for (int d = lane; d < c.dim; d += 32) {
                 float v = 0.f;
                 for (int w = 0; w < each; ++w) v += sh[warp + w][d];
-                out[d] = from_compute<T>(v * by);
+                out[d] = from_compute<T>(v);
             }
         }
         __syncthreads();

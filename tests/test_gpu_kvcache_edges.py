@@ -101,7 +101,7 @@ def apart(seed, lens, new, heads, dim, page, fmt, exponents, gap, favoured):
 @pytest.mark.parametrize("new", [1, 3, 140])
 @pytest.mark.parametrize("exponents,favoured", [
     ((0, -26), (1,)), ((-26, 0), (0,)), ((0, -40), (1,)), ((-24, 10, -24), (0,)), ((30, -90), (1,)), ((-126, 20), (0,)), ((100, -126), (1,)),
-    ((-10, -126, -10), (1,)), ((-6, -8, -30, -7), (2, 3)), ((-126,), (0,)), ((-126, -100), (0,))])
+    ((-10, -126, -10), (1,)), ((-6, -8, -30, -7), (2, 3)), ((-126,), (0,)), ((110,), (0,)), ((-126, -100), (0,))])
 @pytest.mark.parametrize("page,dim", [(16, 64), (64, 128)])
 def test_values_of_scales_far_apart(TF, fmt, new, exponents, favoured, page, dim):
     """A row keeps the bits of the page it weighs, whatever scale the pages beside it have."""
@@ -149,3 +149,17 @@ def test_rows_do_not_depend_on_pages_they_do_not_see(TF, new):
         want, bound = want[:check_rows], bound[:check_rows]
         off = (out[:check_rows].double() - want).abs()
         assert bool((off <= bound + P.half_step(Q.dtype) * (want.abs() + bound) + torch.finfo(Q.dtype).tiny).all())
+
+
+@pytest.mark.parametrize("fmt,exponent", [("int8", 120), ("e4m3", 118)])
+@pytest.mark.parametrize("lens,new,q_heads,dim", [([3000], [1], 4, 64), ([3000], [150], 4, 64), ([40000], [1], 2, 128), ([900, 700, 650], [1, 1, 1], 12, 128),
+                                                  ([900], [1], 2, 256)])
+def test_values_near_the_end_of_float32(TF, fmt, exponent, lens, new, q_heads, dim):
+    """Averages of values near float32's largest, in one part and joined out of few and of many: nothing on the way is larger than they are."""
+    b = P.Batch(39, lens, new, 1, dim, 16, fmt).fill(lens, (-9, -8))
+    b.vs[b.host_table.flatten()] = 2.0**exponent
+    v = b.v.view(torch.uint8)
+    v &= 0x7F  # positive, up to the largest code
+    if fmt == "e4m3":
+        v[v == 0x7F] = 0x7E
+    check(TF, b, b.rand(b.rows, q_heads, dim, dtype=torch.bfloat16), 0.05, max_new=max(new))
