@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
         const int steps = step1 - step0;
 
         const int pos_min = sq.first + first_row / a.group, pos_max = sq.first + (first_row + rows - 1) / a.group;
-        const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's
+        const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's, and those in front of seen_begin: their pages may be anyone's
+        const int seen_begin = a.window > 0 ? int(max(int64_t(pos_min) - a.window + 1, int64_t(0))) : 0;
 
         float o[NB][MT][4], l[NB][2], m[NB][2], big[NB][2];  // output, sum (of this lane's tokens), the maxima for the sum and for the output
 #pragma unroll
@@ -210,12 +211,12 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
         auto token0 = [&](int step) { return ln.lo + (step0 + step) * STEP + warp * WT; };
         auto page_number = [&](int step) {
             const int j = token0(step);
-            return step < steps && j < seen_end ? table[j >> c.page_shift] : -1;
+            return step < steps && j < seen_end && j + WT > seen_begin ? table[j >> c.page_shift] : -1;
         };
         auto issue = [&](int step, int stage, int32_t number) {
             if (step < steps) {
                 const int j = token0(step);
-                const int left = seen_end - j;  // tokens to load
+                const int left = j + WT > seen_begin ? seen_end - j : 0;  // tokens to load
                 const bool ok = left > 0 && number >= 0 && number < c.pages;
                 if (left > 0 && !ok && lane == 0) raise(a.flag, FLAG_PAGE);
                 const uint32_t dst = ring_u + stage * 2 * K::TILE;

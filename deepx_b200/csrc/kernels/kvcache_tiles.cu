@@ -49,11 +49,11 @@ enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS 
 __device__ int g_status = 0;
 
 // 256 rows of a sequence, the same for all heads: rows first_row.. of the flattened (new token, head of the group), tokens lo..hi
-// in steps of KEYS from lo (a multiple of KEYS).
+// in steps of KEYS from lo (a multiple of KEYS); the first token that one of the rows sees (pages wholly in front of it may be anyone's).
 struct alignas(16) Group {
     int64_t row0;
     int b, first, end;  // sequence, position of its first new token, tokens its pages can be read for
-    int first_row, rows, lo, hi, steps;
+    int first_row, rows, lo, hi, steps, first_seen;
 };
 // The plan: the groups, the units of the line in front of each, the groups in front of a sequence.
 struct Plan {
@@ -93,7 +93,8 @@ __device__ __forceinline__ Group group_of(const Seq &q, const Attn &a, int b, in
     const int64_t hi = max(min(int64_t(q.end), p1 + 1), int64_t(0));
     const int64_t lo = a.window > 0 ? max(int64_t(0), p0 - a.window + 1) : 0;
     x.hi = int(hi);
-    x.lo = int(min(lo, hi) / KEYS * KEYS);
+    x.first_seen = int(min(lo, hi));
+    x.lo = x.first_seen / KEYS * KEYS;
     x.steps = hi > x.lo ? int((hi - x.lo + KEYS - 1) / KEYS) : 1;  // rows that see nothing are written too
     return x;
 }
@@ -670,18 +671,19 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             // lane g of a warp (mod GROUPS) knows group g of a step: its page, and where its codes begin (-1: nowhere)
             const int32_t *table = s.table + int64_t(p.it.b) * s.cols;
             // A page's number is asked for a step before it is looked at: nothing waits for it.
+            auto token_of = [&](int step) { return p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16; };
+            auto seen = [&](int step, int j) { return step < p.steps && j < p.it.hi && j + 16 > p.it.first_seen; };
             auto entry_of = [&](int step) {
-                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
-                return step < p.steps && j < p.it.hi ? table[j >> c.page_shift] : -1;
+                const int j = token_of(step);
+                return seen(step, j) ? table[j >> c.page_shift] : -1;
             };
             auto page_of = [&](int step, int32_t entry) {
-                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
                 if (uint32_t(entry) < uint64_t(c.pages)) return entry;
-                if (warp == 8 && lane < GROUPS && step < p.steps && j < p.it.hi) raise(a.flag, FLAG_PAGE);
+                if (warp == 8 && lane < GROUPS && seen(step, token_of(step))) raise(a.flag, FLAG_PAGE);
                 return -1;
             };
             auto begin_of = [&](int step, int32_t number) {
-                const int j = p.it.lo + (p.step0 + step) * KEYS + (lane % GROUPS) * 16;
+                const int j = token_of(step);
                 return number < 0 ? int64_t(-1) : ((int64_t(number) * c.heads + p.head) * c.page + (j & (c.page - 1))) * c.dim;
             };
             uint4 x[TURNS];

@@ -328,8 +328,9 @@ int dx_kvcache_write(int dtype, const void *k, int64_t k_stride, const void *v, 
 int dx_kvcache_read(int dtype, const dx_kvseqs *seqs, const dx_kvcache *cache, void *k, int64_t k_stride, void *v, int64_t v_stride,
                     int32_t *flag, void *stream);
 /* Attention of the new tokens over the cache: out[t,h] = sum_j p_j v_j with p = softmax_j(scale * q[t,h] . k_j) over the
- * positions j <= the token's own, and j > own - window when window > 0; key head h / (q_heads / kv_heads).  The new tokens'
- * keys are in the cache already (dx_kvcache_write).  A row that sees no key is zero.  q and out: [rows][q_heads][head_dim],
+ * positions j <= the token's own, and j > own - window when window > 0; key head h / (q_heads / kv_heads).  Pages wholly in front of the
+ * window of a sequence's first new token are not looked at: they may have been given back, their entries in the table hold anything.  The
+ * new tokens' keys are in the cache already (dx_kvcache_write).  A row that sees no key is zero.  q and out: [rows][q_heads][head_dim],
  * DX_F16 or DX_BF16; scale > 0.  Codes are multiplied exactly; what multiplies them, a token's weight times its page's v_scale, is
  * rounded to a half (2^-11 of itself; what is less than 2^-20 of the row's largest, 2^-31 of that one); a row of
  * a bfloat16 q keeps its 8 bits down to 2^-17 of its largest element; sums are float32, the sum that divides is that of the

@@ -163,3 +163,33 @@ def test_values_near_the_end_of_float32(TF, fmt, exponent, lens, new, q_heads, d
     if fmt == "e4m3":
         v[v == 0x7F] = 0x7E
     check(TF, b, b.rand(b.rows, q_heads, dim, dtype=torch.bfloat16), 0.05, max_new=max(new))
+
+
+# ---- pages behind a window ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("page,q_heads,dim", [(16, 4, 64), (32, 4, 128), (16, 8, 256), (64, 20, 96), (128, 2, 64)])
+@pytest.mark.parametrize("window,lens,new", [(1, [500, 64, 3], [1, 1, 1]), (100, [500, 333, 129], [1, 2, 4]), (33, [700, 256], [1, 16]),
+                                             (17, [700, 300, 5], [300, 100, 5]), (129, [900, 400], [130, 260])])
+def test_pages_behind_the_window_are_not_looked_at(TF, fmt, page, q_heads, dim, window, lens, new):
+    """Pages in front of every row's window may have been given back: their table entries are of no page, the pages' bytes and scales
+    anything; no flag, and not one bit of the result is another."""
+    b = P.Batch(38 + page, lens, new, 2, dim, page, fmt).fill(lens)
+    Q = b.rand(b.rows, 2 * q_heads, dim, dtype=torch.bfloat16)
+    for hint in (max(new), 0):
+        want = attend(TF, b, Q, dim ** -0.5, window, hint)
+        table = b.table.clone()
+        for i, (n, m) in enumerate(zip(lens, new)):
+            for c in range(max(0, n - m - window + 1) // page):
+                table[i, c] = (-1, b.pages, 2**31 - 1, -2**31)[c % 4]
+        got = attend(TF, b, Q, dim ** -0.5, window, hint, table)
+        assert int(b.flag) == 0
+        assert torch.equal(got, want)
+    b.table = table
+    check(TF, b, Q, dim ** -0.5, window, max(new))
+    # the page that the first row's window begins in is looked at
+    i = 0
+    c = max(0, lens[i] - new[i] - window + 1) // page
+    table = b.table.clone()
+    table[i, c] = -1
+    attend(TF, b, Q, dim ** -0.5, window, max(new), table)
+    assert int(b.flag) == 1
