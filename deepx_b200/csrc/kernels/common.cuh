@@ -20,6 +20,29 @@ int check_launch(const char *what);  // cudaGetLastError → DX_E_CUDA
 
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
+// ---- memory that a call names -----------------------------------------------------
+// `rows` rows of `width` bytes, `pitch` bytes from one to the next (pitch >= width).
+struct Span {
+    const char *at;
+    int64_t rows, pitch, width;
+};
+inline Span span(const void *p, int64_t bytes) { return {static_cast<const char *>(p), 1, bytes, bytes}; }
+inline Span span(const void *p, int64_t rows, int64_t pitch, int64_t width) { return {static_cast<const char *>(p), rows, pitch, width}; }
+// Whether two of them share a byte.  Columns of the same rows do not; rows of two different pitches that lie among one another are taken to.
+inline bool meet(const Span &a, const Span &b) {
+    if (!a.at || !b.at || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+    if (a.at >= b.at + (b.rows - 1) * b.pitch + b.width || b.at >= a.at + (a.rows - 1) * a.pitch + a.width) return false;
+    if (a.rows == 1 || b.rows == 1) {
+        const Span &many = a.rows == 1 ? b : a, &one = a.rows == 1 ? a : b;
+        const int64_t to = one.at - many.at - many.width;  // rows that end at or in front of `one` begin here at the latest
+        const int64_t i = to < 0 ? 0 : to / many.pitch + 1;
+        return i < many.rows && many.at + i * many.pitch < one.at + one.width;
+    }
+    if (a.pitch != b.pitch) return true;
+    const int64_t shift = ((a.at - b.at) % a.pitch + a.pitch) % a.pitch;
+    return shift < b.width || shift + a.width > a.pitch;
+}
+
 // ---- programmatic dependent launch -----------------------------------------------
 // A kernel launched through launch_pdl may be scheduled while the kernel before it on the stream drains: its CTAs
 // become resident and run up to griddep_wait(), which returns once the earlier kernel has completed and its writes

@@ -324,17 +324,29 @@ __global__ void __launch_bounds__(CTA) read_kernel(Cache c, Seqs s, T *k, int64_
     }
 }
 
-int check_rows(const char *what, int dtype, const Seqs &s, const Cache &c, const void *k, int64_t k_stride, const void *v, int64_t v_stride) {
+// What both entries check of their rows and of what their memory shares; `write`: the rows are read and the cache written, else the other way round.
+int check_rows(const char *what, bool write, int dtype, const Seqs &s, const Cache &c, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *flag) {
     if (dtype != DX_F32 && dtype != DX_F16 && dtype != DX_BF16) return fail(DX_E_DTYPE, "%s: unsupported dtype code %d (float32, float16, bfloat16)", what, dtype);
     const int64_t width = int64_t(c.heads) * c.dim;
     if (k_stride < width || v_stride < width) return fail(DX_E_SHAPE, "%s: rows of %lld elements overlap at strides %lld and %lld", what, (long long)width, (long long)k_stride, (long long)v_stride);
     if (s.rows == 0 || s.batch == 0) return DX_OK;
     if (!k || !v) return fail(DX_E_ARG, "%s: null tensor pointer", what);
-    const int64_t es = dx_dtype_size(dtype), codes = c.pages * c.heads * int64_t(c.page) * c.dim;
-    for (const void *p : {k, v}) {
-        const int64_t bytes = ((s.rows - 1) * (p == k ? k_stride : v_stride) + width) * es;
-        if (overlap(p, bytes, c.k, codes) || overlap(p, bytes, c.v, codes)) return fail(DX_E_ALIAS, "%s: a tensor overlaps the cache", what);
+    const int64_t es = dx_dtype_size(dtype);
+    const Span rows[2] = {span(k, s.rows, k_stride * es, width * es), span(v, s.rows, v_stride * es, width * es)}, raised = span(flag, 4);
+    const CacheSpans cache(c, s);
+    for (const Span &x : rows)
+        if (meet(x, cache.codes[0]) || meet(x, cache.codes[1]) || meet(x, cache.scales[0]) || meet(x, cache.scales[1])) return fail(DX_E_ALIAS, "%s: a tensor overlaps the cache", what);
+    if (!write && (meet(rows[0], rows[1]) || cache.lists_met_by(rows[0]) || cache.lists_met_by(rows[1])))
+        return fail(DX_E_ALIAS, "%s: an output overlaps the other one or starts, lens or table", what);
+    if (write) {
+        const Span *out[4] = {&cache.codes[0], &cache.codes[1], &cache.scales[0], &cache.scales[1]};
+        for (int i = 0; i < 4; ++i) {
+            if (cache.lists_met_by(*out[i])) return fail(DX_E_ALIAS, "%s: the cache overlaps starts, lens or table", what);
+            for (int n = 0; n < i; ++n)
+                if (meet(*out[i], *out[n])) return fail(DX_E_ALIAS, "%s: the cache's tensors overlap", what);
+        }
     }
+    if (cache.met_by(raised) || meet(rows[0], raised) || meet(rows[1], raised)) return fail(DX_E_ALIAS, "%s: the flag lies in a tensor", what);
     return DX_OK;
 }
 
@@ -389,7 +401,7 @@ extern "C" int dx_kvcache_write(int dtype, const void *k, int64_t k_stride, cons
     kv::Cache c;
     kv::Seqs s;
     if (int e = kv::check("kvcache_write", cache, seqs, &c, &s)) return e;
-    if (int e = kv::check_rows("kvcache_write", dtype, s, c, k, k_stride, v, v_stride)) return e;
+    if (int e = kv::check_rows("kvcache_write", true, dtype, s, c, k, k_stride, v, v_stride, flag)) return e;
     if (s.rows == 0 || s.batch == 0) return DX_OK;
     cudaStream_t st = as_stream(stream);
 #define DX_CALL(T, FMT) kv::launch_write<T, FMT>(k, k_stride, v, v_stride, c, s, flag, st)
@@ -404,7 +416,7 @@ extern "C" int dx_kvcache_read(int dtype, const dx_kvseqs *seqs, const dx_kvcach
     kv::Cache c;
     kv::Seqs s;
     if (int e = kv::check("kvcache_read", cache, seqs, &c, &s)) return e;
-    if (int e = kv::check_rows("kvcache_read", dtype, s, c, k, k_stride, v, v_stride)) return e;
+    if (int e = kv::check_rows("kvcache_read", false, dtype, s, c, k, k_stride, v, v_stride, flag)) return e;
     if (s.rows == 0 || s.batch == 0) return DX_OK;
     cudaStream_t st = as_stream(stream);
 #define DX_CALL(T, FMT) kv::launch_read<T, FMT>(c, s, k, k_stride, v, v_stride, flag, st)

@@ -31,11 +31,22 @@ struct Seqs {
 
 // Checks of the two descriptors that every entry point makes; DX_OK, or the code `fail` returned.
 int check(const char *what, const dx_kvcache *c, const dx_kvseqs *s, Cache *cache, Seqs *seqs);
-// Whether [a, a+na) and [b, b+nb) share a byte.
-inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    const char *x = static_cast<const char *>(a), *y = static_cast<const char *>(b);
-    return na > 0 && nb > 0 && x < y + nb && y < x + na;
-}
+// The memory that the descriptors name.
+struct CacheSpans {
+    Span codes[2], scales[2], lists[3];
+    CacheSpans(const Cache &c, const Seqs &s) {
+        const int64_t n = c.pages * c.heads, bytes = n * c.page * c.dim;
+        codes[0] = span(c.k, bytes), codes[1] = span(c.v, bytes), scales[0] = span(c.k_scale, n * 4), scales[1] = span(c.v_scale, n * 4);
+        lists[0] = span(s.starts, (int64_t(s.batch) + 1) * 4), lists[1] = span(s.lens, int64_t(s.batch) * 4);
+        lists[2] = span(s.table, int64_t(s.batch) * s.cols * 4);
+    }
+    bool met_by(const Span &x) const {
+        for (int i = 0; i < 2; ++i)
+            if (meet(x, codes[i]) || meet(x, scales[i])) return true;
+        return lists_met_by(x);
+    }
+    bool lists_met_by(const Span &x) const { return meet(x, lists[0]) || meet(x, lists[1]) || meet(x, lists[2]); }
+};
 
 #ifdef __CUDACC__
 __device__ __forceinline__ void raise(int32_t *flag, int bit) {

@@ -622,15 +622,17 @@ extern "C" int dx_kvcache_attention(int dtype, const void *q, int64_t q_stride, 
     if (s.rows * (q_heads / c.heads) > INT32_MAX) return fail(DX_E_SHAPE, "kvcache_attention: %lld rows of %lld heads each over a key head", (long long)s.rows, (long long)(q_heads / c.heads));
     if (s.rows == 0 || s.batch == 0) return DX_OK;
     if (!q || !out) return fail(DX_E_ARG, "kvcache_attention: null tensor pointer");
-    const int64_t qb = ((s.rows - 1) * q_stride + width) * 2, ob = ((s.rows - 1) * out_stride + width) * 2;
-    const int64_t codes = c.pages * c.heads * int64_t(c.page) * c.dim;
-    if (kv::overlap(q, qb, out, ob) || kv::overlap(out, ob, c.k, codes) || kv::overlap(out, ob, c.v, codes))
-        return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
+    const Span qs = span(q, s.rows, q_stride * 2, width * 2), outs = span(out, s.rows, out_stride * 2, width * 2), raised = span(flag, 4);
+    const kv::CacheSpans spans(c, s);
+    if (meet(outs, qs) || spans.met_by(outs)) return fail(DX_E_ALIAS, "kvcache_attention: the output overlaps an input");
+    if (meet(outs, raised) || meet(qs, raised) || spans.met_by(raised)) return fail(DX_E_ALIAS, "kvcache_attention: the flag lies in a tensor");
     const int64_t rows = kv::rows_of(q_heads, c, s, max_new);
     const bool tiles = kv::by_tiles(c, rows);
     const size_t need = tiles ? kv::tiles_workspace(c, s, int(q_heads / c.heads)) : kv::workspace(c.dim);
     if (!workspace || workspace_bytes < need) return fail(DX_E_WORKSPACE, "kvcache_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned_to(workspace, 256)) return fail(DX_E_ARG, "kvcache_attention: the workspace must start on a 256-byte boundary");
+    const Span scratch = span(workspace, int64_t(need));
+    if (meet(scratch, outs) || meet(scratch, qs) || meet(scratch, raised) || spans.met_by(scratch)) return fail(DX_E_ALIAS, "kvcache_attention: the workspace overlaps a tensor");
     kv::Attn a{q, out, q_stride, out_stride, int(q_heads), int(q_heads / c.heads), int(window > INT32_MAX ? 0 : window), float(scale * 1.4426950408889634),
                q_stride % 8 == 0 && aligned_to(q, 16), out_stride % 8 == 0 && aligned_to(out, 16), static_cast<uint8_t *>(workspace), flag};
     cudaStream_t st = as_stream(stream);

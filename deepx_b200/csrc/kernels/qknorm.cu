@@ -274,21 +274,21 @@ extern "C" int dx_qknorm_rope(int dtype, const void *q, int64_t q_stride, int64_
     } sides[2] = {{q, q_out, q_stride, q_out_stride, q_heads}, {k, k_out, k_stride, k_out_stride, k_heads}};
     for (const Side &x : sides)
         if (x.heads && (x.stride < x.heads * head_dim || x.out_stride < x.heads * head_dim)) return fail(DX_E_SHAPE, "qknorm_rope: rows overlap at strides %lld and %lld", (long long)x.stride, (long long)x.out_stride);
-    // A token's rows in one buffer (a packed projection) interleave with the other tensor's: only equal-stride rows that
-    // do not share columns, or the very same rows, may.
-    for (const Side &o : sides)
+    // An output may be its own input, or stand beside other tensors' columns in the rows of one buffer (a packed projection); it meets nothing else.
+    const int64_t wide = head_dim * es;
+    const Span others[] = {span(norm ? q_weight : nullptr, wide), span(norm ? k_weight : nullptr, wide), span(rotated ? inv_freq : nullptr, rotated / 2 * 4),
+                           span(rotated ? positions : nullptr, tokens * dx_dtype_size(pos_dtype))};
+    auto out_of = [&](const Side &x) { return span(x.heads ? x.out : nullptr, tokens, x.out_stride * es, x.heads * wide); };
+    if (meet(out_of(sides[0]), out_of(sides[1]))) return fail(DX_E_ALIAS, "qknorm_rope: the outputs overlap");
+    for (const Side &o : sides) {
         for (const Side &i : sides) {
-            if (!o.heads || !i.heads) continue;
-            const bool same = &o == &i && o.out == i.in && o.out_stride == i.stride;
-            const int64_t ow = o.heads * head_dim * es, iw = i.heads * head_dim * es;
-            const char *a = static_cast<const char *>(o.out), *b = static_cast<const char *>(i.in);
-            const int64_t ob = (tokens - 1) * o.out_stride * es + ow, ib = (tokens - 1) * i.stride * es + iw;
-            if (same || a + ob <= b || b + ib <= a) continue;
-            const int64_t pitch = o.out_stride * es;
-            const int64_t shift = ((a - b) % pitch + pitch) % pitch;
-            const bool apart = o.out_stride == i.stride && shift >= iw && shift + ow <= pitch;
-            if (!apart) return fail(DX_E_ALIAS, "qknorm_rope: an output overlaps an input other than its own");
+            const bool own = &o == &i && o.out == i.in && o.out_stride == i.stride;
+            if (!own && meet(out_of(o), span(i.heads ? i.in : nullptr, tokens, i.stride * es, i.heads * wide)))
+                return fail(DX_E_ALIAS, "qknorm_rope: an output overlaps an input other than its own");
         }
+        for (const Span &x : others)
+            if (meet(out_of(o), x)) return fail(DX_E_ALIAS, "qknorm_rope: an output overlaps a weight, inv_freq or positions");
+    }
     RopeArgs a{q, k, q_weight, k_weight, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, tokens, int(q_heads), int(k_heads),
                int(head_dim), int(rotated), interleaved, norm, float(eps), inv_freq, positions, pos_dtype == DX_I64};
     cudaStream_t st = as_stream(stream);

@@ -282,7 +282,8 @@ int dx_softmax(int dtype, const void *x, void *out, int64_t rows, int64_t cols, 
  * `rotated` dimensions turn by the angles positions[t] * inv_freq[i], i < rotated/2, in the pairs (i, i + rotated/2), or
  * (2i, 2i+1) when `interleaved`; the others pass.  float32 arithmetic, angles in float64, one rounding at the end.
  * q is [tokens][q_heads][head_dim] with `q_stride` elements from token to token (k alike; k_heads = 0: no keys), the
- * outputs likewise; an output may be its input (same pointer and stride).  head_dim <= DX_ROPE_MAX_DIM, `rotated` even,
+ * outputs likewise; an output may be its input (same pointer and stride), or stand in columns of the same rows as other tensors, but
+ * meet no other argument's memory (DX_E_ALIAS).  head_dim <= DX_ROPE_MAX_DIM, `rotated` even,
  * 0..head_dim.  positions: DX_I32 or DX_I64.  dtype: DX_F32, DX_F16, DX_BF16 (weights the same, inv_freq float32). */
 #define DX_ROPE_MAX_DIM 512
 int dx_qknorm_rope(int dtype, const void *q, int64_t q_stride, int64_t q_heads, const void *k, int64_t k_stride, int64_t k_heads,
@@ -304,7 +305,10 @@ int dx_qknorm_rope(int dtype, const void *q, int64_t q_stride, int64_t q_heads, 
  *
  * `flag` (device int32, may be NULL) collects: bit 0, a page number outside the cache (its tokens are not written, read as
  * zeros and masked); bit 1, starts that do not ascend within the rows, or a length outside the table (what fits is worked
- * on); bit 2, a value that is not a number (stored as 0).  No call touches memory out of range for any content of these. */
+ * on); bit 2, a value that is not a number (stored as 0).  No call touches memory out of range for any content of these.
+ *
+ * What a call writes meets no other memory that it uses, the other tensors that it writes included (DX_E_ALIAS); columns of the same
+ * rows of a buffer do not meet. */
 typedef enum { DX_CACHE_I8 = 0, DX_CACHE_E4M3 = 1, DX_CACHE_FORMAT_COUNT = 2 } dx_cache_format;
 typedef struct dx_kvcache {
     void *k, *v;

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import kvcache_plain as P
+from test_gpu_qknorm import check as check_rope
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +194,47 @@ def test_pages_behind_the_window_are_not_looked_at(TF, fmt, page, q_heads, dim, 
     table[i, c] = -1
     attend(TF, b, Q, dim ** -0.5, window, max(new), table)
     assert int(b.flag) == 1
+
+
+# ---- columns of one buffer ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("first", [0, 1])
+def test_outputs_beside_one_another_in_one_buffer(TF, dtype, first):
+    """Keys and values read into columns of the same rows, queries and keys turned into such columns, an output beside its queries: what a
+    packed projection's buffer is used for.  The columns between stay as they were."""
+    dt, lens, new = P.FLOATS[dtype], [70, 9], [64, 9]
+    b = P.Batch(40, lens, new, 2, 64, 16, "int8").fill(lens)
+    b.table = b.host_table.int().cuda()
+    buf = torch.full((b.rows, first + 600), 7.0, dtype=dt, device="cuda")
+
+    def columns(at, heads):
+        return buf[:, first + at: first + at + heads * 64].unflatten(1, (heads, 64))
+
+    K, V = (torch.empty(b.rows, 2, 64, dtype=dt, device="cuda") for _ in "kv")
+    TF.kvcache_read(*b.cache(), *b.seqs(), K, V, b.flag)
+    TF.kvcache_read(*b.cache(), *b.seqs(), columns(320, 2), columns(128, 2), b.flag)
+    assert torch.equal(columns(320, 2), K) and torch.equal(columns(128, 2), V)
+    inv = (10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)).float().cuda()
+    pos = torch.arange(b.rows, device="cuda")
+    Q = b.rand(b.rows, 4, 64, dtype=dt)
+    TF.qknorm_rope(Q, K, None, None, inv, pos, 1e-6, False, columns(0, 4), columns(320, 2))
+    check_rope(columns(0, 4), Q, None, inv, pos, 1e-6, False)  # another kernel off 16-byte boundaries: other bits than that of whole tensors
+    check_rope(columns(320, 2), K, None, inv, pos, 1e-6, False)
+    if dt != torch.float32:
+        out, turned = torch.empty_like(Q), columns(0, 4).clone()
+        TF.kvcache_attention(turned, *b.cache(), *b.seqs(), 0.125, 64, 0, out, b.flag)
+        TF.kvcache_attention(columns(0, 4), *b.cache(), *b.seqs(), 0.125, 64, 0, columns(256, 4), b.flag)
+        assert torch.equal(columns(256, 4), out) and torch.equal(columns(0, 4), turned)
+    assert bool((buf[:, :first] == 7).all()) and bool((buf[:, first + 512:] == 7).all())
+
+
+def test_overlapping_outputs_are_an_error(TF):
+    b = P.Batch(41, [20], [20], 1, 64, 16, "int8").fill([20])
+    K = torch.zeros(20, 1, 64, device="cuda")
+    inv, pos = torch.zeros(32, device="cuda"), torch.arange(20, device="cuda")
+    with pytest.raises(Exception, match="overlap"):
+        TF.kvcache_read(*b.cache(), *b.seqs(), K, K)
+    with pytest.raises(Exception, match="overlap"):
+        TF.kvcache_write(K, K, *b.seqs(), b.k, b.k, b.ks, b.vs)
+    with pytest.raises(Exception, match="overlap"):
+        TF.qknorm_rope(K, K.clone(), None, None, inv, pos, 1e-6, False, K, K)
