@@ -194,10 +194,14 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
         const int seen_end = min(sq.end, pos_max + 1);  // tokens from here on are no row's, and those in front of seen_begin: their pages may be anyone's
         const int seen_begin = a.window > 0 ? int(max(int64_t(pos_min) - a.window + 1, int64_t(0))) : 0;
 
-        float o[NB][MT][4], l[NB][2], m[NB][2], big[NB][2];  // output, sum (of this lane's tokens), the maxima for the sum and for the output
+        float o[NB][MT][4], l[NB][2];  // output, sum (of this lane's tokens)
+        Maxima most[NB][2];
+        float unit[NB][2];  // 2^(7 - d)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            m[nb][0] = m[nb][1] = big[nb][0] = big[nb][1] = NEG_INF;
+            most[nb][0].clear();
+            most[nb][1].clear();
+            unit[nb][0] = unit[nb][1] = exp2_approx(UP - D_LEAST);
             l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                         }
             }
             // ---- running maxima: a row's rise when a score is 2^8 above one of them ----
-            const float v_log = scale_log2(v_scale);
+            const float power = scale_power(v_scale);
             float top[NB][2];
             bool rise = false;
 #pragma unroll
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                     float v = fmaxf(x[nb][0][e], x[nb][0][e + 2]);
 #pragma unroll
                     for (int tt = 1; tt < TT; ++tt) v = fmaxf(v, fmaxf(x[nb][tt][e], x[nb][tt][e + 2]));
-                    rise |= v > m[nb][e] + LAG || v + v_log > big[nb][e] + LAG;
+                    rise |= v - most[nb][e].m > fminf(LAG, most[nb][e].d + (LAG - power));
                     top[nb][e] = v;
                 }
             if (__any_sync(0xffffffffu, rise)) {
@@ -392,14 +396,12 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                     float by[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float v = top[nb][e];
+                        float v = top[nb][e], of_sum;
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                        const float to = v > m[nb][e] + LAG ? ceilf(v) : m[nb][e], big_to = v + v_log > big[nb][e] + LAG ? ceilf(v + v_log) : big[nb][e];
-                        l[nb][e] *= to == m[nb][e] ? 1.f : exp2_approx(m[nb][e] - to);
-                        by[e] = big_to == big[nb][e] ? 1.f : exp2_approx(big[nb][e] - big_to);
-                        m[nb][e] = to;
-                        big[nb][e] = big_to;
+                        most[nb][e].rise(v, [&](float m) { return v - m + power; }, of_sum, by[e]);
+                        l[nb][e] *= of_sum;
+                        unit[nb][e] = exp2_approx(UP - most[nb][e].d);
                     }
 #pragma unroll
                     for (int d = 0; d < MT; ++d) {
@@ -413,21 +415,16 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
             uint32_t p[NB][TT][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                float a[2], sum[2] = {0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 2; ++e) a[e] = fmaxf(v_log - or_zero(big[nb][e]) + UP, -CAP - or_zero(m[nb][e]));
+                // finite also for a row that does not see the page
+                const float h0 = fminf(unit[nb][0] * v_scale, -LOWEST), h1 = fminf(unit[nb][1] * v_scale, -LOWEST), m0 = most[nb][0].m, m1 = most[nb][1].m;
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
-                    float y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = exp2_approx(x[nb][tt][e] + a[e & 1]);
-                    sum[0] += y[0] + y[2];
-                    sum[1] += y[1] + y[3];
-                    p[nb][tt][0] = transpose8(half2_bits(y[0], y[1]));
-                    p[nb][tt][1] = transpose8(half2_bits(y[2], y[3]));
+                    const float y0 = exp2_approx(x[nb][tt][0] - m0), y1 = exp2_approx(x[nb][tt][1] - m1), y2 = exp2_approx(x[nb][tt][2] - m0), y3 = exp2_approx(x[nb][tt][3] - m1);
+                    l[nb][0] += y0 + y2;
+                    l[nb][1] += y1 + y3;
+                    p[nb][tt][0] = transpose8(half2_bits(y0 * h0, y1 * h1));
+                    p[nb][tt][1] = transpose8(half2_bits(y2 * h0, y3 * h1));
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) l[nb][e] += sum[e] * exp2_approx(-a[e] - or_zero(m[nb][e]));
             }
 
             // ---- values: lane (g, t) multiplies tokens 2t, 2t+1, 2t+8, 2t+9 of its chunk's dimensions ----
@@ -482,11 +479,11 @@ __global__ void __launch_bounds__(CTA, Cfg<DP, NB, WT>::BLOCKS) attention_kernel
                 float sum = l[nb][e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                const Out by = way_out(big[nb][e], m[nb][e], sum);
+                const Out by = way_out(most[nb][e].d, sum);
                 auto result = [&](float x) { return x * by.first * by.second; };
                 const int row = 8 * nb + 2 * t + e;
                 if (g == 0) {
-                    sm_m[warp][row] = m[nb][e];
+                    sm_m[warp][row] = most[nb][e].m;
                     sm_l[warp][row] = sum;
                 }
 #pragma unroll

@@ -43,13 +43,12 @@ template <typename F> int allow_shared(F *kernel, int bytes, std::atomic<uint64_
 }
 
 #ifdef __CUDACC__
-// A row has two running maxima, both rounded up to a whole number: m of its scores x (in powers of two), for the sum of its weights, and M
-// of x + log2(s), s the scale of the values' page, for its output.  The weight that multiplies a value's code is the half 2^(x + log2(s) - M + 7):
-// M lags the true maximum by up to 8, so a weight is at most 2^15, what is 2^-31 of the row's largest is still a half, and a page that the row
-// does not weigh takes no bits from the others, whatever its scale is.  The exponential y is one for both: y = 2^(x + a), a = log2(s) - M + 7, and
-// the sum gets y * f, f = 2^(-a - m), in 32 bits.  So that y is not lost where the sum needs it, a is -100 - m at least: below that the weight is
-// zero as a half either way.
-constexpr float LAG = 8.f, UP = 7.f, CAP = 100.f;
+// A row's weights are 2^(x - m), x its scores in powers of two, m their running maximum, which may lag by LAG; their sum is one of 32-bit
+// numbers.  What multiplies a value's code is the half of 2^(x - m) * s * 2^(7 - d), s the scale of the value's page and d the running maximum of
+// x - m + log2(s), with the same lag: at most 2^15, and what is 2^-31 of the row's largest is still a half.  So a page that the row does not weigh
+// takes no bits from the others, whatever its scale is.  Both are whole numbers (rounded up), and d is a small one where x is not: scores
+// of any size are exact beside it.  Below D_LEAST no value is a normal number; a row begins there.
+constexpr float LAG = 8.f, UP = 7.f, D_LEAST = -118.f, LOWEST = -3.402823466e38f;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr int JOIN_CTA = 512;
 
@@ -60,20 +59,35 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// log2 of a page's scale, a whole number for a power of two; what is below the least normal number (a page never written) counts as zero.
-__device__ __forceinline__ float scale_log2(float s) {
-    const uint32_t u = __float_as_uint(s), part = u & 0x7FFFFFu;
-    const float whole = float(int(u >> 23) - 127);
-    return s >= 1.17549435e-38f ? (part ? whole + __log2f(__uint_as_float(part | 0x3F800000u)) : whole) : NEG_INF;
+// The whole power of two that a scale is or lies below (for zero, one below all others).
+__device__ __forceinline__ float scale_power(float s) {
+    const uint32_t u = __float_as_uint(s) & 0x7FFFFFFFu;
+    return __uint_as_float(0x4B000000u | (u + 0x7FFFFFu) >> 23) - (8388608.f + 127.f);  // the exponent without a conversion
 }
+// A row's running maxima.
+struct Maxima {
+    float m, d;
+    __device__ __forceinline__ void clear() { m = LOWEST, d = D_LEAST; }
+    // The row's largest score is `top`; top_v(m): its largest score less m with its scale's power.  How much the sum and the output so far are
+    // in the new units.
+    template <typename TopV> __device__ __forceinline__ void rise(float top, TopV top_v, float &of_sum, float &of_output) {
+        const float to = top - m > LAG ? ceilf(top) : m;
+        of_sum = to == m ? 1.f : exp2_approx(m - to);
+        const float was = to == m ? d : d + (m - to);
+        m = to;
+        const float now = top_v(m);
+        d = fmaxf(now > was + LAG ? ceilf(now) : was, D_LEAST);
+        of_output = d == was ? 1.f : exp2_approx(was - d);
+    }
+};
 __device__ __forceinline__ float or_zero(float m) { return m == NEG_INF ? 0.f : m; }
-// What brings a row's output, in units of 2^(M - 7), and its sum, in units of 2^m, to the result: output * first * second.  Two factors, as
-// one could be out of float32's range where the result is not.
+// What brings a row's output, in units of 2^(d - 7), over its sum to the result: output * first * second.  Two factors, as one could be out of
+// float32's range where the result is not.
 struct Out {
     float first, second;
 };
-__device__ __forceinline__ Out way_out(float big, float m, float sum) {
-    const float half = exp2_approx(big == NEG_INF ? 0.f : 0.5f * (big - m - UP));
+__device__ __forceinline__ Out way_out(float d, float sum) {
+    const float half = exp2_approx(0.5f * (d - UP));
     return {half, sum == 0.f ? 0.f : half / sum};
 }
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {

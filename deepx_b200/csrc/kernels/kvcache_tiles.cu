@@ -43,6 +43,7 @@ constexpr int STAGES = 4, INFO = 8;
 constexpr int CONVERTERS = 3;  // warps for K, and for V
 constexpr int OVERHEAD = 6;
 constexpr int PLAN_CTA = 1024;
+constexpr float CAP = 100.f, CAP_INVERSE = 0x1p100f;
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000ll;  // ~2 s
 enum Status : int { S_OK = 0, S_KEYS = 1, S_VALUES = 2, S_SCORES = 3, S_WEIGHTS = 4, S_QUERIES = 5, S_OUTPUT = 6, S_ROOM = 7 };
 
@@ -233,6 +234,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
           "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(at)
+                 : "memory");
+}
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -275,11 +281,15 @@ template <int DP> struct Cfg {
     static constexpr int O_COL = 256;
 };
 
-// What the softmax needs of a step: for each group of sixteen tokens K's scale, log2 of V's and V's inverse; which groups are there.
+// What the softmax needs of a step: for each group of sixteen tokens K's scale, V's, V's power of two (minus infinity for zero) and that one's
+// inverse; which groups are there, and ODD where a scale of V is no power of two (or none whose inverse is a normal number).
 struct Info {
-    float k[GROUPS], v_log[GROUPS], v_inv[GROUPS];
+    float k[GROUPS], v_log[GROUPS], v_inv[GROUPS], v[GROUPS];
     int there;
 };
+constexpr int ODD = 1 << GROUPS;
+__device__ __forceinline__ float power_of_two(float whole) { return __int_as_float((int(whole) + 127) << 23); }
+__device__ __forceinline__ float power_in(float unit) { return float((__float_as_int(unit) >> 23) - 127); }
 
 // The products of a step, by one thread.  `base`: the block's operands, Q of both tiles, then the stages of K, then those of V.
 template <int DP> __device__ __forceinline__ void scores_of(uint32_t base, int tile, int place, int stage) {
@@ -465,7 +475,9 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             const int tile_first = int(min(int64_t(p.it.first) + (p.it.first_row + t * TILE_ROWS) / a.group, int64_t(p.it.end) - 1));  // least `last` of the tile
             const int64_t tile_after = a.window > 0 ? int64_t(p.it.first) + (p.it.first_row + min(p.it.rows, (t + 1) * TILE_ROWS) - 1) / a.group - a.window : -1;
 
-            float m = NEG_INF, big = NEG_INF, unit = 1.f;  // the maxima for the sum and for the output; 2^(big - m - UP)
+            // The row's maxima: m, and d as 2^(d - 7) and m + d.  Where m is so large that a scale's power is not exact beside it, m + d is minus
+            // infinity: each step then goes the long way.
+            float m = LOWEST, unit = power_of_two(D_LEAST - UP), big = LOWEST + D_LEAST;
             uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             for (int step = 0; step < p.steps; ++step, ++n, ++n_s) {
                 const int j0 = p.it.lo + (p.step0 + step) * KEYS, place = n_s & 1;
@@ -474,7 +486,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 fence_after();
                 const Info &f = info[n % INFO];
                 const int there = f.there;
-                const bool masked = j0 + KEYS - 1 > tile_first || j0 <= tile_after || there != (1 << GROUPS) - 1;  // the same in all threads
+                const bool masked = j0 + KEYS - 1 > tile_first || j0 <= tile_after || (there & (ODD - 1)) != ODD - 1;  // the same in all threads
                 // the columns of a run of 32 that this row sees, a bit each
                 auto seen = [&](int col) {
                     const int hi = min(max(last - j0 - col + 1, 0), 32), lo = int(min(max(after - j0 - col + 1, int64_t(0)), int64_t(32)));
@@ -491,7 +503,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 // From a score of group g to its exponent.  Hidden scores are infinite before they are multiplied: the factor is never zero, however
                 // small the row and the keys' scale are (a score that the least normal number stands for is zero beside any other).
                 auto factor = [&](int g) { return fmaxf(c_row * f.k[g], 1.17549435e-38f); };
-                float top = NEG_INF, top_v = NEG_INF;  // of the row's scores, and with the values' scales
+                float top_of[GROUPS], top = NEG_INF, top_v = NEG_INF;  // of a group's scores, the row's, and the row's with the values' scales
                 auto largest = [&](const uint32_t (&x)[32], int col) {
                     float v[4];
 #pragma unroll
@@ -500,9 +512,13 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
 #pragma unroll
                         for (int e = 2; e < 8; ++e) v[g] = fmaxf(v[g], __uint_as_float(x[8 * g + e]));
                     }
-                    const float lo = fmaxf(v[0], v[1]) * factor(col >> 4), hi = fmaxf(v[2], v[3]) * factor((col >> 4) + 1);
-                    top = fmaxf(top, fmaxf(lo, hi));
-                    top_v = fmaxf(top_v, fmaxf(lo + f.v_log[col >> 4], hi + f.v_log[(col >> 4) + 1]));
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float s = __fmul_rn(fmaxf(v[2 * g], v[2 * g + 1]), factor((col >> 4) + g));
+                        top_of[(col >> 4) + g] = s;
+                        top = fmaxf(top, s);
+                        top_v = fmaxf(top_v, s + f.v_log[(col >> 4) + g]);
+                    }
                 };
                 // ---- the row's largest score ----
                 uint32_t x[2][32];
@@ -515,14 +531,25 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                 }
                 largest(x[0], 0);
                 largest(x[1], 32);
-                bool o_known = step == 0;
-                const bool rise = top > m + LAG || top_v > big + LAG;
-                if (__any_sync(0xffffffffu, rise)) {
-                    const float to = top > m + LAG ? ceilf(top) : m, big_to = top_v > big + LAG ? ceilf(top_v) : big;
-                    const float by_l = to == m ? 1.f : exp2_approx(m - to), by = big_to == big ? 1.f : exp2_approx(big - big_to);
-                    m = to;
-                    big = big_to;
-                    unit = big == NEG_INF ? 1.f : ldexpf(1.f, int(big - m - UP));
+                bool o_known = step == 0, stored = false;
+                // ---- weights, over the scores that have been read ----
+                // One exponential y = 2^(x - m + a), a = log2(s) - d + 7, is what multiplies the codes; the sum gets y * 2^-a.  So that y is not lost where
+                // the sum needs it, a is -CAP at least: below that, what multiplies the codes is zero as a half either way.
+                auto lower = [&](int g) { return fminf(unit * f.v_inv[g], CAP_INVERSE); };
+                const bool rise = top > m + LAG || !(top_v < big + LAG);
+                if (__any_sync(0xffffffffu, rise) || there >= ODD) {
+                    Maxima most{m, power_in(unit) + UP};
+                    float by_l, by;
+                    most.rise(top, [&](float m) {
+                        float v = NEG_INF;
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) v = fmaxf(v, top_of[g] - m + f.v_log[g]);
+                        return v;
+                    }, by_l, by);
+                    m = most.m;
+                    unit = power_of_two(most.d - UP);
+                    const bool huge = fabsf(m) > 4194304.f && m != LOWEST;
+                    big = huge ? NEG_INF : m + most.d;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) l2[e] = fma2(l2[e], pair(by_l, by_l), pair(0.f, 0.f));
                     if (step > 0 && __any_sync(0xffffffffu, by != 1.f)) {
@@ -539,27 +566,50 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                             tmem_st16(o_tmem + d, y);
                         }
                     }
-                }
-                const float base = UP - or_zero(big), least = -CAP - or_zero(m);
-                // ---- weights, over the scores that have been read ----
+                    if (__any_sync(0xffffffffu, huge) || there >= ODD) {  // the long way: m is subtracted from the rounded score, then a joins them
+#pragma unroll 1
+                        for (int g = 0; g < GROUPS; ++g) {  // a group's weights lie where its own scores and those of the groups in front of it were
+                            uint32_t z[16], w[8];
+                            tmem_ld16(here + 16 * g, z);
+                            wait_ld();
+                            const uint32_t bits = masked ? seen(16 * g) : ~0u;
+                            const float s = f.v_log[g] == NEG_INF ? NEG_INF : log2f(f.v[g]);
+                            const float cg = factor(g), a = fmaxf(s + (UP - most.d), -CAP), ig = fminf(unit * exp2f(-s), CAP_INVERSE);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    uint32_t w[16];
+                            for (int e = 0; e < 16; e += 2) {
+                                float y[2];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float cg = factor(2 * q + g), mg = fmaxf(f.v_log[2 * q + g] + base, least), ig = fminf(unit * f.v_inv[2 * q + g], 0x1p100f);  // 2^CAP
-                        const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
-#pragma unroll
-                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                            float y0, y1;
-                            unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
-                            y0 = exp2_approx(y0);
-                            y1 = exp2_approx(y1);
-                            l2[(e >> 1) & 1] = fma2(pair(y0, y1), i2, l2[(e >> 1) & 1]);
-                            w[e / 2] = half2_bits(y0, y1);
+                                for (int k = 0; k < 2; ++k)
+                                    y[k] = bits >> (e + k) & 1 ? exp2_approx(__fmul_rn(__uint_as_float(z[e + k]), cg) - m + a) : 0.f;
+                                l2[(e >> 1) & 1] = fma2(pair(y[0], y[1]), pair(ig, ig), l2[(e >> 1) & 1]);
+                                w[e / 2] = half2_bits(y[0], y[1]);
+                            }
+                            tmem_st8(here + 8 * g, w);
                         }
+                        stored = true;
                     }
-                    tmem_st16(here + 16 * q, w);
+                }
+                if (!stored) {
+                    const float base = UP - big, least = -CAP - m;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float cg = factor(2 * q + g), mg = fmaxf(f.v_log[2 * q + g] + base, least), ig = lower(2 * q + g);
+                            const uint64_t c2 = pair(cg, cg), m2 = pair(mg, mg), i2 = pair(ig, ig);
+#pragma unroll
+                            for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                                float y0, y1;
+                                unpair(fma2(pair(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), c2, m2), y0, y1);
+                                y0 = exp2_approx(y0);
+                                y1 = exp2_approx(y1);
+                                l2[(e >> 1) & 1] = fma2(pair(y0, y1), i2, l2[(e >> 1) & 1]);
+                                w[e / 2] = half2_bits(y0, y1);
+                            }
+                        }
+                        tmem_st16(here + 16 * q, w);
+                    }
                 }
                 wait_st();
                 // Each step sees the product of the step before complete, before it lets its own begin: so no wait on this barrier is two of
@@ -576,7 +626,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
             unpair(l2[0], l0, l1);
             unpair(l2[1], l3, l4);
             const float sum = (l0 + l1) + (l3 + l4);
-            const Out by = way_out(big, m, sum);
+            const Out by = way_out(power_in(unit) + UP, sum);
             auto result = [&](uint32_t x) { return __uint_as_float(x) * by.first * by.second; };
             const bool whole = p.step0 == 0 && p.steps == p.it.steps;
             float *part = parts + (int64_t(blockIdx.x) * 2 + (p.step0 == 0 ? 1 : 0)) * C::PART;
@@ -737,10 +787,13 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
                     Info &f = info[n % INFO];
                     if (lane < GROUPS) {
                         f.k[lane] = ks;
-                        f.v_log[lane] = scale_log2(vs);
-                        f.v_inv[lane] = exp2f(-f.v_log[lane]);
+                        const bool none = vs < 1.17549435e-38f;  // a page never written
+                        f.v_log[lane] = none ? NEG_INF : scale_power(vs);
+                        f.v_inv[lane] = __uint_as_float(none ? 0x7F800000u : 0x7F000000u - (__float_as_uint(vs) & 0x7F800000u));
+                        f.v[lane] = vs;
                     }
-                    if (lane == 0) f.there = int(mask);
+                    const bool odd = __any_sync(0xffffffffu, (__float_as_uint(vs) & 0x7FFFFFu) || vs > 0x1p125f);
+                    if (lane == 0) f.there = int(mask) | (odd ? ODD : 0);
                 }
                 fence_async_smem();
                 mbar_arrive(is_v ? v_full(stage) : k_full(stage));

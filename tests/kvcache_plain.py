@@ -161,11 +161,12 @@ def attention_rows(batch, Q, scale, window=0):
     """(out, bound) as `attention`, with a bound that depends on nothing but what a row weighs: its weights p, and the values v = s * code
     of the tokens it sees, s the scale of a token's page.
 
-    A weight times its page's scale is held in 16 bits, so that the largest of a row is 2^7 or more times (a maximum may be rounded up to a whole
-    power of two: 2^6): relative to its own size each is off by 2^-11, or by the fixed half step 2^-25 of what is below 2^-14, which is 2^-31 of
-    the row's largest p * s.  A code is at most 127 (448): together 2^-11 of A = sum p|v|, and 2^-31 * keys * 127 (448) * max(p * s).
+    A weight times its page's scale (a power of two) is held in 16 bits, so that the largest of a row is 2^7 or more times (a maximum may be
+    rounded up to a whole power of two: 2^6): relative to its own size each is off by 2^-11, or by the fixed half step 2^-25 of what is below 2^-14,
+    which is 2^-31 of the row's largest p * s.  A code is at most 127 (448): together 2^-11 of A = sum p|v|, and 2^-31 * keys * 127 (448) * max(p * s).
+    Weights are 32-bit numbers: those below 2^-126 of the largest are zero, at most 2^-126 * sum |v|.
     The sum that divides is of weights in 32 bits.  Scores, sums and exponentials as in `attention`; the arguments of the exponentials
-    that count are below 256, and there are three of them for a weight (its own, that of its group's factor, that of the parts' maxima): 3 * 2^-17
+    that count are below 256, and there are three of them for a weight (its own, that of the scale's unit, that of the parts' maxima): 3 * 2^-17
     is inside 2^-15."""
     heads = Q.shape[1]
     group = heads // batch.heads
@@ -195,6 +196,7 @@ def attention_rows(batch, Q, scale, window=0):
             out[row: row + m, h] = p @ vh
             score = ((q.abs() @ kh.abs().T) * scale * seen).amax(-1, keepdim=True)
             fixed = 2.0**-31 * seen.double().sum(-1, keepdim=True) * LARGEST[batch.fmt] * (p * torch.nan_to_num(vs)).amax(-1, keepdim=True)
+            fixed = fixed + 2.0**-126 * (seen.double() @ vh.abs())
             bound[row: row + m, h] = fixed + (p @ vh.abs()) * (2.0**-11 + 4 * batch.dim * 2.0**-23 * score + n * 2.0**-23 + 2.0**-15)
     return out, bound
 

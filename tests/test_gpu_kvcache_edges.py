@@ -129,6 +129,52 @@ def test_written_values_of_scales_far_apart(TF, new):
         check(TF, b, Q, 0.125, max_new=new)
 
 
+@pytest.mark.parametrize("new", [1, 4, 140])
+@pytest.mark.parametrize("power", [20, 24, 27, 40, 80])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_of_scales_far_apart_under_huge_scores(TF, new, power, dim):
+    """Scores of about 2^power, the same for every token of half of the pages and far below on the others: each of those tokens has
+    the same weight, whatever its page's value scale is, and no bit of a scale is lost beside the score.  Weights are exact here but for
+    their rounding to 16 bits and the exponential's 2^-21: 2^-11 + 2^-15 of the mean |v|, as in kvcache_plain.attention_rows, and its
+    fixed term of the largest scale among pages of one weight."""
+    lens, page = [900, 500], 16
+    exponents = (-6, -3, -30, -7, -12, -3, -20, -5, -6)
+    b = apart(43, lens, [new, new], 1, dim, page, "int8", exponents, 1.0, (0, 2, 4, 6, 8))
+    b.ks[b.host_table.flatten()] = 2.0 ** (power - 20)
+    Q = (torch.randint(4, 8, (b.rows, 4, dim), generator=b.g).cuda() * 2.0**18).bfloat16()  # the products and their sums are exact
+    out = attend(TF, b, Q, 1.0 / dim, max_new=new).double()
+    assert int(b.flag) == 0
+    for i, n in enumerate(lens):
+        v = b.history(b.v, b.vs, i)[:, 0]
+        token = torch.arange(n, device="cuda")
+        chosen = (token // page) % len(exponents) % 2 == 0
+        for t in range(new):
+            use = v[: n - new + t + 1][chosen[: n - new + t + 1]]
+            want, size = use.mean(0), use.abs().mean(0)
+            bound = size * (2.0**-11 + 2.0**-15 + n * 2.0**-23) + 2.0**-30 * 127 * 2.0**-6
+            off = (out[b.host_starts[i] + t] - want).abs()
+            assert bool((off <= bound + P.half_step(torch.bfloat16) * (want.abs() + bound)).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 4, 140])
+def test_scales_that_are_no_powers_of_two(TF, fmt, new):
+    """A cache that another program made: scales of any positive float, a few of them powers of two.  A scale may lie below its power of two
+    by up to half, the largest weight then 2^5 times: twice the fixed term, so twice the bound."""
+    for spread in (1.0, 12.0):
+        lens = [700, 90 + new]
+        b = P.Batch(44, lens, [new, new], 2, 96, 16, fmt).fill(lens, (-9, -7))
+        for scales in (b.ks, b.vs):
+            u = torch.rand(scales.shape, generator=b.g).cuda()
+            scales.copy_(torch.where(u < 0.2, scales, scales * torch.exp2(u * 2 - 1)))
+        b.vs *= torch.exp2((torch.rand(b.vs.shape, generator=b.g).cuda() - 0.5) * spread)
+        Q = b.rand(b.rows, 6, 96, dtype=torch.bfloat16)
+        want, bound = P.attention_rows(b, Q, 0.1)
+        off = (attend(TF, b, Q, 0.1, max_new=new).double() - want).abs()
+        bound = 2 * bound
+        assert bool((off <= bound + P.half_step(Q.dtype) * (want.abs() + bound)).all()) and int(b.flag) == 0
+
+
 @pytest.mark.parametrize("new", [1, 5, 140])
 def test_rows_do_not_depend_on_pages_they_do_not_see(TF, new):
     """What stands in the pages in front of a row's window and behind the row (its scales too) does not change one bit of it."""
