@@ -284,3 +284,26 @@ def test_overlapping_outputs_are_an_error(TF):
         TF.kvcache_write(K, K, *b.seqs(), b.k, b.k, b.ks, b.vs)
     with pytest.raises(Exception, match="overlap"):
         TF.qknorm_rope(K, K.clone(), None, None, inv, pos, 1e-6, False, K, K)
+
+
+# ---- head sizes above 128 that are no power of two ---------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [144, 208, 240])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_large_head_sizes(TF, fmt, dim, page):
+    """Written, read back and attended: single tokens, few and many rows, few parts and many, a window."""
+    for lens, new in (([1, 300, 17], [1, 1, 1]), ([130, 70], [130, 33]), ([9000], [1]), ([0, 2, 600], [3, 1, 5])):
+        b = P.Batch(42 + dim, lens, new, 2, dim, page, fmt, extra_rows=1).fill([max(0, n - m) for n, m in zip(lens, new)], (-9, -3))
+        K, V = b.rand(b.rows, 2, dim, dtype=torch.bfloat16), b.rand(b.rows, 2, dim, dtype=torch.bfloat16)
+        want = P.write(b, K, V)
+        TF.kvcache_write(K, V, *b.seqs(), *b.cache(), b.flag)
+        for got, w in zip(b.cache(), want):
+            assert torch.equal(got.cpu().view(torch.uint8), w.view(torch.uint8))
+        R, S = torch.full_like(K, 7.0), torch.full_like(V, 7.0)
+        TF.kvcache_read(*b.cache(), *b.seqs(), R, S, b.flag)
+        for got, codes, scales in ((R, b.k, b.ks), (S, b.v, b.vs)):
+            for i, (n, m) in enumerate(zip(lens, new)):
+                at = b.host_starts[i] + max(0, m - n)
+                assert torch.equal(got[at: b.host_starts[i] + m], b.history(codes, scales, i)[max(0, n - m):].to(K.dtype))
+        for window in (0, 50):
+            check(TF, b, b.rand(b.rows, 6, dim, dtype=torch.bfloat16), dim ** -0.5, window, max(new))
