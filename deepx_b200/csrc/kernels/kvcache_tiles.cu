@@ -702,7 +702,7 @@ template <typename T, int FMT, int DP> __global__ void __launch_bounds__(THREADS
     } else if (warp < 8 + 2 * CONVERTERS) {
         // ===== codes into halfs: keys or values =====
         const bool is_v = warp >= 8 + CONVERTERS;
-        const int sub = (warp - 7) % CONVERTERS;  // the first warp, which has the steps' info to see to as well, is not the one with a turn more
+        const int sub = (warp - 6) % CONVERTERS;  // the first warp, which has the steps' info to see to as well, has no turn more than the others
         constexpr int PER_ROW = DP / 16, WARP_ROWS = 32 / PER_ROW, UNITS = KEYS / WARP_ROWS, TURNS = (UNITS + CONVERTERS - 1) / CONVERTERS;
         auto has = [&](int turn) { return turn + 1 < TURNS || sub < UNITS - CONVERTERS * (TURNS - 1); };  // the same in all threads of the warp
         // In turn i the warp takes rows WARP_ROWS * (sub + CONVERTERS * i)..., a thread sixteen codes, chunk ch of one row: eight lanes in a row are
