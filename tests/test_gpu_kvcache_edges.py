@@ -158,6 +158,20 @@ def test_values_of_scales_far_apart_under_huge_scores(TF, new, power, dim):
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("new", [1, 4, 140])
+@pytest.mark.parametrize("exponents", [(0, -6, -5), (0,), (-6, 0, 0), (0, 100, -126)])
+def test_values_of_scale_zero(TF, fmt, new, exponents):
+    """Pages of value scale zero (never written) have their share of the sum and add nothing, whatever their codes are; exponent 0 stands for one."""
+    lens, page = [500, 33 + new], 16
+    b = P.Batch(45, lens, [new, new], 1, 64, page, fmt).fill(lens, (-7, -5))
+    for i, n in enumerate(lens):
+        for c in range(-(-n // page)):
+            e = exponents[c % len(exponents)]
+            b.vs[int(b.host_table[i, c])] = 2.0**e if e else 0.0
+    check(TF, b, b.rand(b.rows, 4, 64, dtype=torch.bfloat16), 0.125, max_new=new)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 4, 140])
 def test_scales_that_are_no_powers_of_two(TF, fmt, new):
     """A cache that another program made: scales of any positive float, a few of them powers of two.  A scale may lie below its power of two
     by up to half, the largest weight then 2^5 times: twice the fixed term, so twice the bound."""
