@@ -6,17 +6,18 @@
 // For one new token a sequence this is bound by memory: every code is read once and used for a few rows.  Keys and values are the
 // tensor cores' 16-row operand (sixteen tokens times a few rows; sixteen dimensions times a few rows), so that a group of up to eight
 // rows wastes nothing and the halfs made of a code serve all rows at once.  One pass with the running maximum m and sum of the
-// softmax; codes become halfs exactly, so the only rounding to 16 bits is that of the weights (and each row of a bfloat16 query is
-// brought to size 1 by a power of two first, which keeps its 8 bits; elements 2^-17 below the row's largest begin to lose some).
+// softmax; codes become halfs exactly, so the only rounding to 16 bits is that of the weights times their page's scale (and each row of a
+// bfloat16 query is brought to size 1 by a power of two first, which keeps its 8 bits; elements 2^-17 below the row's largest begin to lose some).
 //
 // Work is split over the keys: the 64-token steps of all tiles of rows and heads of all sequences stand in one line, and each
 // block takes an equal piece of it, whatever the lengths are (they are known on the device alone).  A piece may begin or end
 // inside an item (one tile of rows, one head); such items' parts meet in the workspace and a second kernel joins them, always
 // in the order of the keys: the same bits every time.
 //
-// Measured (B200, 32 query and 8 key heads of 128): one token after 262100, int8, f16: 95 to 102 us, 5.3 to 5.6 TB/s of the copy's 6.5; 64 single
-// tokens after 300 to 8192, e4m3, bf16: 72 us, 4.6 TB/s, 7 of them the join; one token after 1500: 11 us on the device, two launches and
-// the chain from the lengths to the pages to the keys.  More than the copy's time goes into each block's way to its first keys, the
+// Measured (B200, 32 query and 8 key heads of 128): one token after 262100, int8, f16: 94 to 101 us, 5.3 to 5.7 TB/s of the copy's 6.5; 64 single
+// tokens after 300 to 8192, e4m3, bf16: 71 us, 4.7 TB/s, 7 of them the join; one token after 1500: 11 us on the device, two launches and
+// the chain from the lengths to the pages to the keys; a prompt of 4096, 8 and 4 heads of 256: 930 us, as its keys are read and turned into halfs again for each
+// sixteen rows.  More than the copy's time goes into each block's way to its first keys, the
 // joints between items and turning codes into halfs with twelve warps an SM.
 #include "kvcache_attention.cuh"
 

@@ -15,15 +15,15 @@
 // the exponent, so they cost no instruction for each element.  A row's maximum may lag by 2^8 before O is
 // scaled again (in TMEM, by the row's thread), which after the first steps hardly happens.
 //
-// Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 394 to 404 us with the plan and the join (14 us), 690 TFLOP/s,
-// 0.43 of a large matrix product's rate; 12 sequences of 1 to 700 new tokens up to 5000, 14 and 2 heads of 64: 91 us.  A step of 64 keys takes
-// about 2800 cycles: 1300 the exponentials and weights of a row, 560 its maximum, 380 and 270 the waits before and after, while the first
-// converter's way through a step is nearly as long (with the exponentials left out the kernel waits for keys and gains 4 %, with the
+// Measured (B200): two prompts of 4096 tokens, 32 query and 8 key heads of 128, int8, bf16: 400 to 406 us with the plan and the join (14 us), 683 TFLOP/s,
+// 0.42 of a large matrix product's rate, 242 us with a window of 1024; 12 sequences of 1 to 700 new tokens up to 5000, 14 and 2 heads of 64: 94 us.
+// 2 to 4 % of it is what the values' scales cost in the maximum and the sum.  A step of 64 keys takes, without that, about 2800 cycles:
+// 1300 the exponentials and weights of a row, 560 its maximum, 380 and 270 the waits before and after, while the first converter's way through a step is nearly as long (with the exponentials left out the kernel waits for keys and gains 4 %, with the
 // conversion left out 2 %).  Not taken, as slower: two threads a row (16 softmax warps of 80 registers: 520 us), the tiles in turns, loading
-// the next scores early.
+// the next scores early, weights times their page's scale in place of a common exponent (windowed 246 us, two prompts with heads of 64 170 in place of 165).
 //
 // The steps of all items stand in one line, planned by a small kernel first, and every block takes an equal piece of it, where an
-// item counts OVERHEAD steps more than it has (its queries, its way out: about 10,000 cycles; without that the blocks of a prompt's first
+// item counts OVERHEAD steps more than it has (its queries, its way out: 13,000 to 15,000 cycles measured, five steps of 2800, counted as six for heads of either size; without that the blocks of a prompt's first
 // rows, whose items have few steps, took twice the others' time); items that more than one block works on are joined as in kvcache_attention.cu.
 //
 // Every wait is bounded by a clock; when one runs out a status word is set (dx_kvcache_status), all roles leave, TMEM is freed.
