@@ -171,6 +171,25 @@ def test_values_of_scale_zero(TF, fmt, new, exponents):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [4, 140])
+@pytest.mark.parametrize("size", [float("inf"), 1e30, 1e7])
+def test_rows_beside_one_of_huge_scores(TF, fmt, new, size):
+    """A row of huge or infinite queries does not harm the rows beside it (some of a warp may then be rounded in another order)."""
+    lens = [300, 40 + new]
+    for dim in (64, 128):
+        b = P.Batch(46, lens, [new, new], 1, dim, 16, fmt).fill(lens, (-9, -4))
+        Q = b.rand(b.rows, 4, dim, dtype=torch.bfloat16)
+        bad = Q.clone()
+        bad[1, 2] = size
+        bad[new + 2, 0] = -size
+        out = attend(TF, b, bad, 0.125, max_new=new).double()
+        want, bound = P.attention_rows(b, Q, 0.125)
+        for row, head in ((1, 2), (new + 2, 0)):
+            out[row, head] = want[row, head]
+        assert bool(((out - want).abs() <= bound + P.half_step(Q.dtype) * (want.abs() + bound)).all()) and int(b.flag) == 0
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("new", [1, 4, 140])
 def test_scales_that_are_no_powers_of_two(TF, fmt, new):
     """A cache that another program made: scales of any positive float, a few of them powers of two.  A scale may lie below its power of two
